@@ -1,0 +1,454 @@
+"""Cases for the sequence-layer operators of the public ops module: root-mean-square norm (with the residual's addition, its gradient
+and its 8-bit output), dropout from a counter-based generator, and linear attention with a decay for each head (whole sequences, their
+gradients, and single tokens).
+
+`listed()` and `draw()` give cases, `prepare()` their inputs on the GPU, `run()` one pass: in elementary torch operations where `own` is
+false, through pytorch_tecogan_amd.ops where it is true.  `exact()` states the same results in 64 bits, `work()` the bytes and
+operations that a pass cannot do without.
+
+Sizes: 64 / 128 channels and heads of 16 .. 64 channels are the generator's and discriminator's widths; 4 x 10 x 32 x 32 is one training
+batch of ten-frame LR clips, 40 x 128 x 128 its HR frames, 128 x 128 x 120 the long inference clip; a pixel's frames are one sequence, or a
+frame's pixels in raster order are."""
+import math
+
+import torch
+
+own = False
+
+DTYPES = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+EPS = 1e-6
+
+
+# ------------------------------------------------------------------------------------------------------------- cases
+def _norm(name, rows, channels, dtype, residual, mode):
+    return {"name": name, "op": "rms_norm", "rows": rows, "channels": channels, "dtype": dtype, "residual": residual, "mode": mode}
+
+
+def _drop(name, rows, channels, dtype, p, residual, train):
+    return {"name": name, "op": "dropout", "rows": rows, "channels": channels, "dtype": dtype, "p": p, "residual": residual,
+            "train": train}
+
+
+def _attn(name, batch, tokens, heads, kv_heads, dk, dv, dtype, mode, ragged=False, state=False, decay0=1, decay_step=1):
+    return {"name": name, "op": "linear_attention", "batch": batch, "tokens": tokens, "heads": heads, "kv_heads": kv_heads, "dk": dk,
+            "dv": dv, "dtype": dtype, "mode": mode, "ragged": ragged, "state": state, "decay0": decay0, "decay_step": decay_step}
+
+
+def listed():
+    return [
+        # one 32 x 32 LR frame of a live stream: the latency of a single call
+        _norm("norm_live_frame", 32 * 32, 64, "bf16", True, "forward"),
+        # a training batch of four ten-frame clips, forward and backward
+        _norm("norm_clip_train", 4 * 10 * 32 * 32, 64, "bf16", True, "train"),
+        # the HR frames of that batch, handed to an 8-bit consumer
+        _norm("norm_hr_e4m3", 40 * 128 * 128, 64, "bf16", True, "e4m3"),
+        # a wide odd-sized layer at the width of a flattened feature vector, half precision
+        _norm("norm_wide_odd_train", 4099, 1001, "f16", False, "train"),
+        # one LR frame's features, with the skip connection
+        _drop("dropout_live_frame", 32 * 32, 64, "f32", 0.1, True, False),
+        # HR features of a training batch, forward and backward
+        _drop("dropout_hr_train", 40 * 128 * 128, 64, "bf16", 0.25, True, True),
+        # single tokens: the next frame of a live 32 x 32 stream, each pixel a sequence
+        _attn("attn_step_live", 32 * 32, 1, 4, 4, 16, 16, "bf16", "step"),
+        # the next frame of a 128 x 128 stream
+        _attn("attn_step_frame", 128 * 128, 1, 4, 4, 16, 16, "bf16", "step"),
+        # ten-frame training clips, each pixel of four 32 x 32 clips a sequence
+        _attn("attn_clip_train", 4 * 32 * 32, 10, 4, 4, 16, 16, "bf16", "train"),
+        # the 120-frame inference clip at 128 x 128, each pixel a sequence
+        _attn("attn_seq120", 128 * 128, 120, 4, 4, 16, 16, "f16", "forward", decay0=2),
+        # a 128 x 128 frame's pixels in raster order as one long sequence, shared key / value heads, training
+        _attn("attn_raster_train", 2, 128 * 128, 4, 2, 64, 64, "bf16", "train", state=True, decay0=3, decay_step=2),
+        # a padded batch of clips of unequal length, odd head sizes, full precision
+        _attn("attn_ragged_train", 3, 777, 3, 3, 40, 56, "f32", "train", ragged=True, state=True, decay0=2, decay_step=2),
+    ]
+
+
+def _log_int(rng, lo, hi):
+    return min(hi, max(lo, int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))))
+
+
+def draw(rng):
+    op = rng.choice(["rms_norm", "dropout", "linear_attention", "linear_attention"])
+    dtype = rng.choice(["f32", "bf16", "f16"])
+    if op == "rms_norm":
+        channels = rng.choice([64, 128, _log_int(rng, 16, 4096)])
+        rows = _log_int(rng, 1, max(2, (1 << 24) // channels))
+        c = _norm("", rows, channels, dtype, rng.random() < 0.6, rng.choice(["forward", "train", "e4m3"]))
+    elif op == "dropout":
+        channels = rng.choice([64, 128, _log_int(rng, 16, 4096)])
+        rows = _log_int(rng, 1, max(2, (1 << 24) // channels))
+        c = _drop("", rows, channels, dtype, round(rng.uniform(0.02, 0.6), 3), rng.random() < 0.6, rng.random() < 0.5)
+    else:
+        mode = rng.choice(["forward", "train", "step"])
+        kv_heads = rng.choice([1, 2, 3, 4])
+        heads = kv_heads * rng.choice([1, 1, 2])
+        dk, dv = rng.choice([16, 32, 64, rng.randint(8, 128)]), rng.choice([16, 32, 64, rng.randint(8, 128)])
+        if mode == "step":
+            batch = _log_int(rng, 1, max(2, (1 << 22) // (heads * dk * dv)))
+            c = _attn("", batch, 1, heads, kv_heads, dk, dv, dtype, mode)
+        else:
+            tokens = _log_int(rng, 1, 8192)
+            batch = _log_int(rng, 1, max(2, (1 << 22) // (tokens * heads * max(dk, dv))))
+            c = _attn("", batch, tokens, heads, kv_heads, dk, dv, dtype, mode, ragged=rng.random() < 0.4, state=rng.random() < 0.5,
+                      decay0=rng.randint(1, 4), decay_step=rng.randint(1, 2))
+    del c["name"]
+    return c
+
+
+# ------------------------------------------------------------------------------------------------------------- inputs
+def _device():
+    return torch.device("cuda", torch.cuda.current_device())
+
+
+def _log_decay(case, dev):
+    """-2^-(decay0 + decay_step h): from a memory of a few tokens to one of thousands"""
+    return torch.tensor([-2.0 ** -(case["decay0"] + case["decay_step"] * h) for h in range(case["heads"])], dtype=torch.float32, device=dev)
+
+
+def prepare(case, seed):
+    dev = _device()
+    gen = torch.Generator(device=dev)
+    gen.manual_seed(seed)
+    dt = DTYPES[case["dtype"]]
+
+    def normal(*shape, dtype=dt):
+        return torch.randn(*shape, device=dev, generator=gen, dtype=torch.float32).to(dtype)
+
+    s = {"case": case}
+    if case["op"] in ("rms_norm", "dropout"):
+        shape = (case["rows"], case["channels"])
+        s["x"] = normal(*shape)
+        s["residual"] = normal(*shape) if case["residual"] else None
+        if case["op"] == "rms_norm":
+            s["weight"] = 1.0 + 0.1 * torch.randn(case["channels"], device=dev, generator=gen)
+            if case["mode"] == "train":
+                s["dy"] = normal(*shape)
+                s["ds"] = normal(*shape) if case["residual"] else None
+        else:
+            s["rng"] = torch.tensor([seed * 2654435761 + 12345, seed % 1000], dtype=torch.int64, device=dev)   # (seed, step)
+            s["layer"] = seed % 7
+            if case["train"]:
+                s["dy"] = normal(*shape)
+        return s
+    B, T, H, HK, DK, DV = (case[k] for k in ("batch", "tokens", "heads", "kv_heads", "dk", "dv"))
+    s["log_decay"] = _log_decay(case, dev)
+    if case["mode"] == "step":
+        s["q"], s["k"], s["v"] = normal(B, H, DK), normal(B, HK, DK), normal(B, HK, DV)
+        s["state"] = normal(B, H, DK, DV, dtype=torch.float32)
+        return s
+    s["q"], s["k"], s["v"] = normal(B, T, H, DK), normal(B, T, HK, DK), normal(B, T, HK, DV)
+    s["state"] = normal(B, H, DK, DV, dtype=torch.float32) if case["state"] else None
+    s["lengths"] = None
+    if case["ragged"]:
+        u = torch.rand(B, device=dev, generator=gen)
+        s["lengths"] = (T - (u * (T // 2 + 1)).floor()).to(torch.int32)
+    if case["mode"] == "train":
+        s["do"] = normal(B, T, H, DV)
+        s["dstate"] = normal(B, H, DK, DV, dtype=torch.float32) if case["state"] else None
+    return s
+
+
+# --------------------------------------------------------------------------------------------------------- plain forms
+def _plain_norm(s):
+    case, x = s["case"], s["x"]
+    f = x.float() if s["residual"] is None else x.float() + s["residual"].float()
+    rstd = torch.rsqrt((f * f).mean(dim=1, keepdim=True) + EPS)
+    xhat = f * rstd
+    y = xhat * s["weight"]
+    out = {} if s["residual"] is None else {"s": f.to(x.dtype)}
+    if case["mode"] == "e4m3":
+        scale = y.abs().amax(dim=1, keepdim=True).clamp_min(2.0 ** -100) / 448.0
+        out.update(q=(y / scale).to(torch.float8_e4m3fn), scale=scale[:, 0])
+        return out
+    out["y"] = y.to(x.dtype)
+    if case["mode"] == "train":
+        dy = s["dy"].float()
+        g = dy * s["weight"]
+        dx = rstd * (g - xhat * (g * xhat).mean(dim=1, keepdim=True))
+        if s["ds"] is not None:
+            dx = dx + s["ds"].float()
+        out.update(dx=dx.to(x.dtype), dweight=(dy * xhat).sum(dim=0))
+    return out
+
+
+def _mul32(x, m):
+    """(high, low) 32 bits of x * m for x < 2^32 held in int64: two 16-bit halves of m, so that no product passes 2^48"""
+    a = x * (m & 0xffff)
+    b = x * (m >> 16) + (a >> 16)
+    return b >> 16, ((b & 0xffff) << 16) | (a & 0xffff)
+
+
+def _philox_keep(n, p, rng, layer):
+    """keep[i] of the elements 0 .. n - 1: word i % 4 of Philox4x32-10 (Salmon, Moraes, Dror, Shaw 2011) at the counter
+    (i / 4 low, i / 4 high, layer, step) under the key `seed`, against p 2^32"""
+    seed, step = rng[0], rng[1] & 0xffffffff
+    k0, k1 = seed & 0xffffffff, (seed >> 32) & 0xffffffff
+    block = torch.arange((n + 3) // 4, dtype=torch.int64, device=rng.device)
+    c = [block & 0xffffffff, block >> 32, torch.full_like(block, layer), step.expand_as(block)]
+
+    def once(c, k0, k1):
+        h0, l0 = _mul32(c[0], 0xD2511F53)
+        h1, l1 = _mul32(c[2], 0xCD9E8D57)
+        return [h1 ^ c[1] ^ k0, l1, h0 ^ c[3] ^ k1, l0], (k0 + 0x9E3779B9) & 0xffffffff, (k1 + 0xBB67AE85) & 0xffffffff
+
+    for _ in range(10):
+        c, k0, k1 = once(c, k0, k1)
+    words = torch.stack(c, dim=1).reshape(-1)[:n]
+    return words >= int(math.floor(p * 2.0 ** 32 + 0.5))
+
+
+def _plain_dropout(s):
+    case, x = s["case"], s["x"]
+    keep = _philox_keep(x.numel(), case["p"], s["rng"], s["layer"]).view_as(x)
+    up = 1.0 / (1.0 - case["p"])
+    y = torch.where(keep, x.float() * up, torch.zeros((), device=x.device))
+    if s["residual"] is not None:
+        y = y + s["residual"].float()
+    out = {"y": y.to(x.dtype)}
+    if case["train"]:
+        out["dx"] = torch.where(keep, s["dy"].float() * up, torch.zeros((), device=x.device)).to(x.dtype)
+    return out
+
+
+def _chunked(q, k, v, log_decay, state, lengths, scale):
+    """float (B, T, H, D) tensors -> (o, final state): chunks of 64 tokens, inside a chunk the masked product of queries and keys, between
+    chunks the sum of key-value products weighted by the decay.  The decays' angles are taken in 64 bits."""
+    B, T, H, DK = q.shape
+    DV, L = v.shape[3], 64 if T > 16 else 16
+    NC = (T + L - 1) // L
+    dev = q.device
+    a = log_decay.double()
+
+    def chunks(x):
+        x = torch.nn.functional.pad(x, (0, 0, 0, 0, 0, NC * L - T))
+        return x.view(B, NC, L, H, x.shape[3]).permute(0, 3, 1, 2, 4).contiguous()
+
+    n = torch.full((B,), T, device=dev, dtype=torch.int64) if lengths is None else lengths.long()
+    live = (torch.arange(T, device=dev)[None, :] < n[:, None])[:, :, None, None]
+    zero = torch.zeros((), device=dev)
+    q, k, v = torch.where(live, q, zero), torch.where(live, k, zero), torch.where(live, v, zero)
+    qc, kc, vc = chunks(q), chunks(k), chunks(v)
+    i = torch.arange(L, device=dev, dtype=torch.float64)
+    gap = i[:, None] - i[None, :]
+    inside = torch.where(gap >= 0, torch.exp(a[:, None, None] * gap.clamp_min(0)), 0.0).float()
+    o = ((qc @ kc.transpose(3, 4)) * inside[None, :, None]) @ vc
+    kv = (kc * torch.exp(a[:, None] * (L - 1 - i)).float()[None, :, None, :, None]).transpose(3, 4) @ vc          # (B, H, NC, DK, DV)
+    c = torch.arange(NC, device=dev, dtype=torch.float64)
+    gap = c[:, None] - 1 - c[None, :]
+    between = torch.where(gap >= 0, torch.exp(a[:, None, None] * L * gap.clamp_min(0)), 0.0).float()
+    before = (between @ kv.reshape(B, H, NC, DK * DV)).view(B, H, NC, DK, DV)
+    if state is not None:
+        before = before + torch.exp(a[:, None] * L * c).float()[None, :, :, None, None] * state[:, :, None]
+    o = o + torch.exp(a[:, None] * (i + 1)).float()[None, :, None, :, None] * (qc @ before)
+    o = (scale * o).permute(0, 2, 3, 1, 4).reshape(B, NC * L, H, DV)[:, :T]
+    t = torch.arange(T, device=dev, dtype=torch.float64)
+    left = n.double()[:, None] - 1 - t[None, :]                                                                     # (B, T)
+    w = torch.where(left[:, :, None] >= 0, torch.exp(a * left.clamp_min(0)[:, :, None]), 0.0).float()              # (B, T, H)
+    final = (k * w[..., None]).permute(0, 2, 3, 1).contiguous() @ v.permute(0, 2, 1, 3).contiguous()
+    if state is not None:
+        final = final + torch.exp(a * n.double()[:, None]).float()[:, :, None, None] * state
+    return o, final
+
+
+def _plain_attention(s):
+    case, dt = s["case"], s["q"].dtype
+    G, scale = case["heads"] // case["kv_heads"], case["dk"] ** -0.5
+    if case["mode"] == "step":
+        q, k, v = s["q"].float(), s["k"].float().repeat_interleave(G, 1), s["v"].float().repeat_interleave(G, 1)
+        s["state"].mul_(torch.exp(s["log_decay"])[:, None, None]).add_(k[..., None] * v[..., None, :])
+        return {"o": (scale * (q[..., None, :] @ s["state"])[..., 0, :]).to(dt), "state": s["state"]}
+    train = case["mode"] == "train"
+    leaf = [s[n].float() for n in ("q", "k", "v")] + ([s["state"].clone()] if case["state"] else [])
+    with torch.set_grad_enabled(train):
+        for x in leaf:
+            x.requires_grad_(train)
+        q, k, v = leaf[0], leaf[1].repeat_interleave(G, 2), leaf[2].repeat_interleave(G, 2)
+        o, final = _chunked(q, k, v, s["log_decay"], leaf[3] if case["state"] else None, s["lengths"], scale)
+        out = {"o": o.detach().to(dt), "state": final.detach()}
+        if train:
+            to, seed = ([o, final], [s["do"].float(), s["dstate"]]) if case["state"] else ([o], [s["do"].float()])
+            g = torch.autograd.grad(to, leaf, seed)
+            out.update(dq=g[0].to(dt), dk=g[1].to(dt), dv=g[2].to(dt))
+            if case["state"]:
+                out["dstate"] = g[3]
+    return out
+
+
+# ------------------------------------------------------------------------------------------------------- the framework
+def _own(s):
+    from pytorch_tecogan_amd import ops
+    case = s["case"]
+    if case["op"] == "rms_norm":
+        if case["mode"] == "e4m3":
+            r = ops.rms_norm_e4m3(s["x"], s["weight"], residual=s["residual"], eps=EPS)
+            return dict(zip(("q", "scale", "s"), r))
+        if case["mode"] == "forward":
+            r = ops.rms_norm(s["x"], s["weight"], residual=s["residual"], eps=EPS)
+            return {"y": r} if s["residual"] is None else {"y": r[0], "s": r[1]}
+        r = ops.rms_norm(s["x"], s["weight"], residual=s["residual"], eps=EPS, stats=True)
+        total = s["x"] if s["residual"] is None else r[1]
+        dx, dweight = ops.rms_norm_backward(s["dy"], total, r[-1], s["weight"], ds=s["ds"])
+        out = {"y": r[0], "dx": dx, "dweight": dweight}
+        return out if s["residual"] is None else dict(out, s=total)
+    if case["op"] == "dropout":
+        out = {"y": ops.dropout(s["x"], case["p"], s["rng"], layer=s["layer"], residual=s["residual"])}
+        if case["train"]:
+            out["dx"] = ops.dropout_backward(s["dy"], case["p"], s["rng"], layer=s["layer"])
+        return out
+    if case["mode"] == "step":
+        return {"o": ops.linear_attention_step(s["q"], s["k"], s["v"], s["log_decay"], s["state"]), "state": s["state"]}
+    o, final = ops.linear_attention(s["q"], s["k"], s["v"], s["log_decay"], state=s["state"], lengths=s["lengths"])
+    out = {"o": o, "state": final}
+    if case["mode"] == "train":
+        dq, dk, dv, dstate = ops.linear_attention_backward(s["do"], s["q"], s["k"], s["v"], s["log_decay"], state=s["state"],
+                                                           lengths=s["lengths"], dstate=s["dstate"])
+        out.update(dq=dq, dk=dk, dv=dv)
+        if case["state"]:
+            out["dstate"] = dstate
+    return out
+
+
+def run(state):
+    if own:
+        return _own(state)
+    return {"rms_norm": _plain_norm, "dropout": _plain_dropout, "linear_attention": _plain_attention}[state["case"]["op"]](state)
+
+
+# ---------------------------------------------------------------------------------------------------------------- work
+def work(case):
+    size = 4 if case["dtype"] == "f32" else 2
+    if case["op"] in ("rms_norm", "dropout"):
+        n, rows, C = case["rows"] * case["channels"], case["rows"], case["channels"]
+        r = 1 if case["residual"] else 0
+        if case["op"] == "rms_norm":
+            if case["mode"] == "e4m3":
+                return {"bytes": n * size * (1 + 2 * r) + n + 4 * rows + 4 * C, "flops": 6 * n}
+            if case["mode"] == "forward":
+                return {"bytes": n * size * (2 + 2 * r) + 4 * C, "flops": 5 * n}
+            # x (and residual, ds), dy in; y (and s), dx out; the sum is not read again
+            return {"bytes": n * size * (4 + 3 * r) + 8 * C, "flops": 15 * n}
+        # a generator call is 10 rounds of two 32 x 32 products and four exclusive-ors for four elements
+        t = 2 if case["train"] else 1
+        return {"bytes": n * size * (2 * t + r), "flops": n * (15 + 2 * t)}
+    B, T, H, HK, DK, DV = (case[k] for k in ("batch", "tokens", "heads", "kv_heads", "dk", "dv"))
+    rows = B * T * (0.75 if case["ragged"] else 1.0)
+    qo, kv, st = rows * H * (DK + DV) * size, rows * HK * (DK + DV) * size, B * H * DK * DV * 4
+    if case["mode"] == "step":
+        return {"bytes": qo + kv + 2 * st, "flops": 5 * B * H * DK * DV}
+    states = st * (2 if case["state"] else 1)
+    if case["mode"] == "forward":
+        return {"bytes": qo + kv + states, "flops": int(rows * H * 5 * DK * DV)}
+    # q, k, v, do in; o, dq, dk, dv out; the recurrences of the state and of its gradient, and a product for each of o, dq, dk, dv
+    return {"bytes": 2 * (qo + kv) + 2 * states, "flops": int(rows * H * 14 * DK * DV)}
+
+
+# --------------------------------------------------------------------------------------------------------------- exact
+def _exact_norm(s):
+    case, x = s["case"], s["x"].double()
+    if s["residual"] is not None:
+        x = x + s["residual"].double()
+    w, C = s["weight"].double(), case["channels"]
+    ms = torch.einsum("rc,rc->r", x, x) / C + EPS
+    y = x * w / ms.sqrt()[:, None]
+    out = {} if s["residual"] is None else {"s": x}
+    if case["mode"] == "e4m3":
+        scale = torch.maximum(y.max(dim=1).values, -y.min(dim=1).values).clamp_min(2.0 ** -100) / 448.0
+        return dict(out, q=y / scale[:, None], scale=scale)
+    out["y"] = y
+    if case["mode"] == "train":
+        dy = s["dy"].double()
+        dx = dy * w / ms.sqrt()[:, None] - x * (torch.einsum("rc,rc,c->r", dy, x, w) / (C * ms * ms.sqrt()))[:, None]
+        out["dx"] = dx if s["ds"] is None else dx + s["ds"].double()
+        out["dweight"] = torch.einsum("rc,rc,r->c", dy, x, 1.0 / ms.sqrt())
+    return out
+
+
+def _exact_keep(n, p, rng, layer):
+    """the same mask on the host: numpy's unsigned 64-bit products"""
+    import numpy as np
+    seed, step = (int(v) for v in rng.cpu())
+    seed &= 0xffffffffffffffff
+    low = np.uint64(0xffffffff)
+    block = np.arange((n + 3) // 4, dtype=np.uint64)
+    x = [block & low, block >> np.uint64(32), np.full_like(block, layer), np.full_like(block, step & 0xffffffff)]
+    ka, kb = seed & 0xffffffff, seed >> 32
+    for r in range(10):
+        left, right = x[0] * np.uint64(0xD2511F53), x[2] * np.uint64(0xCD9E8D57)
+        x = [(right >> np.uint64(32)) ^ x[1] ^ np.uint64((ka + r * 0x9E3779B9) & 0xffffffff), right & low,
+             (left >> np.uint64(32)) ^ x[3] ^ np.uint64((kb + r * 0xBB67AE85) & 0xffffffff), left & low]
+    keep = np.stack(x, axis=1).reshape(-1)[:n].astype(np.float64) / 2.0 ** 32 >= math.floor(p * 2.0 ** 32 + 0.5) / 2.0 ** 32
+    return torch.from_numpy(keep).to(rng.device)
+
+
+def _exact_dropout(s):
+    case, x = s["case"], s["x"].double()
+    keep = _exact_keep(x.numel(), case["p"], s["rng"], s["layer"]).view_as(x).double()
+    y = x * keep / (1.0 - case["p"])
+    out = {"y": y if s["residual"] is None else y + s["residual"].double()}
+    if case["train"]:
+        out["dx"] = s["dy"].double() * keep / (1.0 - case["p"])
+    return out
+
+
+def _exact_attention(s):
+    """the sums over pairs of tokens as they stand, 256 query rows at a time"""
+    case = s["case"]
+    B, T, H, HK, DK, DV = (case[k] for k in ("batch", "tokens", "heads", "kv_heads", "dk", "dv"))
+    a, scale, dev = s["log_decay"].double(), DK ** -0.5, s["q"].device
+    head = torch.arange(H, device=dev) // (H // HK)
+    if case["mode"] == "step":
+        q, k, v = s["q"].double(), s["k"].double()[:, head], s["v"].double()[:, head]
+        state = s["state"].double() * a.exp()[:, None, None] + torch.einsum("bhm,bhn->bhmn", k, v)
+        return {"o": scale * torch.einsum("bhm,bhmn->bhn", q, state), "state": state}
+    rows = 256 if T > 256 else T
+    heads_first = lambda x: x.double().permute(0, 2, 1, 3).contiguous()   # noqa: E731
+    q, k, v = heads_first(s["q"]), heads_first(s["k"])[:, head].contiguous(), heads_first(s["v"])[:, head].contiguous()
+    n = torch.full((B,), T, device=dev) if s["lengths"] is None else s["lengths"].long()
+    t = torch.arange(T, device=dev)
+    live = (t[None] < n[:, None]).double()[:, None, :, None]
+    q, k, v = q * live, k * live, v * live
+    train = case["mode"] == "train"
+    do = heads_first(s["do"]) * live if train else None
+    o = torch.zeros(B, H, T, DV, dtype=torch.float64, device=dev)
+    dq, dk, dv = torch.zeros_like(q), torch.zeros_like(k), torch.zeros_like(v)
+    for i0 in range(0, T, rows):
+        i = t[i0:i0 + rows]
+        e = min(T, i0 + rows)
+        gap = (i[:, None] - t[None, :e]).double()
+        w = torch.exp(a[:, None, None] * gap.clamp_min(0)) * (gap >= 0) * scale
+        score = (q[:, :, i0:e] @ k[:, :, :e].transpose(2, 3)) * w
+        o[:, :, i0:e] = score @ v[:, :, :e]
+        if train:
+            dscore = (do[:, :, i0:e] @ v[:, :, :e].transpose(2, 3)) * w
+            dq[:, :, i0:e] = dscore @ k[:, :, :e]
+            dk[:, :, :e] += dscore.transpose(2, 3) @ q[:, :, i0:e]
+            dv[:, :, :e] += score.transpose(2, 3) @ do[:, :, i0:e]
+    since = torch.exp(a[None, :, None] * (t + 1.0)[None, None]).expand(B, H, T)[..., None]                  # decay of the first state at t
+    left = torch.exp(a[None, :, None] * (n[:, None] - 1 - t[None]).clamp_min(0).double()[:, None])[..., None] * live   # decay from t to the end
+    last = torch.exp(a[None] * n.double()[:, None])[..., None, None]
+    final = (k * left).transpose(2, 3) @ v
+    out = {"o": None, "state": final}
+    if case["state"]:
+        S0 = s["state"].double()
+        o = o + scale * (q * since) @ S0
+        out["state"] = final + last * S0
+        if train:
+            dS = s["dstate"].double()
+            dq = dq + scale * since * (do @ S0.transpose(2, 3))
+            dk = dk + left * (v @ dS.transpose(2, 3))
+            dv = dv + left * (k @ dS)
+            out["dstate"] = last * dS + scale * (q * since).transpose(2, 3) @ do
+    back = lambda x: x.permute(0, 2, 1, 3).contiguous()   # noqa: E731
+    share = lambda x: x.view(B, HK, H // HK, T, x.shape[3]).sum(dim=2)   # noqa: E731
+    out["o"] = back(o)
+    if train:
+        out.update(dq=back(dq), dk=back(share(dk)), dv=back(share(dv)))
+    return out
+
+
+def exact(case, seed):
+    if case["op"] == "linear_attention" and case["mode"] != "step" and \
+            case["batch"] * case["heads"] * case["tokens"] ** 2 * (case["dk"] + case["dv"]) > 2e12:
+        return None   # (minutes of 64-bit products)
+    s = prepare(case, seed)
+    return {"rms_norm": _exact_norm, "dropout": _exact_dropout, "linear_attention": _exact_attention}[case["op"]](s)
