@@ -286,10 +286,9 @@ def _own(s):
             r = ops.rms_norm(s["x"], s["weight"], residual=s["residual"], eps=EPS)
             return {"y": r} if s["residual"] is None else {"y": r[0], "s": r[1]}
         r = ops.rms_norm(s["x"], s["weight"], residual=s["residual"], eps=EPS, stats=True)
-        total = s["x"] if s["residual"] is None else r[1]
-        dx, dweight = ops.rms_norm_backward(s["dy"], total, r[-1], s["weight"], ds=s["ds"])
+        dx, dweight = ops.rms_norm_backward(s["dy"], s["x"], r[-1], s["weight"], residual=s["residual"], ds=s["ds"])
         out = {"y": r[0], "dx": dx, "dweight": dweight}
-        return out if s["residual"] is None else dict(out, s=total)
+        return out if s["residual"] is None else dict(out, s=r[1])
     if case["op"] == "dropout":
         out = {"y": ops.dropout(s["x"], case["p"], s["rng"], layer=s["layer"], residual=s["residual"])}
         if case["train"]:
