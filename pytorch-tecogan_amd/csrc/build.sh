@@ -22,13 +22,15 @@ fi
 pids=""
 # -amdgpu-kernarg-preload-count: kernels whose arguments are passed one by one (everything but the by-value launch structs) get their
 # first 16 dwords preloaded into SGPRs with the wave - no s_load round trip in front of a workgroup's first address (r05_k log)
-FLAGS="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -Wall -Wno-unused-function -mllvm -amdgpu-kernarg-preload-count=16 $EXTRA"
+# -packed-fp32-ops: no v_pk_add_f32 / v_pk_mul_f32 / v_pk_fma_f32 (some of their forms have given wrong results on this hardware now and
+# then); the host pass of each compile says that it does not know the feature
+FLAGS="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -Wall -Wno-unused-function -mllvm -amdgpu-kernarg-preload-count=16 -Xclang -target-feature -Xclang -packed-fp32-ops $EXTRA"
 objs=""
 for f in $SRCS; do
   o=$OBJ/$f.o
   objs="$objs $o"
   src=$f.hip; [ -f $src ] || src=exp/$f.hip   # (the rejected variants' sources live under exp/, next to the experiments build's objects)
-  if [ ! -f $o ] || [ $src -nt $o ] || [ common.h -nt $o ] || [ rbw_common.h -nt $o ] || [ ../../include/tecogan_hip.h -nt $o ]; then
+  if [ ! -f $o ] || [ $src -nt $o ] || [ common.h -nt $o ] || [ rbw_common.h -nt $o ] || [ build.sh -nt $o ] || [ ../../include/tecogan_hip.h -nt $o ]; then
     rm -f $o   # a failed compile must not leave the previous object behind for the link below
     # conv3_rw: the producer waves' epilogue arithmetic shares a SIMD with the consumer's MFMA stream; SLP-packed f32 operations
     # (v_pk_add_f32 / v_pk_mul_f32) cost ~+25 cycles each beside MFMAs (MI355X_MICROARCH.md, 'price of one filler')
