@@ -564,6 +564,52 @@ int tg_resample_u8(const void* frames_u8, void* tmp_u8, float* out_nchw, const i
                    int ksize_w, const int32_t* bounds_h, const int32_t* kk_h, int ksize_h, int N, int H, int W, int OH,
                    int OW, void* stream);
 
+/* ---- sequence layers: norm, dropout and linear attention beside the batch norm and the activations above -------------------------
+ * No reference counterpart (the reference's layers end at code/ops.py:45-88); additions only, so the ABI version stays.  Tensors are
+ * row-major with the channel dimension contiguous, TG_F32 / TG_BF16 / TG_F16, any size and alignment of the element type (16-byte
+ * aligned pointers and strides take the wide loads); strides are in ELEMENTS.  No float atomics: the same call gives the same bits.
+ *
+ * tg_rms_norm: s = x + res (res may be null: s = x), y = s * rstd * weight, rstd = 1 / sqrt(mean_c s^2 + eps), per row of C channels;
+ *   weight [C] fp32 or null (ones); x, res rows at x_stride, res_stride; y, s [rows][C] contiguous; s (null: not stored; written only with
+ *   res) is rounded to the element type, y is computed from the unrounded sum; rstd [rows] or null.
+ * tg_rms_norm_e4m3: q [rows][C] = e4m3(y / scale[row]), scale[row] = max(max_c |y|, 2^-100) / 448.  A NaN in a row makes its scale NaN.
+ * tg_rms_norm_bwd: dx = rstd (g - xhat mean_c(g xhat)) (+ ds), g = dy weight, xhat = (x + res) rstd; dweight [C] (null: not wanted) =
+ *   sum_rows dy xhat, through `scratch` of tg_rms_norm_bwd_scratch_floats floats. */
+int tg_rms_norm(int dtype, const void* x, int64_t x_stride, const void* res, int64_t res_stride, const float* weight, void* y, void* s,
+                float* rstd, int64_t rows, int C, float eps, void* stream);
+int tg_rms_norm_e4m3(int dtype, const void* x, int64_t x_stride, const void* res, int64_t res_stride, const float* weight, void* q,
+                     float* scale, void* s, int64_t rows, int C, float eps, void* stream);
+int64_t tg_rms_norm_bwd_scratch_floats(int64_t rows, int C);
+int tg_rms_norm_bwd(int dtype, const void* dy, int64_t dy_stride, const void* x, int64_t x_stride, const void* res, int64_t res_stride,
+                    const float* rstd, const float* weight, const void* ds, int64_t ds_stride, void* dx, float* dweight, float* scratch,
+                    int64_t rows, int C, void* stream);
+
+/* y[i] = (res ? res[i] : 0) + (keep_i ? x[i] / (1 - p) : 0), i < n contiguous elements, 0 <= p < 1.  keep_i: word i % 4 of Philox4x32-10 at the
+ * counter (i / 4 low, i / 4 high, layer, step) under the key seed is >= round(p 2^32); rng = {seed, step} int64 in DEVICE memory (the
+ * step's low 32 bits count).  The gradient is the same call on dy without res. */
+int tg_dropout(int dtype, const void* x, const void* res, void* y, int64_t n, double p, const int64_t* rng, int layer, void* stream);
+
+/* S_t = exp(log_decay[h]) S_{t-1} + k_t v_t^T, o_t = scale q_t S_t per sequence and head; q [B][T][H][DK], k [B][T][HK][DK], v [B][T][HK][DV]
+ * at the given strides of (sequence, token, head), H % HK == 0: head h reads stored head h / (H / HK); 1 <= DK, DV <= 128.
+ * Outputs o, dq [B][T][H][..], dk, dv [B][T][HK][..] are contiguous; states [B][H][DK][DV] fp32; lengths [B] int32 or null: tokens at and
+ * behind lengths[b] (clamped to 0 .. T) are not read, their rows of the outputs are zero and the last state is the one at the length.
+ * state_in null: zeros.  tg_linear_attention_bwd: dstate_out null: zeros; dstate_in may be null; scratch:
+ * tg_linear_attention_bwd_scratch_floats floats (0: null).  log_decay is a constant (no gradient).
+ * tg_linear_attention_step: one token (strides of sequence and head; T and the token stride are not looked at), `state` updated in place. */
+typedef struct {
+  int32_t B, T, H, HK, DK, DV;
+  int64_t q_stride[3], k_stride[3], v_stride[3];   /* sequence, token, head */
+  float scale;
+} tg_la_desc;
+int tg_linear_attention(int dtype, const tg_la_desc* d, const void* q, const void* k, const void* v, const float* log_decay,
+                        const int32_t* lengths, const float* state_in, void* o, float* state_out, void* stream);
+int64_t tg_linear_attention_bwd_scratch_floats(const tg_la_desc* d);
+int tg_linear_attention_bwd(int dtype, const tg_la_desc* d, const void* q, const void* k, const void* v, const void* dout,
+                            const int64_t* dout_stride, const float* log_decay, const int32_t* lengths, const float* state_in,
+                            const float* dstate_out, void* dq, void* dk, void* dv, float* dstate_in, float* scratch, void* stream);
+int tg_linear_attention_step(int dtype, const tg_la_desc* d, const void* q, const void* k, const void* v, const float* log_decay, void* o,
+                             float* state, void* stream);
+
 /* ---- step schedule support (no reference counterpart: the reference runs everything on one CUDA stream) ------- */
 /* Creates a stream confined to every CU except the first `reserve_cus` CU-mask bits (hipExtStreamCreateWithCUMask; 64 bits
  * = 8 CUs on each of the 8 XCDs of an MI355X).  The dense lane of the step runs there, so that the generator chain's

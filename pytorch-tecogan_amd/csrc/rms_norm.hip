@@ -1,0 +1,492 @@
+// Root-mean-square norm over the last dimension, with the residual's addition in front of it, its gradient, and an 8-bit output.
+//
+//   s = x + r          y = s * rstd * w          rstd = 1 / sqrt(mean_c s^2 + eps)
+//   e4m3:  scale = max(max_c |y|, 2^-100) / 448,  q = e4m3(y / scale)            (448: the largest e4m3 value)
+//   backward, g = dy * w, xhat = s * rstd:
+//          dx = rstd * (g - xhat * mean_c(g * xhat)) + ds                       (the gradient of x and of r alike)
+//          dw = sum over rows of dy * xhat
+//
+// One pass: a row lives in the registers of L lanes (8 .. 64 of a wave, or the 256 of a workgroup), 16 bytes per load where C, the
+// strides and the pointers allow it and one element per load otherwise; longer rows are read again for each pass over them.  The sum
+// of squares, the row's maximum and dw are held in 32 bits.  y is computed from the UNROUNDED sum, so storing s in 16 bits costs y
+// nothing, and the backward pass adds x and r again for the same reason (dw from a 16-bit s would be off by 2^-9 of each term: 1.6e-3 of
+// the sum instead of 1e-7, for one operand less to read).  dw: every workgroup adds the rows it walks in registers and writes one partial row,
+// a second launch adds those in index order - no atomics, the same bits every time.
+#include "common.h"
+
+namespace {
+
+template <typename T, int W> struct Row {   // W consecutive elements as floats
+  __device__ __forceinline__ static void load(const void* p, int64_t i, float* v) {
+    if constexpr (W == 1) v[0] = load_elem<T>(p, i);
+    else Vec<T>::load(reinterpret_cast<const char*>(p) + i * ElemTraits<T>::kBytes, v);
+  }
+  __device__ __forceinline__ static void store(void* p, int64_t i, const float* v) {
+    if constexpr (W == 1) store_elem<T>(p, i, v[0]);
+    else Vec<T>::store(reinterpret_cast<char*>(p) + i * ElemTraits<T>::kBytes, v);
+  }
+};
+
+template <int W> __device__ __forceinline__ void load_f32(const float* p, int i, float* v) {
+  if constexpr (W == 1) v[0] = p[i];
+  else
+#pragma unroll
+    for (int k = 0; k < W; k += 4) Vec<F32>::load(p + i + k, v + k);
+}
+
+// W floats -> W e4m3 bytes (v_cvt_pk_fp8_f32: round to nearest even; |v| <= 448 up to one rounding by construction, NaN stays NaN)
+template <int W> __device__ __forceinline__ void store_e4m3(unsigned char* p, const float* v) {
+  if constexpr (W == 1) {
+    p[0] = (unsigned char)(__builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[0], 0, false) & 0xff);
+  } else {
+    int d[W / 4];
+#pragma unroll
+    for (int k = 0; k < W / 4; ++k) {
+      d[k] = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * k], v[4 * k + 1], 0, false);
+      d[k] = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * k + 2], v[4 * k + 3], d[k], true);
+    }
+    if constexpr (W == 8) *reinterpret_cast<int2*>(p) = make_int2(d[0], d[1]);
+    else *reinterpret_cast<int*>(p) = d[0];
+  }
+}
+
+// sum / maximum over the L lanes of a row; every lane gets it.  L = 256: the whole workgroup (red: 4 floats of LDS)
+template <int L> __device__ __forceinline__ float row_sum(float v, float* red) {
+#pragma unroll
+  for (int o = (L < 64 ? L : 64) / 2; o; o >>= 1) v += __shfl_xor(v, o, 64);
+  if constexpr (L > 64) {
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = (red[0] + red[1]) + (red[2] + red[3]);
+  }
+  return v;
+}
+// of the BITS of non-negative floats: their order is the integers', and a NaN is above everything, so it reaches the scale
+template <int L> __device__ __forceinline__ unsigned row_max(unsigned v, unsigned* red) {
+#pragma unroll
+  for (int o = (L < 64 ? L : 64) / 2; o; o >>= 1) v = max(v, (unsigned)__shfl_xor((int)v, o, 64));
+  if constexpr (L > 64) {
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = max(max(red[0], red[1]), max(red[2], red[3]));
+  }
+  return v;
+}
+// the floor keeps 1 / scale finite; a row whose largest |y| is below 2^-100 (an all-zero row above all) gets that scale
+__device__ __forceinline__ float e4m3_scale(unsigned amax_bits) {
+  const unsigned lo = 0x0d800000u;   // 2^-100
+  return __uint_as_float(max(amax_bits, lo)) / 448.f;
+}
+__device__ __forceinline__ unsigned abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+
+struct FwdArgs {
+  const void *x, *res;
+  const float* w;
+  void *y, *s;          // y: T rows, or e4m3 bytes
+  float *rstd, *scale;
+  int64_t xs, rs, rows; // row strides of x and res (elements)
+  int C;
+  float eps;
+};
+
+template <typename T, int W, int L, int NV, bool Q8> __global__ __launch_bounds__(256) void rms_fwd_kernel(FwdArgs a) {
+  __shared__ float red[4];
+  const int li = threadIdx.x & (L - 1);
+  const int64_t rpb = 256 / L;
+  const float inv_c = 1.f / (float)a.C;
+  for (int64_t row = (int64_t)blockIdx.x * rpb + threadIdx.x / L; ; row += (int64_t)gridDim.x * rpb) {
+    if (row - threadIdx.x / L >= a.rows) break;   // the whole workgroup leaves together
+    const bool live = row < a.rows;
+    float v[NV][W];
+    float ss = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int e = (li + L * i) * W;
+#pragma unroll
+      for (int k = 0; k < W; ++k) v[i][k] = 0.f;
+      if (live && e < a.C) {
+        Row<T, W>::load(a.x, row * a.xs + e, v[i]);
+        if (a.res) {
+          float r[W];
+          Row<T, W>::load(a.res, row * a.rs + e, r);
+#pragma unroll
+          for (int k = 0; k < W; ++k) v[i][k] += r[k];
+          if (a.s) Row<T, W>::store(a.s, row * a.C + e, v[i]);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < W; ++k) ss = fmaf(v[i][k], v[i][k], ss);
+    }
+    const float rstd = 1.f / sqrtf(row_sum<L>(ss, red) * inv_c + a.eps);
+    if (a.rstd && live && li == 0) a.rstd[row] = rstd;
+    unsigned amax = 0;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int e = (li + L * i) * W;
+      float w[W];
+#pragma unroll
+      for (int k = 0; k < W; ++k) w[k] = 1.f;
+      if (a.w && e < a.C) load_f32<W>(a.w, e, w);
+#pragma unroll
+      for (int k = 0; k < W; ++k) v[i][k] = v[i][k] * rstd * w[k];
+      if constexpr (Q8) {
+#pragma unroll
+        for (int k = 0; k < W; ++k) amax = max(amax, e < a.C ? abs_bits(v[i][k]) : 0u);
+      } else {
+        if (live && e < a.C) Row<T, W>::store(a.y, row * a.C + e, v[i]);
+      }
+    }
+    if constexpr (Q8) {
+      const float scale = e4m3_scale(row_max<L>(amax, reinterpret_cast<unsigned*>(red)));
+      const float inv = 1.f / scale;
+      if (live && li == 0) a.scale[row] = scale;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int e = (li + L * i) * W;
+#pragma unroll
+        for (int k = 0; k < W; ++k) v[i][k] *= inv;
+        if (live && e < a.C) store_e4m3<W>(reinterpret_cast<unsigned char*>(a.y) + row * a.C + e, v[i]);
+      }
+    }
+  }
+}
+
+// rows longer than the registers hold: one workgroup per row, the row read again for each pass over it
+template <typename T, int W, bool Q8> __global__ __launch_bounds__(256) void rms_fwd_long_kernel(FwdArgs a) {
+  __shared__ float red[4];
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    auto load = [&](int e, float* v) {
+      Row<T, W>::load(a.x, row * a.xs + e, v);
+      if (a.res) {
+        float r[W];
+        Row<T, W>::load(a.res, row * a.rs + e, r);
+#pragma unroll
+        for (int k = 0; k < W; ++k) v[k] += r[k];
+      }
+    };
+    float ss = 0.f;
+    for (int e = threadIdx.x * W; e < a.C; e += 256 * W) {
+      float v[W];
+      load(e, v);
+      if (a.res && a.s) Row<T, W>::store(a.s, row * a.C + e, v);
+#pragma unroll
+      for (int k = 0; k < W; ++k) ss = fmaf(v[k], v[k], ss);
+    }
+    const float rstd = 1.f / sqrtf(row_sum<256>(ss, red) / (float)a.C + a.eps);
+    if (a.rstd && threadIdx.x == 0) a.rstd[row] = rstd;
+    auto out = [&](int e, float* v) {
+      load(e, v);
+      float w[W];
+#pragma unroll
+      for (int k = 0; k < W; ++k) w[k] = 1.f;
+      if (a.w) load_f32<W>(a.w, e, w);
+#pragma unroll
+      for (int k = 0; k < W; ++k) v[k] = v[k] * rstd * w[k];
+    };
+    float inv = 1.f;
+    if constexpr (Q8) {
+      unsigned amax = 0;
+      for (int e = threadIdx.x * W; e < a.C; e += 256 * W) {
+        float v[W];
+        out(e, v);
+#pragma unroll
+        for (int k = 0; k < W; ++k) amax = max(amax, abs_bits(v[k]));
+      }
+      const float scale = e4m3_scale(row_max<256>(amax, reinterpret_cast<unsigned*>(red)));
+      inv = 1.f / scale;
+      if (threadIdx.x == 0) a.scale[row] = scale;
+    }
+    for (int e = threadIdx.x * W; e < a.C; e += 256 * W) {
+      float v[W];
+      out(e, v);
+      if constexpr (Q8) {
+#pragma unroll
+        for (int k = 0; k < W; ++k) v[k] *= inv;
+        store_e4m3<W>(reinterpret_cast<unsigned char*>(a.y) + row * a.C + e, v);
+      } else {
+        Row<T, W>::store(a.y, row * a.C + e, v);
+      }
+    }
+  }
+}
+
+struct BwdArgs {
+  const void *dy, *x, *res, *ds;
+  const float *rstd, *w;
+  void* dx;
+  float* partial;        // [gridDim.x][C], or null: no dw
+  int64_t dys, xs, rs, dss, rows;
+  int C;
+};
+
+template <typename T, int W> __device__ __forceinline__ void load_sum(const BwdArgs& a, int64_t row, int e, float* v) {
+  Row<T, W>::load(a.x, row * a.xs + e, v);
+  if (a.res) {
+    float r[W];
+    Row<T, W>::load(a.res, row * a.rs + e, r);
+#pragma unroll
+    for (int k = 0; k < W; ++k) v[k] += r[k];
+  }
+}
+
+template <typename T, int W, int L, int NV> __global__ __launch_bounds__(256) void rms_bwd_kernel(BwdArgs a) {
+  __shared__ float red[4];
+  __shared__ float fold[L >= 256 ? 1 : 256 * W];
+  const int li = threadIdx.x & (L - 1);
+  const int64_t rpb = 256 / L;
+  const float inv_c = 1.f / (float)a.C;
+  float w[NV][W], dw[NV][W];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int e = (li + L * i) * W;
+#pragma unroll
+    for (int k = 0; k < W; ++k) { w[i][k] = 1.f; dw[i][k] = 0.f; }
+    if (a.w && e < a.C) load_f32<W>(a.w, e, w[i]);
+  }
+  for (int64_t row = (int64_t)blockIdx.x * rpb + threadIdx.x / L; ; row += (int64_t)gridDim.x * rpb) {
+    if (row - threadIdx.x / L >= a.rows) break;
+    const bool live = row < a.rows;
+    const float rstd = live ? a.rstd[row] : 0.f;
+    float g[NV][W], xh[NV][W];
+    float dot = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int e = (li + L * i) * W;
+#pragma unroll
+      for (int k = 0; k < W; ++k) g[i][k] = xh[i][k] = 0.f;
+      if (live && e < a.C) {
+        Row<T, W>::load(a.dy, row * a.dys + e, g[i]);
+        load_sum<T, W>(a, row, e, xh[i]);
+      }
+#pragma unroll
+      for (int k = 0; k < W; ++k) {
+        xh[i][k] *= rstd;
+        dw[i][k] = fmaf(g[i][k], xh[i][k], dw[i][k]);
+        g[i][k] *= w[i][k];
+        dot = fmaf(g[i][k], xh[i][k], dot);
+      }
+    }
+    const float m = row_sum<L>(dot, red) * inv_c;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int e = (li + L * i) * W;
+      if (!live || e >= a.C) continue;
+      float d[W];
+#pragma unroll
+      for (int k = 0; k < W; ++k) d[k] = 0.f;
+      if (a.ds) Row<T, W>::load(a.ds, row * a.dss + e, d);
+#pragma unroll
+      for (int k = 0; k < W; ++k) d[k] = fmaf(rstd, fmaf(-xh[i][k], m, g[i][k]), d[k]);
+      Row<T, W>::store(a.dx, row * a.C + e, d);
+    }
+  }
+  if (!a.partial) return;
+  if constexpr (L >= 256) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int e = (li + L * i) * W;
+      if (e < a.C)
+#pragma unroll
+        for (int k = 0; k < W; ++k) a.partial[(int64_t)blockIdx.x * a.C + e + k] = dw[i][k];
+    }
+  } else {   // the workgroup's 256 / L rows meet in LDS, one vector index at a time
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      __syncthreads();
+#pragma unroll
+      for (int k = 0; k < W; ++k) fold[(threadIdx.x / L) * (L * W) + li * W + k] = dw[i][k];
+      __syncthreads();
+      for (int c = threadIdx.x; c < L * W; c += 256) {
+        float t = 0.f;
+        for (int r = 0; r < 256 / L; ++r) t += fold[r * (L * W) + c];
+        if (L * W * i + c < a.C) a.partial[(int64_t)blockIdx.x * a.C + L * W * i + c] = t;
+      }
+    }
+  }
+}
+
+template <typename T, int W> __global__ __launch_bounds__(256) void rms_bwd_long_kernel(BwdArgs a) {   // dx of rows longer than the registers hold
+  __shared__ float red[4];
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const float rstd = a.rstd[row];
+    auto load = [&](int e, float* g, float* xh) {
+      Row<T, W>::load(a.dy, row * a.dys + e, g);
+      load_sum<T, W>(a, row, e, xh);
+      float w[W];
+#pragma unroll
+      for (int k = 0; k < W; ++k) w[k] = 1.f;
+      if (a.w) load_f32<W>(a.w, e, w);
+#pragma unroll
+      for (int k = 0; k < W; ++k) { g[k] *= w[k]; xh[k] *= rstd; }
+    };
+    float dot = 0.f;
+    for (int e = threadIdx.x * W; e < a.C; e += 256 * W) {
+      float g[W], xh[W];
+      load(e, g, xh);
+#pragma unroll
+      for (int k = 0; k < W; ++k) dot = fmaf(g[k], xh[k], dot);
+    }
+    const float m = row_sum<256>(dot, red) / (float)a.C;
+    for (int e = threadIdx.x * W; e < a.C; e += 256 * W) {
+      float g[W], xh[W], d[W];
+      load(e, g, xh);
+#pragma unroll
+      for (int k = 0; k < W; ++k) d[k] = 0.f;
+      if (a.ds) Row<T, W>::load(a.ds, row * a.dss + e, d);
+#pragma unroll
+      for (int k = 0; k < W; ++k) d[k] = fmaf(rstd, fmaf(-xh[k], m, g[k]), d[k]);
+      Row<T, W>::store(a.dx, row * a.C + e, d);
+    }
+  }
+}
+// and their dw: a thread per column, gridDim.y slabs of rows
+template <typename T> __global__ __launch_bounds__(256) void rms_dw_long_kernel(BwdArgs a) {
+  const int c = blockIdx.x * 256 + threadIdx.x;
+  if (c >= a.C) return;
+  float t = 0.f;
+  for (int64_t row = blockIdx.y; row < a.rows; row += gridDim.y) {
+    float v[1];
+    load_sum<T, 1>(a, row, c, v);
+    t = fmaf(load_elem<T>(a.dy, row * a.dys + c), v[0] * a.rstd[row], t);
+  }
+  a.partial[(int64_t)blockIdx.y * a.C + c] = t;
+}
+
+// dw[c] = sum over the n partial rows, in order within 16 interleaved slices and then over the slices
+__global__ __launch_bounds__(1024) void rms_dw_fold_kernel(const float* partial, float* dw, int n, int C) {
+  __shared__ float t[16][64];
+  const int c = blockIdx.x * 64 + (threadIdx.x & 63), z = threadIdx.x >> 6;
+  float v = 0.f;
+  if (c < C)
+    for (int i = z; i < n; i += 16) v += partial[(int64_t)i * C + c];
+  t[z][threadIdx.x & 63] = v;
+  __syncthreads();
+  if (z == 0 && c < C) {
+#pragma unroll
+    for (int i = 1; i < 16; ++i) v += t[i][threadIdx.x];
+    dw[c] = v;
+  }
+}
+
+constexpr int kMaxGrid = 1 << 20;      // (forward) workgroups; rows beyond are walked
+constexpr int kBwdGrid = 1024;         // (backward) workgroups = partial rows of dw
+
+struct Shape { int L, NV; };           // 0 lanes: the long form
+inline Shape pick(int C, int W) {
+  const int n = (C + W - 1) / W;
+  if (W == 1) {
+    if (n <= 64) return {64, 1};
+    if (n <= 256) return {64, 4};
+    if (n <= 1024) return {64, 16};
+    if (n <= 4096) return {256, 16};
+    return {0, 0};
+  }
+  if (n <= 8) return {8, 1};
+  if (n <= 16) return {16, 1};
+  if (n <= 32) return {32, 1};
+  if (n <= 64) return {64, 1};
+  if (n <= 128) return {64, 2};
+  if (n <= 256) return {64, 4};
+  if (n <= 512) return {256, 2};
+  if (n <= 1024) return {256, 4};
+  return {0, 0};
+}
+inline int bwd_grid(int64_t rows, int L) {
+  const int64_t rpb = L ? 256 / L : 1, n = (rows + rpb - 1) / rpb;
+  return (int)(n < kBwdGrid ? n : kBwdGrid);
+}
+
+template <typename T, int W, bool Q8> int launch_fwd(const FwdArgs& a, hipStream_t st) {
+  const Shape sh = pick(a.C, W);
+  const int64_t rpb = sh.L ? 256 / sh.L : 1, need = (a.rows + rpb - 1) / rpb;
+  const int grid = (int)(need < kMaxGrid ? need : kMaxGrid);
+#define TG_RMS(LL, NN) if (sh.L == LL && sh.NV == NN) { rms_fwd_kernel<T, W, LL, NN, Q8><<<grid, 256, 0, st>>>(a); return tg_launch_status(); }
+  if constexpr (W == 1) { TG_RMS(64, 1) TG_RMS(64, 4) TG_RMS(64, 16) TG_RMS(256, 16) }
+  else { TG_RMS(8, 1) TG_RMS(16, 1) TG_RMS(32, 1) TG_RMS(64, 1) TG_RMS(64, 2) TG_RMS(64, 4) TG_RMS(256, 2) TG_RMS(256, 4) }
+#undef TG_RMS
+  rms_fwd_long_kernel<T, W, Q8><<<grid, 256, 0, st>>>(a);
+  return tg_launch_status();
+}
+
+template <typename T, int W> int launch_bwd(const BwdArgs& a, float* dw, hipStream_t st) {
+  const Shape sh = pick(a.C, W);
+  const int grid = bwd_grid(a.rows, sh.L);
+  auto go = [&]() -> int {
+#define TG_RMS(LL, NN) if (sh.L == LL && sh.NV == NN) { rms_bwd_kernel<T, W, LL, NN><<<grid, 256, 0, st>>>(a); return tg_launch_status(); }
+    if constexpr (W == 1) { TG_RMS(64, 1) TG_RMS(64, 4) TG_RMS(64, 16) TG_RMS(256, 16) }
+    else { TG_RMS(8, 1) TG_RMS(16, 1) TG_RMS(32, 1) TG_RMS(64, 1) TG_RMS(64, 2) TG_RMS(64, 4) TG_RMS(256, 2) TG_RMS(256, 4) }
+#undef TG_RMS
+    rms_bwd_long_kernel<T, W><<<grid, 256, 0, st>>>(a);
+    if (a.partial) rms_dw_long_kernel<T><<<dim3((a.C + 255) / 256, grid), 256, 0, st>>>(a);
+    return tg_launch_status();
+  };
+  const int rc = go();
+  if (rc != TG_OK || !dw) return rc;
+  rms_dw_fold_kernel<<<(a.C + 63) / 64, 1024, 0, st>>>(a.partial, dw, grid, a.C);
+  return tg_launch_status();
+}
+
+inline int elem_bytes(int dtype) { return dtype == TG_F32 ? 4 : 2; }
+inline bool known(int dtype) { return dtype == TG_F32 || dtype == TG_BF16 || dtype == TG_F16; }
+inline bool elem_aligned(const void* p, int dtype) { return (reinterpret_cast<uintptr_t>(p) & (elem_bytes(dtype) - 1)) == 0; }
+inline bool wide(int dtype, int C, int64_t stride, const void* p) {   // 16-byte accesses possible for this operand?
+  const int n = 16 / elem_bytes(dtype);
+  return !p || (C % n == 0 && stride % n == 0 && tg_aligned16(p));
+}
+
+template <bool Q8>
+int rms_fwd(int dtype, const FwdArgs& a, hipStream_t st) {
+  if (!known(dtype) || a.rows < 0 || a.C <= 0 || a.xs < 0 || a.rs < 0 || !(a.eps >= 0.f)) return TG_E_BADARG;
+  if (a.rows == 0) return TG_OK;
+  if (!a.x || !a.y || (Q8 && !a.scale)) return TG_E_BADARG;
+  if (!elem_aligned(a.x, dtype) || !elem_aligned(a.res, dtype) || !elem_aligned(a.s, dtype) || (!Q8 && !elem_aligned(a.y, dtype)) ||
+      (reinterpret_cast<uintptr_t>(a.w) & 3) || (reinterpret_cast<uintptr_t>(a.rstd) & 3) || (reinterpret_cast<uintptr_t>(a.scale) & 3))
+    return TG_E_ALIGN;
+  const bool v = wide(dtype, a.C, a.xs, a.x) && wide(dtype, a.C, a.rs, a.res) && wide(dtype, a.C, a.C, a.s) && wide(dtype, a.C, a.C, a.y) &&
+                 (!a.w || tg_aligned16(a.w));
+  TG_DISPATCH_DTYPE(dtype, return v ? (launch_fwd<BF16, 8, Q8>(a, st)) : (launch_fwd<BF16, 1, Q8>(a, st)),
+                    return v ? (launch_fwd<F16, 8, Q8>(a, st)) : (launch_fwd<F16, 1, Q8>(a, st)),
+                    return v ? (launch_fwd<F32, 4, Q8>(a, st)) : (launch_fwd<F32, 1, Q8>(a, st)));
+}
+
+}  // namespace
+
+extern "C" int tg_rms_norm(int dtype, const void* x, int64_t x_stride, const void* res, int64_t res_stride, const float* weight, void* y,
+                           void* s, float* rstd, int64_t rows, int C, float eps, void* stream) {
+  return rms_fwd<false>(dtype, FwdArgs{x, res, weight, y, s, rstd, nullptr, x_stride, res_stride, rows, C, eps}, (hipStream_t)stream);
+}
+
+extern "C" int tg_rms_norm_e4m3(int dtype, const void* x, int64_t x_stride, const void* res, int64_t res_stride, const float* weight,
+                                void* q, float* scale, void* s, int64_t rows, int C, float eps, void* stream) {
+  return rms_fwd<true>(dtype, FwdArgs{x, res, weight, q, s, nullptr, scale, x_stride, res_stride, rows, C, eps}, (hipStream_t)stream);
+}
+
+extern "C" int64_t tg_rms_norm_bwd_scratch_floats(int64_t rows, int C) {
+  if (rows <= 0 || C <= 0) return 0;
+  return (rows < kBwdGrid ? rows : kBwdGrid) * (int64_t)C;
+}
+
+extern "C" int tg_rms_norm_bwd(int dtype, const void* dy, int64_t dy_stride, const void* x, int64_t x_stride, const void* res,
+                               int64_t res_stride, const float* rstd, const float* weight, const void* ds, int64_t ds_stride, void* dx,
+                               float* dweight, float* scratch, int64_t rows, int C, void* stream) {
+  if (!known(dtype) || rows < 0 || C <= 0 || dy_stride < 0 || x_stride < 0 || res_stride < 0 || ds_stride < 0 || (dweight && rows && !scratch))
+    return TG_E_BADARG;
+  const BwdArgs a{dy, x, res, ds, rstd, weight, dx, dweight ? scratch : nullptr, dy_stride, x_stride, res_stride, ds_stride, rows, C};
+  hipStream_t st = (hipStream_t)stream;
+  if (rows == 0) {   // the gradient of no rows
+    if (dweight) rms_dw_fold_kernel<<<(C + 63) / 64, 1024, 0, st>>>(nullptr, dweight, 0, C);
+    return tg_launch_status();
+  }
+  if (!dy || !x || !rstd || !dx) return TG_E_BADARG;
+  if (!elem_aligned(dy, dtype) || !elem_aligned(x, dtype) || !elem_aligned(res, dtype) || !elem_aligned(ds, dtype) || !elem_aligned(dx, dtype) ||
+      ((reinterpret_cast<uintptr_t>(weight) | reinterpret_cast<uintptr_t>(rstd) | reinterpret_cast<uintptr_t>(dweight) |
+        reinterpret_cast<uintptr_t>(scratch)) & 3))
+    return TG_E_ALIGN;
+  const bool v = wide(dtype, C, dy_stride, dy) && wide(dtype, C, x_stride, x) && wide(dtype, C, res_stride, res) && wide(dtype, C, ds_stride, ds) &&
+                 wide(dtype, C, C, dx) && (!weight || tg_aligned16(weight));
+  TG_DISPATCH_DTYPE(dtype, return v ? (launch_bwd<BF16, 8>(a, dweight, st)) : (launch_bwd<BF16, 1>(a, dweight, st)),
+                    return v ? (launch_bwd<F16, 8>(a, dweight, st)) : (launch_bwd<F16, 1>(a, dweight, st)),
+                    return v ? (launch_bwd<F32, 4>(a, dweight, st)) : (launch_bwd<F32, 1>(a, dweight, st)));
+}

@@ -7,6 +7,8 @@ import torch
 import torch.nn as nn
 
 from . import kernels as K
+from .sequence import (dropout, dropout_backward, dropout_rng, linear_attention, linear_attention_backward,  # noqa: F401
+                       linear_attention_step, rms_norm, rms_norm_backward, rms_norm_e4m3)
 
 
 def preprocess(image):

@@ -1,0 +1,113 @@
+"""The sequence-layer operators without a GPU: the C entry points check their arguments before any launch (status codes below), the Python
+forms refuse host tensors, and the names are where a user of `from ops import *` finds them."""
+import ctypes as C
+import os
+import sys
+
+import pytest
+import torch
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+if ROOT not in sys.path:
+    sys.path.insert(0, ROOT)
+import pytorch_tecogan_amd  # noqa: E402,F401
+from pytorch_tecogan_amd import _lib as L  # noqa: E402
+from pytorch_tecogan_amd import ops  # noqa: E402
+
+BADARG, UNSUPPORTED, ALIGN = -1, -2, -3
+P = 0x10000   # never dereferenced: every call below is refused before a launch
+
+
+def desc(B=2, T=5, H=2, HK=2, DK=16, DV=8):
+    st = lambda h, d: (T * h * d, h * d, d)   # noqa: E731
+    return L.LaDesc(B, T, H, HK, DK, DV, st(H, DK), st(HK, DK), st(HK, DV), 0.25)
+
+
+def test_rms_norm_arguments():
+    f = L.load().tg_rms_norm
+    good = [L.TG_BF16, P, 64, None, 0, P, P, None, None, 4, 64, 1e-6, None]
+    for at, value, want in ((0, 7, BADARG), (1, None, BADARG), (6, None, BADARG), (9, -1, BADARG), (10, 0, BADARG), (2, -64, BADARG), (11, -1.0, BADARG),
+                            (11, float("nan"), BADARG), (1, P + 1, ALIGN), (3, P + 1, ALIGN), (6, P + 1, ALIGN), (5, P + 2, ALIGN), (8, P + 2, ALIGN)):
+        bad = list(good)
+        bad[at] = value
+        assert f(*bad) == want, (at, value)
+    assert f(*(good[:9] + [0] + good[10:])) == 0   # no rows: nothing to launch
+    f = L.load().tg_rms_norm_e4m3
+    good = [L.TG_F32, P, 64, None, 0, P, P, P, None, 4, 64, 1e-6, None]
+    for at, value, want in ((7, None, BADARG), (6, None, BADARG), (7, P + 2, ALIGN), (1, P + 2, ALIGN)):
+        bad = list(good)
+        bad[at] = value
+        assert f(*bad) == want, (at, value)
+    f = L.load().tg_rms_norm_bwd
+    good = [L.TG_F16, P, 64, P, 64, None, 0, P, P, None, 0, P, P, P, 4, 64, None]
+    for at, value, want in ((1, None, BADARG), (3, None, BADARG), (7, None, BADARG), (11, None, BADARG), (13, None, BADARG), (14, -1, BADARG), (15, 0, BADARG),
+                            (1, P + 1, ALIGN), (9, P + 1, ALIGN), (12, P + 2, ALIGN), (13, P + 2, ALIGN)):
+        bad = list(good)
+        bad[at] = value
+        assert f(*bad) == want, (at, value)
+    n = L.load().tg_rms_norm_bwd_scratch_floats
+    assert n(0, 64) == 0 and n(3, 0) == 0 and n(1, 64) >= 64 and n(1 << 40, 128) >= 128
+
+
+def test_dropout_arguments():
+    f = L.load().tg_dropout
+    good = [L.TG_BF16, P, None, P, 100, 0.5, P, 0, None]
+    for at, value, want in ((0, 3, BADARG), (1, None, BADARG), (3, None, BADARG), (4, -1, BADARG), (5, 1.0, BADARG), (5, -0.1, BADARG), (5, float("nan"), BADARG),
+                            (6, None, BADARG), (1, P + 1, ALIGN), (2, P + 1, ALIGN), (3, P + 1, ALIGN), (6, P + 4, ALIGN)):
+        bad = list(good)
+        bad[at] = value
+        assert f(*bad) == want, (at, value)
+    assert f(*(good[:4] + [0] + good[5:])) == 0
+
+
+def test_linear_attention_arguments():
+    lib = L.load()
+    ref = C.byref
+    for d, want in ((desc(B=-1), BADARG), (desc(T=-1), BADARG), (desc(H=0), BADARG), (desc(HK=0), BADARG), (desc(DK=0), BADARG), (desc(DV=0), BADARG),
+                    (desc(H=3), UNSUPPORTED), (desc(DK=129), UNSUPPORTED), (desc(DV=129), UNSUPPORTED)):
+        assert lib.tg_linear_attention(L.TG_F32, ref(d), P, P, P, P, None, None, P, P, None) == want
+        assert lib.tg_linear_attention_step(L.TG_F32, ref(d), P, P, P, P, P, P, None) == want
+        assert lib.tg_linear_attention_bwd(L.TG_F32, ref(d), P, P, P, P, (C.c_int64 * 3)(80, 16, 8), P, None, None, None, P, P, P, None, P, None) == want
+        assert lib.tg_linear_attention_bwd_scratch_floats(ref(d)) == 0
+    d = desc()
+    good = [L.TG_BF16, ref(d), P, P, P, P, None, None, P, P, None]
+    for at, value, want in ((0, 9, BADARG), (1, None, BADARG), (2, None, BADARG), (3, None, BADARG), (4, None, BADARG), (5, None, BADARG), (8, None, BADARG),
+                            (9, None, BADARG), (2, P + 1, ALIGN), (4, P + 1, ALIGN), (8, P + 1, ALIGN), (9, P + 2, ALIGN), (5, P + 2, ALIGN), (7, P + 2, ALIGN),
+                            (6, P + 2, ALIGN)):
+        bad = list(good)
+        bad[at] = value
+        assert lib.tg_linear_attention(*bad) == want, (at, value)
+    good = [L.TG_BF16, ref(d), P, P, P, P, P, P, None]
+    for at, value, want in ((2, None, BADARG), (3, None, BADARG), (4, None, BADARG), (5, None, BADARG), (6, None, BADARG), (7, None, BADARG), (2, P + 1, ALIGN),
+                            (7, P + 2, ALIGN), (5, P + 2, ALIGN)):
+        bad = list(good)
+        bad[at] = value
+        assert lib.tg_linear_attention_step(*bad) == want, (at, value)
+    shared = desc(H=4, HK=2)
+    good = [L.TG_BF16, ref(shared), P, P, P, P, (C.c_int64 * 3)(160, 32, 8), P, None, None, None, P, P, P, None, P, None]
+    for at, value, want in ((2, None, BADARG), (5, None, BADARG), (6, None, BADARG), (7, None, BADARG), (11, None, BADARG), (13, None, BADARG), (15, None, BADARG),
+                            (12, P + 1, ALIGN), (15, P + 2, ALIGN), (14, P + 2, ALIGN), (9, P + 2, ALIGN), (10, P + 2, ALIGN)):
+        bad = list(good)
+        bad[at] = value
+        assert lib.tg_linear_attention_bwd(*bad) == want, (at, value)
+    # an empty batch: nothing to launch
+    assert lib.tg_linear_attention(L.TG_F32, ref(desc(B=0)), None, None, None, None, None, None, None, None, None) == 0
+
+
+def test_host_tensors_are_refused():
+    x = torch.zeros(4, 64)
+    q = torch.zeros(2, 3, 2, 16)
+    rng, decay = torch.zeros(2, dtype=torch.int64), torch.zeros(2)
+    for call in (lambda: ops.rms_norm(x), lambda: ops.rms_norm_e4m3(x), lambda: ops.rms_norm_backward(x, x, torch.zeros(4)), lambda: ops.dropout(x, 0.1, rng),
+                 lambda: ops.dropout_backward(x, 0.1, rng), lambda: ops.linear_attention(q, q, q, decay),
+                 lambda: ops.linear_attention_backward(q, q, q, q, decay), lambda: ops.linear_attention_step(q[0], q[0], q[0], decay, torch.zeros(3, 2, 16, 16))):
+        with pytest.raises(L.TecoganHipError):
+            call()
+
+
+def test_names_are_public():
+    """`from ops import *` (code/ops.py) re-exports every public name of the package's ops module"""
+    from pytorch_tecogan_amd import sequence
+    for name in sequence.__all__:
+        assert getattr(ops, name) is getattr(sequence, name)
+        assert getattr(ops, name).__doc__
