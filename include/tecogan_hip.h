@@ -593,16 +593,17 @@ int tg_dropout(int dtype, const void* x, const void* res, void* y, int64_t n, do
  * at the given strides of (sequence, token, head), H % HK == 0: head h reads stored head h / (H / HK); 1 <= DK, DV <= 128.
  * Outputs o, dq [B][T][H][..], dk, dv [B][T][HK][..] are contiguous; states [B][H][DK][DV] fp32; lengths [B] int32 or null: tokens at and
  * behind lengths[b] (clamped to 0 .. T) are not read, their rows of the outputs are zero and the last state is the one at the length.
- * state_in null: zeros.  tg_linear_attention_bwd: dstate_out null: zeros; dstate_in may be null; scratch:
- * tg_linear_attention_bwd_scratch_floats floats (0: null).  log_decay is a constant (no gradient).
+ * state_in null: zeros.  tg_linear_attention_bwd: dstate_out null: zeros; dstate_in may be null.  scratch: *_scratch_floats floats (0: may
+ * be null), this call's alone until it has run.  log_decay is a constant (no gradient).
  * tg_linear_attention_step: one token (strides of sequence and head; T and the token stride are not looked at), `state` updated in place. */
 typedef struct {
   int32_t B, T, H, HK, DK, DV;
   int64_t q_stride[3], k_stride[3], v_stride[3];   /* sequence, token, head */
   float scale;
 } tg_la_desc;
+int64_t tg_linear_attention_scratch_floats(const tg_la_desc* d);
 int tg_linear_attention(int dtype, const tg_la_desc* d, const void* q, const void* k, const void* v, const float* log_decay,
-                        const int32_t* lengths, const float* state_in, void* o, float* state_out, void* stream);
+                        const int32_t* lengths, const float* state_in, void* o, float* state_out, float* scratch, void* stream);
 int64_t tg_linear_attention_bwd_scratch_floats(const tg_la_desc* d);
 int tg_linear_attention_bwd(int dtype, const tg_la_desc* d, const void* q, const void* k, const void* v, const void* dout,
                             const int64_t* dout_stride, const float* log_decay, const int32_t* lengths, const float* state_in,

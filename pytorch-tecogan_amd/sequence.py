@@ -236,6 +236,11 @@ def dropout_backward(dy, p, rng, layer=0):
 _Strides = C.c_int64 * 3
 
 
+def _channels_last(t):
+    """t with contiguous channels (and a token stride that the kernels' 32-bit integers hold)"""
+    return t if (t.stride(-1) == 1 or t.shape[-1] == 1) and t.stride(1) < 1 << 31 else t.contiguous()
+
+
 def _desc(q, k, v, log_decay, scale, step):
     """(dtype, descriptor, tensors) after the checks that the sequence and the single-token form share"""
     dt = _floats(q, "q")
@@ -254,7 +259,7 @@ def _desc(q, k, v, log_decay, scale, step):
     if log_decay.requires_grad and torch.is_grad_enabled():
         _fail("log_decay is a constant of the heads: it has no gradient")
     log_decay = _f32(q, log_decay, "log_decay", (H,))
-    q, k, v = (t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous() for t in (q, k, v))
+    q, k, v = (_channels_last(t) for t in (q, k, v))
     strides = [t.stride() for t in (q, k, v)]
     if step:
         strides = [(s[0], 0, s[1]) for s in strides]
@@ -278,8 +283,10 @@ def _attention_fwd(q, k, v, log_decay, scale, state, lengths):
     lengths = _lengths(q, lengths)
     o = torch.empty((d.B, d.T, d.H, d.DV), dtype=q.dtype, device=q.device)
     last = torch.empty(shape, dtype=torch.float32, device=q.device)
+    n = L.load().tg_linear_attention_scratch_floats(C.byref(d))
+    scratch = torch.empty(n, dtype=torch.float32, device=q.device) if n else None
     _call(q.device, "tg_linear_attention", dt, C.byref(d), q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), _ptr(lengths),
-          _ptr(state), o.data_ptr(), last.data_ptr())
+          _ptr(state), o.data_ptr(), last.data_ptr(), _ptr(scratch))
     return o, last
 
 
@@ -323,7 +330,7 @@ def linear_attention_backward(do, q, k, v, log_decay, scale=None, state=None, le
         dt, d, q, k, v, log_decay = _desc(q, k, v, log_decay, scale, False)
     shape = (d.B, d.H, d.DK, d.DV)
     _like(q, do, "do", torch.Size((d.B, d.T, d.H, d.DV)))
-    do = do if do.stride(-1) == 1 or d.DV == 1 else do.contiguous()
+    do = _channels_last(do)
     state = None if state is None else _f32(q, state, "state", shape)
     dstate = None if dstate is None else _f32(q, dstate, "dstate", shape)
     lengths = _lengths(q, lengths)

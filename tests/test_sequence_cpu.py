@@ -65,15 +65,16 @@ def test_linear_attention_arguments():
     ref = C.byref
     for d, want in ((desc(B=-1), BADARG), (desc(T=-1), BADARG), (desc(H=0), BADARG), (desc(HK=0), BADARG), (desc(DK=0), BADARG), (desc(DV=0), BADARG),
                     (desc(H=3), UNSUPPORTED), (desc(DK=129), UNSUPPORTED), (desc(DV=129), UNSUPPORTED)):
-        assert lib.tg_linear_attention(L.TG_F32, ref(d), P, P, P, P, None, None, P, P, None) == want
+        assert lib.tg_linear_attention(L.TG_F32, ref(d), P, P, P, P, None, None, P, P, None, None) == want
+        assert lib.tg_linear_attention_scratch_floats(ref(d)) == 0
         assert lib.tg_linear_attention_step(L.TG_F32, ref(d), P, P, P, P, P, P, None) == want
         assert lib.tg_linear_attention_bwd(L.TG_F32, ref(d), P, P, P, P, (C.c_int64 * 3)(80, 16, 8), P, None, None, None, P, P, P, None, P, None) == want
         assert lib.tg_linear_attention_bwd_scratch_floats(ref(d)) == 0
     d = desc()
-    good = [L.TG_BF16, ref(d), P, P, P, P, None, None, P, P, None]
+    good = [L.TG_BF16, ref(d), P, P, P, P, None, None, P, P, None, None]
     for at, value, want in ((0, 9, BADARG), (1, None, BADARG), (2, None, BADARG), (3, None, BADARG), (4, None, BADARG), (5, None, BADARG), (8, None, BADARG),
                             (9, None, BADARG), (2, P + 1, ALIGN), (4, P + 1, ALIGN), (8, P + 1, ALIGN), (9, P + 2, ALIGN), (5, P + 2, ALIGN), (7, P + 2, ALIGN),
-                            (6, P + 2, ALIGN)):
+                            (6, P + 2, ALIGN), (10, P + 2, ALIGN)):
         bad = list(good)
         bad[at] = value
         assert lib.tg_linear_attention(*bad) == want, (at, value)
@@ -83,15 +84,25 @@ def test_linear_attention_arguments():
         bad = list(good)
         bad[at] = value
         assert lib.tg_linear_attention_step(*bad) == want, (at, value)
-    shared = desc(H=4, HK=2)
-    good = [L.TG_BF16, ref(shared), P, P, P, P, (C.c_int64 * 3)(160, 32, 8), P, None, None, None, P, P, P, None, P, None]
+    shared = desc(H=10, HK=2)   # (more shared heads than a workgroup sums: through scratch)
+    good = [L.TG_BF16, ref(shared), P, P, P, P, (C.c_int64 * 3)(400, 80, 8), P, None, None, None, P, P, P, None, P, None]
     for at, value, want in ((2, None, BADARG), (5, None, BADARG), (6, None, BADARG), (7, None, BADARG), (11, None, BADARG), (13, None, BADARG), (15, None, BADARG),
                             (12, P + 1, ALIGN), (15, P + 2, ALIGN), (14, P + 2, ALIGN), (9, P + 2, ALIGN), (10, P + 2, ALIGN)):
         bad = list(good)
         bad[at] = value
         assert lib.tg_linear_attention_bwd(*bad) == want, (at, value)
+    # one long sequence is cut into segments: their states need scratch
+    long = desc(B=1, T=4096, H=1, HK=1)
+    need = lib.tg_linear_attention_scratch_floats(ref(long))
+    assert need >= 2 * 16 * 8 and lib.tg_linear_attention_bwd_scratch_floats(ref(long)) >= 4 * 16 * 8
+    assert lib.tg_linear_attention(L.TG_BF16, ref(long), P, P, P, P, None, None, P, P, None, None) == BADARG
+    wild = desc()
+    wild.k_stride[1] = 1 << 31
+    assert lib.tg_linear_attention(L.TG_BF16, ref(wild), P, P, P, P, None, None, P, P, None, None) == UNSUPPORTED
+    wild.k_stride[1] = -16
+    assert lib.tg_linear_attention(L.TG_BF16, ref(wild), P, P, P, P, None, None, P, P, None, None) == BADARG
     # an empty batch: nothing to launch
-    assert lib.tg_linear_attention(L.TG_F32, ref(desc(B=0)), None, None, None, None, None, None, None, None, None) == 0
+    assert lib.tg_linear_attention(L.TG_F32, ref(desc(B=0)), None, None, None, None, None, None, None, None, None, None) == 0
 
 
 def test_host_tensors_are_refused():
