@@ -15,11 +15,11 @@
 // so ONE kernel serves all four: out_i = za g^{i+1-sh} a_i S + scale sum_{j<=i} g^{i-j} (a_i . b_j) c_j,
 // S' = g^n S + zs sum_j g^{n-1-j+sh} b_j c_j^T over tokens taken forwards (sh = 0, za = scale, zs = 1) or backwards (sh = 1, za = 1, zs = scale).
 //
-// Layout: a wave owns 16 columns of c (and of S and out) of one sequence and head and walks its tokens in chunks of 16 CT.  Everything is
+// Layout: a wave owns 16 columns of c (and of S and out) of one head and walks the tokens in chunks of 16 CT.  Everything is
 // made of 16 x 16 tiles in the matrix instructions' own shape: lane (c = lane % 16, g = lane / 16) holds 4 consecutive values 4g .. 4g+3
 // of row / column c.  An accumulator tile X[k][c] has the shape of an operand with c along its free dimension and k along the summed one,
 // so the scores (b a^T, tile [j][i]) and the state (tiles [m][n]) go from accumulators to operands without leaving the registers, and a
-// product with the identity turns a tile that was loaded by rows into one by columns (exactly) - no LDS, no second load.
+// product with the identity turns a tile that was loaded by rows into one by columns (exactly).
 //
 // Long sequences: T is cut into segments of `seg` tokens so that a few heads fill the machine.  la_kernel<STATE> sums each segment's own state,
 // la_scan_kernel joins them into the state in front of every segment, and the segments then run side by side.
@@ -44,7 +44,12 @@ __device__ __forceinline__ s16x8 join(s16x4 a, s16x4 b) { return __builtin_shuff
 __device__ __forceinline__ f32x4 mma2_bf16(s16x4 a0, s16x4 a1, s16x4 b0, s16x4 b1, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, join(a0, a1)), __builtin_bit_cast(bf16x8, join(b0, b1)), c, 0, 0, 0);
 }
-__device__ __forceinline__ s16x4 to_bf16(f32x4 v) { return __builtin_bit_cast(s16x4, __builtin_convertvector(v, bf16x4)); }
+__device__ __forceinline__ unsigned pack_bf16(float a, float b) {   // v_cvt_pk_bf16_f32
+  typedef __attribute__((ext_vector_type(2))) float f32x2;
+  typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
+  return __builtin_bit_cast(unsigned, __builtin_convertvector(f32x2{a, b}, bf16x2));
+}
+__device__ __forceinline__ s16x4 to_bf16(f32x4 v) { return __builtin_bit_cast(s16x4, make_uint2(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]))); }
 __device__ __forceinline__ f32x4 from_bf16(s16x4 v) {
   const uint2 u = __builtin_bit_cast(uint2, v);
   return f32x4{__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u), __uint_as_float(u.y << 16), __uint_as_float(u.y & 0xffff0000u)};
@@ -102,6 +107,7 @@ template <> struct Mat<BF16> {
   typedef Halves Split;
   typedef Thirds Split3;
   __device__ __forceinline__ static Raw one(int d) { return Raw{(short)(d == 0 ? 0x3f80 : 0), (short)(d == 1 ? 0x3f80 : 0), (short)(d == 2 ? 0x3f80 : 0), (short)(d == 3 ? 0x3f80 : 0)}; }
+  __device__ __forceinline__ static s16x4 to_out(f32x4 v) { return to_bf16(v); }
   __device__ __forceinline__ static Op op(Raw v) { return v; }
   __device__ __forceinline__ static Op op_of(f32x4 v) { return to_bf16(v); }   // (of values that are bf16)
   __device__ __forceinline__ static Split split(f32x4 v) { return halves(v); }
@@ -128,6 +134,7 @@ template <> struct Mat<F16> {
   typedef Halves Split;
   typedef Thirds Split3;
   __device__ __forceinline__ static Raw one(int d) { return Raw{(short)(d == 0 ? 0x3c00 : 0), (short)(d == 1 ? 0x3c00 : 0), (short)(d == 2 ? 0x3c00 : 0), (short)(d == 3 ? 0x3c00 : 0)}; }
+  __device__ __forceinline__ static s16x4 to_out(f32x4 v) { return __builtin_bit_cast(s16x4, __builtin_convertvector(v, f16x4)); }
   __device__ __forceinline__ static Op op(Raw v) { return halves(__builtin_convertvector(__builtin_bit_cast(f16x4, v), f32x4)); }
   __device__ __forceinline__ static Op op_of(f32x4 v) { return halves(v); }
   __device__ __forceinline__ static Split split(f32x4 v) { return halves(v); }
@@ -195,14 +202,15 @@ struct Role {
   float za, zs;
   int sh, reverse;
   int fold;              // heads whose outputs are summed (dk, dv of shared heads): waves of one workgroup
-  int out_f32, wide;     // out holds floats; all addresses aligned to 4 elements
+  int out_f32, wide, pieces;   // out holds floats; all addresses aligned to 4 elements; to 16 bytes, and M and N fill 16 bytes
 };
 
 struct LaArgs {
   const float* log_decay;  // [H]
   const int* lengths;      // [B], or null
   int B, T, H;
-  int group;               // waves of a workgroup that belong to one (sequence, stored head, slice)
+  int group;               // waves of a workgroup that belong to one (stored head, slice)
+  int columns, bgroups;    // blockIdx.x = bgroup * columns + column: workgroups over (stored head, slice), and over the sequences
   int seg, segments;       // tokens in a segment (a multiple of 64)
   float scale;
   Role r[3];
@@ -222,228 +230,360 @@ struct Decay {
   }
 };
 
-template <typename T, int MT, int CT, bool WHOLE, bool STATE> __global__ __launch_bounds__(256) void la_kernel(LaArgs p) {
+// How a chunk's rows reach a wave.  STAGED (16-byte aligned operands whose channels fill 16-byte pieces): a wave reads whole rows, 16 bytes per
+// lane and neighbouring lanes side by side, into its own part of the LDS and takes the tiles from there.  (Tiles straight from memory -
+// 16 rows at a time, 8 bytes per lane - cost one L1 access per LANE: 54 per load instruction, and the L1s became the bound: 370 us
+// instead of 311 for 65536 sequences of 120 tokens, the more waves the worse.)  Otherwise every lane loads its tiles' elements itself.
+// The next chunk's rows are on their way, in registers, while this one is worked on.
+template <typename T, int MT, int CT> struct Stage {
+  static constexpr int kBytes = ElemTraits<T>::kBytes;
+  static constexpr int C = 16 * CT;
+  static constexpr int kLanes = kBytes * MT;                      // lanes (16-byte pieces) of a row of a or b
+  static constexpr int kRow = 16 * kLanes + 16;                   // bytes between rows: 16 rows x 16 bytes hit every bank once
+  static constexpr int kCRow = 16 * kBytes + 16;                  // the same for c: 16 columns
+  static constexpr int kLoads = (C * kLanes + 63) / 64, kCLoads = (C * kBytes + 63) / 64;
+  static constexpr int kArea = C * (2 * kRow + kCRow);            // LDS of a wave
+};
+
+// A wave keeps one head's slice and walks the sequences bgroup, bgroup + bgroups, .. (the decay's powers are made once), every sequence's
+// tokens in chunks.
+template <typename T, int MT, int CT, bool STAGED, bool STATE> __global__ __launch_bounds__(256, 2) void la_kernel(LaArgs p) {
   typedef Mat<T> X;
+  typedef Stage<T, MT, CT> G;
   typedef typename X::Raw Raw;
   typedef typename X::Op Op;
   constexpr int kBytes = ElemTraits<T>::kBytes;
   constexpr int C = 16 * CT;
-  __shared__ f32x4 sums[STATE ? 1 : 2][STATE ? 1 : 4][CT][64];
+  constexpr f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+  extern __shared__ __align__(16) char lds[];           // [waves][kArea] if STAGED, then [2][waves][CT][64] sums of 4 floats if a role folds
   const Role& r = p.r[blockIdx.y];
-  const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int slices = (r.N + 15) >> 4, stored = p.H / p.group;
-  const int per = (blockDim.x >> 6) / p.group;                       // (sequence, stored head, slice) triples of a workgroup
-  const int f = blockIdx.x * per + wave / p.group, member = wave % p.group;
-  const bool active = f < p.B * stored * slices;                    // (a wave without work still meets the barriers of the summed roles)
-  const int slice = f % slices, bi = active ? f / slices / stored : 0, h = (active ? f / slices % stored : 0) * p.group + member;
+  const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+  const int slices = (r.N + 15) >> 4;
+  const int per = waves / p.group;                                   // (stored head, slice) pairs of a workgroup
+  const int f = blockIdx.x % p.columns * per + wave / p.group, member = wave % p.group, bgroup = blockIdx.x / p.columns;
+  const bool active = f < p.H / p.group * slices;                   // (a wave without work still meets the barriers of the summed roles)
+  const int slice = f % slices, h = active ? f / slices * p.group + member : 0;
   const int segment = blockIdx.z;
-  const int n = p.lengths ? min(max(p.lengths[bi], 0), p.T) : p.T;
   const int begin = segment * p.seg, end = min(begin + p.seg, p.T);
   const Decay decay(p.log_decay[h]);
-  const char* pa = reinterpret_cast<const char*>(r.a.p) + (bi * r.a.sb + (h / r.a.shared) * r.a.sh) * kBytes;
-  const char* pb = reinterpret_cast<const char*>(r.b.p) + (bi * r.b.sb + (h / r.b.shared) * r.b.sh) * kBytes;
-  const char* pc = reinterpret_cast<const char*>(r.c.p) + (bi * r.c.sb + (h / r.c.shared) * r.c.sh) * kBytes;
+  const char* pa = reinterpret_cast<const char*>(r.a.p) + (h / r.a.shared) * r.a.sh * kBytes;
+  const char* pb = reinterpret_cast<const char*>(r.b.p) + (h / r.b.shared) * r.b.sh * kBytes;
+  const char* pc = reinterpret_cast<const char*>(r.c.p) + ((h / r.c.shared) * r.c.sh + slice * 16) * kBytes;
   const int col = slice * 16 + c;                       // this lane's column of S and of c's transposed tile
   const int n0 = slice * 16 + 4 * g;                    // its 4 columns of c's rows and of out
-  const int64_t pair = (int64_t)bi * p.H + h, states = (int64_t)r.M * r.N;
+  const bool has_col = active && col < r.N;
+  const int64_t states = (int64_t)r.M * r.N;
+  const int row_out = p.H / r.fold * r.N, out_bytes = r.out_f32 ? 4 : kBytes;   // elements of one token of out
   const Raw unit = X::one(c - 4 * g);
+  char* const area_a = lds + wave * (STAGED ? G::kArea : 0);
+  char* const area_b = area_a + C * G::kRow;
+  char* const area_c = area_b + C * G::kRow;
+  f32x4* const sums = reinterpret_cast<f32x4*>(lds + (STAGED ? waves * G::kArea : 0));
 
-  f32x4 S[MT];
-  const float* s0 = STATE ? nullptr : p.segments > 1 ? r.seg + (pair * p.segments + segment) * states : r.s0 ? r.s0 + pair * states : nullptr;
-#pragma unroll
-  for (int t = 0; t < MT; ++t) {
-    S[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-    if (s0 && active && (WHOLE || col < r.N))
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int m = 16 * t + 4 * g + e;
-        if (WHOLE || m < r.M) S[t][e] = s0[m * r.sm + col * r.sn];
-      }
-  }
-  // scale g^{i-j} (i = 16 it + c, j = 16 jt + 4g + e; 0 above the diagonal) by it - jt, zs g^{C-1-j+sh}, za g^{i+1-sh}, g^C - 1
-  f32x4 inside[CT], into[CT];
+  // scale g^{i-j} (i = 16 it + c, j = 16 jt + 4g + e; used on and below the diagonal) by it - jt, za g^{i+1-sh}; zs g^{n-1-j+sh} and g^n - 1 for
+  // whole chunks and for the one of `tail` tokens that ends a sequence
+  f32x4 inside[CT], whole_into[CT], tail_into[CT];
   float from[CT];
+  const float whole_keep = expm1f(decay.la * (float)C);
+  float tail_keep = 0.f;
+  int tail = 0;
+  const float g1 = decay.pow(1);
 #pragma unroll
-  for (int t = 0; t < CT; ++t) {
+  for (int t = 0; t < CT; ++t) {   // (the fourth of four neighbouring powers, the others by one more factor each)
+    tail_into[t] = zero;
+    const int d = 16 * t + c - 4 * g, j = 16 * t + 4 * g;
+    if (!STATE) inside[t][3] = p.scale * decay.pow(max(d - 3, 0));
+    whole_into[t][3] = r.zs * decay.pow(C - 4 - j + r.sh);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      if (!STATE) inside[t][e] = p.scale * decay.pow(max(16 * t + c - 4 * g - e, 0));
-      into[t][e] = r.zs * decay.pow(C - 1 - (16 * t + 4 * g + e) + r.sh);
+    for (int e = 2; e >= 0; --e) {
+      if (!STATE) inside[t][e] = d - e > 0 ? inside[t][e + 1] * g1 : p.scale;
+      whole_into[t][e] = whole_into[t][e + 1] * g1;
     }
     from[t] = r.za * decay.pow(16 * t + c + 1 - r.sh);
   }
-  float keep1 = expm1f(decay.la * (float)C);            // S + (g^C - 1) S keeps a slow decay's last bits
 
-  for (int t0 = begin; t0 < end; t0 += C) {
-    const int cnt = active ? min(C, n - t0) : 0;
-    f32x4 acc[CT];
+  auto length = [&](int bi) { return !active || bi >= p.B ? 0 : p.lengths ? min(max(p.lengths[bi], 0), p.T) : p.T; };
+  const char *qa = nullptr, *qb = nullptr, *qc = nullptr;   // of the sequence that is fetched from
+  auto sequence = [&](int bi) {
+    qa = pa + bi * r.a.sb * kBytes;
+    qb = pb + bi * r.b.sb * kBytes;
+    qc = pc + bi * r.c.sb * kBytes;
+  };
+  // The chunk at t0, on its way (behind the last token its row again: those scores lie above every valid token's diagonal and their weights in
+  // the state are 0)
+  u32x4 fa[G::kLoads], fb[G::kLoads], fc[G::kCLoads];
+  Raw av[CT][MT], bv[CT][MT], cv[CT];
+  const int piece = lane % G::kLanes * 16, piece_c = lane % kBytes * 16;                             // bytes into a row
+  const bool piece_live = piece < r.M * kBytes, piece_c_live = slice * 16 * kBytes + piece_c < r.N * kBytes;   // channels behind M, N: zeros
+  auto fetch = [&](int t0, int n) {
+    auto token = [&](int row) {
+      const int idx = min(t0 + row, n - 1);
+      return (int64_t)(r.reverse ? n - 1 - idx : idx);
+    };
+    if constexpr (STAGED) {
 #pragma unroll
-    for (int t = 0; t < CT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-    if (cnt > 0) {
-      if (cnt < C) {
-        keep1 = expm1f(decay.la * (float)cnt);
-#pragma unroll
-        for (int t = 0; t < CT; ++t)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int j = 16 * t + 4 * g + e;
-            into[t][e] = j < cnt ? r.zs * decay.pow(cnt - 1 - j + r.sh) : 0.f;
-          }
+      for (int i = 0; i < G::kLoads; ++i) {
+        const int row = (64 * i + lane) / G::kLanes;
+        if (!STATE) fa[i] = u32x4{0, 0, 0, 0};
+        fb[i] = u32x4{0, 0, 0, 0};
+        if (piece_live && row < C) {
+          const int64_t tok = token(row);
+          if (!STATE) fa[i] = *reinterpret_cast<const u32x4*>(qa + tok * r.a.st * kBytes + piece);
+          fb[i] = *reinterpret_cast<const u32x4*>(qb + tok * r.b.st * kBytes + piece);
+        }
       }
-      // rows (tokens) of a, b, c; behind the last token its row again: those scores lie above every valid token's diagonal and `into` is 0
-      Raw av[CT][MT], bv[CT][MT], cv[CT];
+#pragma unroll
+      for (int i = 0; i < G::kCLoads; ++i) {
+        const int row = (64 * i + lane) / kBytes;
+        fc[i] = u32x4{0, 0, 0, 0};
+        if (piece_c_live && row < C) fc[i] = *reinterpret_cast<const u32x4*>(qc + token(row) * r.c.st * kBytes + piece_c);
+      }
+    } else {
 #pragma unroll
       for (int it = 0; it < CT; ++it) {
-        const int idx = min(t0 + 16 * it + c, n - 1), tok = r.reverse ? n - 1 - idx : idx;
-        const char* ra = pa + ((int64_t)tok * r.a.st + 4 * g) * kBytes;
-        const char* rb = pb + ((int64_t)tok * r.b.st + 4 * g) * kBytes;
-        const char* rc = pc + ((int64_t)tok * r.c.st + n0) * kBytes;
-        if constexpr (WHOLE) {
+        const int64_t tok = token(16 * it + c);
 #pragma unroll
-          for (int t = 0; t < MT; ++t) {
-            if (!STATE) av[it][t] = *reinterpret_cast<const Raw*>(ra + 16 * t * kBytes);
-            bv[it][t] = *reinterpret_cast<const Raw*>(rb + 16 * t * kBytes);
-          }
-          cv[it] = *reinterpret_cast<const Raw*>(rc);
-        } else {
+        for (int t = 0; t < MT; ++t) {
+          const int m = 16 * t + 4 * g;
+          if (!STATE) av[it][t] = load4<T>(qa + (tok * r.a.st + m) * kBytes, r.M - m, r.wide);
+          bv[it][t] = load4<T>(qb + (tok * r.b.st + m) * kBytes, r.M - m, r.wide);
+        }
+        cv[it] = load4<T>(qc + (tok * r.c.st + 4 * g) * kBytes, r.N - n0, r.wide);
+      }
+    }
+  };
+  // from the registers into the wave's LDS (which the wave alone reads; its LDS operations run in order)
+  auto stage = [&]() {
+    if constexpr (STAGED) {
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
 #pragma unroll
-          for (int t = 0; t < MT; ++t) {
-            const int left = r.M - 16 * t - 4 * g;
-            if (!STATE) av[it][t] = load4<T>(ra + 16 * t * kBytes, left, r.wide);
-            bv[it][t] = load4<T>(rb + 16 * t * kBytes, left, r.wide);
-          }
-          cv[it] = load4<T>(rc, r.N - n0, r.wide);
+      for (int i = 0; i < G::kLoads; ++i) {
+        const int row = (64 * i + lane) / G::kLanes;
+        if (row < C) {
+          if (!STATE) *reinterpret_cast<u32x4*>(area_a + row * G::kRow + piece) = fa[i];
+          *reinterpret_cast<u32x4*>(area_b + row * G::kRow + piece) = fb[i];
         }
       }
-      f32x4 cf[CT];                                      // c by columns: tokens 4g .. 4g+3 of column `col`
 #pragma unroll
-      for (int t = 0; t < CT; ++t) cf[t] = X::raw(cv[t], unit, f32x4{0.f, 0.f, 0.f, 0.f});
-      if constexpr (!STATE) {
-        // scores[jt][it][j][i] = b_j . a_i
-        typename X::Split ps[CT][CT];
+      for (int i = 0; i < G::kCLoads; ++i) {
+        const int row = (64 * i + lane) / kBytes;
+        if (row < C) *reinterpret_cast<u32x4*>(area_c + row * G::kCRow + piece_c) = fc[i];
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+    }
+  };
+  auto A = [&](int it, int t) { if constexpr (STAGED) return *reinterpret_cast<const Raw*>(area_a + (16 * it + c) * G::kRow + (16 * t + 4 * g) * kBytes); else return av[it][t]; };
+  auto Bt = [&](int it, int t) { if constexpr (STAGED) return *reinterpret_cast<const Raw*>(area_b + (16 * it + c) * G::kRow + (16 * t + 4 * g) * kBytes); else return bv[it][t]; };
+  auto Ct = [&](int it) { if constexpr (STAGED) return *reinterpret_cast<const Raw*>(area_c + (16 * it + c) * G::kCRow + 4 * g * kBytes); else return cv[it]; };
+
+  int n = length(bgroup), n_next = 0;
+  sequence(bgroup);
+  if (begin < n) fetch(begin, n);
+  int turn = 0;
+  for (int bi = bgroup; bi < p.B; bi += p.bgroups, n = n_next) {
+    n_next = length(bi + p.bgroups);
+    const int64_t pair = (int64_t)bi * p.H + h;
+    const float* s0 = STATE ? nullptr : p.segments > 1 ? r.seg + (pair * p.segments + segment) * states : r.s0 ? r.s0 + pair * states : nullptr;
+    f32x4 S[MT];
 #pragma unroll
-        for (int it = 0; it < CT; ++it)
+    for (int t = 0; t < MT; ++t) {
+      S[t] = zero;
+      if (s0 && has_col)
 #pragma unroll
-          for (int jt = 0; jt <= it; ++jt) {
-            f32x4 x = {0.f, 0.f, 0.f, 0.f};
-            if constexpr (MT == 1) {
-              x = X::raw(bv[jt][0], av[it][0], x);
-            } else {
+        for (int e = 0; e < 4; ++e) {
+          const int m = 16 * t + 4 * g + e;
+          if (m < r.M) S[t][e] = s0[m * r.sm + col * r.sn];
+        }
+    }
+    for (int t0 = begin; t0 < end; t0 += C, ++turn) {
+      const int cnt = min(C, n - t0);
+      f32x4 acc[CT], cf[CT], x[CT][CT];
+      Op bt[STAGED ? 1 : MT][CT];
 #pragma unroll
-              for (int t = 0; t < MT; t += 2) x = X::raw2(bv[jt][t], bv[jt][t + 1], av[it][t], av[it][t + 1], x);
-            }
+      for (int t = 0; t < CT; ++t) acc[t] = zero;
+      auto next = [&]() {   // the next chunk, of this sequence or of the wave's next one
+        const bool more = t0 + C < end;
+        const int t1 = more ? t0 + C : begin, n1 = more ? n : n_next;
+        if (!more) sequence(bi + p.bgroups);
+        if (t1 < n1) fetch(t1, n1);
+      };
+      if (STAGED) {
+        if (cnt > 0) stage();
+        next();
+      }
+      if (cnt > 0) {
+        // c by columns: tokens 4g .. 4g+3 of column `col`
 #pragma unroll
-            for (int e = 0; e < 4; ++e) x[e] = jt < it || 4 * g + e <= c ? x[e] * inside[it - jt][e] : 0.f;
-            ps[jt][it] = X::split(x);
-          }
-        // acc[it][n][i] = za g^{i+1-sh} sum_m S[m][n] a_i[m]
+        for (int t = 0; t < CT; ++t) cf[t] = X::raw(Ct(t), unit, zero);
+        if constexpr (!STATE) {
+          // scores x[jt][it][j][i] = b_j . a_i, and acc[it][n][i] = sum_m S[m][n] a_i[m]
 #pragma unroll
-        for (int t = 0; t < MT; t += 2) {
-          const typename X::Split s = X::split(S[t]);
+          for (int it = 0; it < CT; ++it)
+#pragma unroll
+            for (int jt = 0; jt <= it; ++jt) x[jt][it] = zero;
           if constexpr (MT == 1) {
+            Raw a[CT], b[CT];
+            const typename X::Split s = X::split(S[0]);
 #pragma unroll
-            for (int it = 0; it < CT; ++it) acc[it] = X::state(s, X::op(av[it][0]), acc[it]);
+            for (int it = 0; it < CT; ++it) {
+              a[it] = A(it, 0);
+              b[it] = Bt(it, 0);
+#pragma unroll
+              for (int jt = 0; jt <= it; ++jt) x[jt][it] = X::raw(b[jt], a[it], zero);
+              acc[it] = X::state(s, X::op(a[it]), zero);
+            }
           } else {
-            const typename X::Split u = X::split(S[t + 1]);
 #pragma unroll
-            for (int it = 0; it < CT; ++it) acc[it] = X::state2(s, u, X::op(av[it][t]), X::op(av[it][t + 1]), acc[it]);
+            for (int t = 0; t < MT; t += 2) {
+              Raw a0[CT], a1[CT], b0[CT], b1[CT];
+              const typename X::Split s = X::split(S[t]), u = X::split(S[t + 1]);
+#pragma unroll
+              for (int it = 0; it < CT; ++it) {
+                a0[it] = A(it, t);
+                a1[it] = A(it, t + 1);
+                b0[it] = Bt(it, t);
+                b1[it] = Bt(it, t + 1);
+#pragma unroll
+                for (int jt = 0; jt <= it; ++jt) x[jt][it] = X::raw2(b0[jt], b1[jt], a0[it], a1[it], x[jt][it]);
+                acc[it] = X::state2(s, u, X::op(a0[it]), X::op(a1[it]), acc[it]);
+              }
+            }
           }
         }
-        Op co[CT];
-        bool odd = false;
+        if constexpr (!STAGED) {
+#pragma unroll
+          for (int t = 0; t < MT; ++t)
+#pragma unroll
+            for (int jt = 0; jt < CT; ++jt) bt[t][jt] = X::op_of(X::raw(bv[jt][t], unit, zero));
+        }
+      }
+      if (!STAGED) next();   // (a, b, c are used up)
+      if (cnt > 0) {
+        if constexpr (!STATE) {
+          typename X::Split ps[CT][CT];
+#pragma unroll
+          for (int it = 0; it < CT; ++it)
+#pragma unroll
+            for (int jt = 0; jt <= it; ++jt) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) x[jt][it][e] = jt < it || 4 * g + e <= c ? x[jt][it][e] * inside[it - jt][e] : 0.f;
+              ps[jt][it] = X::split(x[jt][it]);
+            }
+          Op co[CT];
+          float top = 0.f;
+#pragma unroll
+          for (int t = 0; t < CT; ++t) {
+            acc[t] *= from[t];
+            co[t] = X::op_of(cf[t]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) top = __builtin_elementwise_maximum(top, __builtin_fabsf(cf[t][e]));   // (a NaN stays)
+          }
+          // acc[it][n][i] += sum_j c_j[n] scores[j][i].  A later token's infinity or NaN must not reach an earlier token's sum as 0 * inf: a
+          // chunk that holds one goes token by token
+          auto inner = [&](int it, Op last, f32x4 y) {
+            if constexpr (CT == 1) return X::score(last, ps[0][0], y);
+            else return it == 0 ? X::score(last, ps[0][0], y) : X::score2(co[0], last, ps[0][1], ps[1][1], y);
+          };
+          if (__builtin_expect(__any(!(top <= 3.4028234e38f)), 0)) {
+#pragma unroll
+            for (int it = 0; it < CT; ++it) {
+              const f32x4 before = acc[it];
+#pragma unroll 1
+              for (int i = 0; i < 16; ++i) {
+                const f32x4 y = inner(it, X::upto(co[it], i + 1 - 4 * g), before);
+                if (c == i) acc[it] = y;
+              }
+            }
+          } else {
+#pragma unroll
+            for (int it = 0; it < CT; ++it) acc[it] = inner(it, co[it], acc[it]);
+          }
+        }
+        if (cnt < C && cnt != tail) {
+          tail = cnt;
+          tail_keep = expm1f(decay.la * (float)cnt);
+#pragma unroll
+          for (int t = 0; t < CT; ++t) {
+            const int d = cnt - 1 - 16 * t - 4 * g;   // tokens behind the first of the four
+            const float w0 = r.zs * decay.pow(r.sh);
+            float w = r.zs * decay.pow(max(d - 3, 0) + r.sh);
+#pragma unroll
+            for (int e = 3; e >= 0; --e) {
+              if (e < 3) w = d - e > 0 ? w * g1 : w0;
+              tail_into[t][e] = d - e >= 0 ? w : 0.f;
+            }
+          }
+        }
+        // S[m][n] = g^n S[m][n] + sum_j b_j[m] (into_j c_j[n]); S + (g^n - 1) S keeps a slow decay's last bits
+        typename X::Split3 ws[CT];
+#pragma unroll
+        for (int t = 0; t < CT; ++t) ws[t] = X::split3(cf[t] * (cnt < C ? tail_into[t] : whole_into[t]));
+        const float keep = cnt < C ? tail_keep : whole_keep;
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+          Op b[CT];   // b by columns: tokens 4g .. 4g+3 of column 16 t + c
+#pragma unroll
+          for (int jt = 0; jt < CT; ++jt) {
+            if constexpr (STAGED) b[jt] = X::op_of(X::raw(Bt(jt, t), unit, zero));
+            else b[jt] = bt[t][jt];
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) S[t][e] = fmaf(S[t][e], keep, S[t][e]);
+          if constexpr (CT == 1) S[t] = X::add(b[0], ws[0], S[t]);
+          else S[t] = X::add2(b[0], b[1], ws[0], ws[1], S[t]);
+        }
+      }
+      if constexpr (!STATE) {
+        bool writes = active;
+        if (r.fold > 1) {   // (uniform over the launch's role) the heads of one stored head add up in the first one's wave
+          f32x4* const buf = sums + (turn & 1) * waves * CT * 64;
+#pragma unroll
+          for (int t = 0; t < CT; ++t) buf[(wave * CT + t) * 64 + lane] = acc[t];
+          __syncthreads();   // (two buffers: who writes this one again has passed the next barrier, and so have its readers)
+          writes = active && member == 0;
+          if (writes)
+            for (int k = 1; k < r.fold; ++k)
+#pragma unroll
+              for (int t = 0; t < CT; ++t) acc[t] += buf[((wave + k) * CT + t) * 64 + lane];
+        }
+        // (tokens behind the sequence's length get zeros)
+        char* const base = reinterpret_cast<char*>(r.out) + ((int64_t)bi * p.T * row_out + h / r.fold * r.N) * out_bytes;
 #pragma unroll
         for (int t = 0; t < CT; ++t) {
-          acc[t] *= from[t];
-          co[t] = X::op_of(cf[t]);
+          const int idx = t0 + 16 * t + c;
+          if (!writes || idx >= end || n0 >= r.N) continue;
+          if (idx >= n) acc[t] = zero;
+          const int tok = r.reverse && idx < n ? n - 1 - idx : idx;
+          char* const o = base + ((int64_t)tok * row_out + n0) * out_bytes;
+          if (kBytes == 4 || out_bytes == 4) {
+            if (STAGED || r.wide) *reinterpret_cast<f32x4*>(o) = acc[t];
+            else
 #pragma unroll
-          for (int e = 0; e < 4; ++e) odd |= !(__builtin_fabsf(cf[t][e]) <= 3.4028234e38f);
-        }
-        // acc[it][n][i] += sum_j c_j[n] scores[j][i].  A later token's infinity or NaN must not reach an earlier token's sum as 0 * inf: a
-        // chunk that holds one goes token by token
-        auto inner = [&](int it, Op last, f32x4 x) {
-          if constexpr (CT == 1) return X::score(last, ps[0][0], x);
-          else return it == 0 ? X::score(last, ps[0][0], x) : X::score2(co[0], last, ps[0][1], ps[1][1], x);
-        };
-        if (__builtin_expect(__any(odd), 0)) {
+              for (int e = 0; e < 4; ++e)
+                if (n0 + e < r.N) reinterpret_cast<float*>(o)[e] = acc[t][e];
+          } else if constexpr (kBytes == 2) {
+            const s16x4 v = X::to_out(acc[t]);
+            if (STAGED || r.wide) *reinterpret_cast<s16x4*>(o) = v;
+            else
 #pragma unroll
-          for (int it = 0; it < CT; ++it) {
-            const f32x4 before = acc[it];
-            for (int i = 0; i < 16; ++i) {
-              const f32x4 x = inner(it, X::upto(co[it], i + 1 - 4 * g), before);
-              if (c == i) acc[it] = x;
-            }
+              for (int e = 0; e < 4; ++e)
+                if (n0 + e < r.N) reinterpret_cast<short*>(o)[e] = v[e];
           }
-        } else {
-#pragma unroll
-          for (int it = 0; it < CT; ++it) acc[it] = inner(it, co[it], acc[it]);
-        }
-      }
-      // S[m][n] = g^n S[m][n] + sum_j b_j[m] (into_j c_j[n])
-      typename X::Split3 ws[CT];
-#pragma unroll
-      for (int t = 0; t < CT; ++t) ws[t] = X::split3(cf[t] * into[t]);
-#pragma unroll
-      for (int t = 0; t < MT; ++t) {
-        Op bt[CT];
-#pragma unroll
-        for (int jt = 0; jt < CT; ++jt) bt[jt] = X::op_of(X::raw(bv[jt][t], unit, f32x4{0.f, 0.f, 0.f, 0.f}));
-#pragma unroll
-        for (int e = 0; e < 4; ++e) S[t][e] = fmaf(S[t][e], keep1, S[t][e]);
-        if constexpr (CT == 1) S[t] = X::add(bt[0], ws[0], S[t]);
-        else S[t] = X::add2(bt[0], bt[1], ws[0], ws[1], S[t]);
-      }
-    }
-    if constexpr (!STATE) {
-      bool writes = active;
-      if (r.fold > 1) {   // (uniform over the launch's role) the heads of one stored head add up in the first one's wave
-        const int buf = (t0 / C) & 1;
-#pragma unroll
-        for (int t = 0; t < CT; ++t) sums[buf][wave][t][lane] = acc[t];
-        __syncthreads();   // (two buffers: who writes this one again has passed the next barrier, and so have its readers)
-        writes = active && member == 0;
-        if (writes)
-          for (int k = 1; k < r.fold; ++k)
-#pragma unroll
-            for (int t = 0; t < CT; ++t) acc[t] += sums[buf][wave + k][t][lane];
-      }
-      // (tokens behind the sequence's length get zeros)
-#pragma unroll
-      for (int t = 0; t < CT; ++t) {
-        const int idx = t0 + 16 * t + c;
-        if (!writes || idx >= end || (!WHOLE && n0 >= r.N)) continue;
-        if (idx >= n) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-        const int tok = r.reverse && idx < n ? n - 1 - idx : idx;
-        const int64_t at = (((int64_t)bi * p.T + tok) * (p.H / r.fold) + h / r.fold) * r.N + n0;
-        if (r.out_f32 || kBytes == 4) {
-          float* o = reinterpret_cast<float*>(r.out) + at;
-          if (WHOLE || r.wide) *reinterpret_cast<f32x4*>(o) = acc[t];
-          else
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (n0 + e < r.N) o[e] = acc[t][e];
-        } else if constexpr (kBytes == 2) {
-          s16x4 v;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] = (short)f32_to_bits16<T>(acc[t][e]);
-          short* o = reinterpret_cast<short*>(r.out) + at;
-          if (WHOLE || r.wide) *reinterpret_cast<s16x4*>(o) = v;
-          else
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (n0 + e < r.N) o[e] = v[e];
         }
       }
     }
+    float* s1 = STATE ? r.seg + (pair * p.segments + segment + 1) * states : segment == p.segments - 1 && r.s1 ? r.s1 + pair * states : nullptr;
+    if (s1 && has_col)
+#pragma unroll
+      for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int m = 16 * t + 4 * g + e;
+          if (m < r.M) s1[m * r.sm + col * r.sn] = S[t][e];
+        }
   }
-  float* s1 = STATE ? r.seg + (pair * p.segments + segment + 1) * states : segment == p.segments - 1 && r.s1 ? r.s1 + pair * states : nullptr;
-  if (s1 && active && (WHOLE || col < r.N))
-#pragma unroll
-    for (int t = 0; t < MT; ++t)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int m = 16 * t + 4 * g + e;
-        if (WHOLE || m < r.M) s1[m * r.sm + col * r.sn] = S[t][e];
-      }
 }
 
 // the state in front of every segment, from each segment's own (written one place further on) and the first state: in place.  A workgroup
@@ -461,7 +601,10 @@ __global__ __launch_bounds__(1024) void la_scan_kernel(LaArgs p) {
   const bool live = at < states;
   float* seg = r.seg + pair * p.segments * states + at;
   const int K = (p.segments - 1 + 15) / 16, s_begin = min(z * K, p.segments - 1), s_end = min(s_begin + K, p.segments - 1);
-  auto tokens = [&](int s) { return min(max(n - s * p.seg, 0), p.seg); };   // of segment s
+  // the decay over segment s: whole, the one that holds the sequence's end, or behind it
+  const int last = n / p.seg;
+  const float over = decay.pow(p.seg), part = decay.pow(n - last * p.seg);
+  auto fade = [&](int s) { return s < last ? over : s == last ? part : 1.f; };
   auto count = [&](int a, int b) { return min(max(n - a * p.seg, 0), (b - a) * p.seg); };   // of segments a .. b - 1 (all but the last are whole)
   float own[kMaxSegments / 16], run = 0.f;
 #pragma unroll
@@ -469,7 +612,7 @@ __global__ __launch_bounds__(1024) void la_scan_kernel(LaArgs p) {
     if (s_begin + k < s_end && live) own[k] = seg[(int64_t)(s_begin + k + 1) * states];
 #pragma unroll
   for (int k = 0; k < kMaxSegments / 16; ++k)
-    if (s_begin + k < s_end && live) run = fmaf(decay.pow(tokens(s_begin + k)), run, own[k]);
+    if (s_begin + k < s_end && live) run = fmaf(fade(s_begin + k), run, own[k]);
   total[z][x] = run;
   __syncthreads();
   const float first = r.s0 && live ? r.s0[pair * states + at] : 0.f;
@@ -483,7 +626,7 @@ __global__ __launch_bounds__(1024) void la_scan_kernel(LaArgs p) {
 #pragma unroll
   for (int k = 0; k < kMaxSegments / 16; ++k)
     if (s_begin + k < s_end) {
-      run = fmaf(decay.pow(tokens(s_begin + k)), run, own[k]);
+      run = fmaf(fade(s_begin + k), run, own[k]);
       seg[(int64_t)(s_begin + k + 1) * states] = run;
     }
 }
@@ -561,9 +704,10 @@ constexpr int kFold = 4;   // shared heads that are summed inside a workgroup; m
 
 inline int tiles(int m) { return m <= 16 ? 1 : m <= 32 ? 2 : m <= 64 ? 4 : 8; }
 
-// Waves that the machine wants at once, and the fewest tokens that are worth a segment
+// Segments: as many as two waves per SIMD need, each of at least kMinSegment tokens
 constexpr int64_t kWaves = 2048;
 constexpr int kMinSegment = 128;
+constexpr int kCUs = 256;
 
 // (tokens in a segment, segments) for `waves` waves per segment
 void segmentation(int T, int64_t waves, int* seg, int* segments) {
@@ -577,44 +721,72 @@ void segmentation(int T, int64_t waves, int* seg, int* segments) {
   *segments = (int)((T + s - 1) / s);
 }
 
-template <typename T, int MT, int CT, bool STATE> int go(const LaArgs& a, bool whole, dim3 grid, int threads, hipStream_t st) {
-  if (whole) la_kernel<T, MT, CT, true, STATE><<<grid, threads, 0, st>>>(a);
-  else la_kernel<T, MT, CT, false, STATE><<<grid, threads, 0, st>>>(a);
+// One launch.  Sequences are dealt out so that the grid fills the machine ONCE (a wave makes its decay's powers once, and no second round of
+// workgroups finds the machine half empty: 4096 waves where 3072 fit ran 338 us, 3072 run XXX us)
+template <typename T, int MT, int CT, bool STAGED, bool STATE> int go(LaArgs a, dim3 grid, int threads, hipStream_t st) {
+  const int waves = threads / 64, folds = !STATE && a.group > 1;
+  const int lds = (folds ? 2 * waves * CT * 64 * 16 : 0) + (STAGED ? waves * Stage<T, MT, CT>::kArea : 0);
+  const auto kernel = la_kernel<T, MT, CT, STAGED, STATE>;
+  static std::atomic<int> resident[2][kFold + 1];   // workgroups of a CU, by folds and waves; 0: not known yet
+  int per_cu = resident[folds][waves].load(std::memory_order_relaxed);
+  if (per_cu == 0) {
+    TG_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
+    TG_CHECK_HIP(hipOccupancyMaxActiveBlocksPerMultiprocessor(&per_cu, reinterpret_cast<const void*>(kernel), threads, (size_t)lds));
+    if (per_cu < 1) return TG_E_UNSUPPORTED;
+    resident[folds][waves].store(per_cu, std::memory_order_relaxed);
+  }
+  const int64_t columns = a.columns, others = columns * grid.y * grid.z, room = (int64_t)per_cu * kCUs;
+  const int64_t each = (a.B * others + room - 1) / room;             // sequences of a workgroup
+  a.bgroups = (int)((a.B + each - 1) / each);
+  if (columns * a.bgroups > 0x7fffffff) return TG_E_UNSUPPORTED;
+  grid.x = (unsigned)(columns * a.bgroups);
+  kernel<<<grid, threads, lds, st>>>(a);
   return tg_launch_status();
 }
-template <typename T, int MT> int go_mt(const LaArgs& a, bool whole, bool state, dim3 grid, int threads, hipStream_t st) {
-  // chunks of 32 tokens halve the work on the state per token; sequences of one chunk of 16 would waste half of them
-  if (state) return go<T, MT, 2, true>(a, whole, grid, threads, st);
-  return a.T <= 16 ? go<T, MT, 1, false>(a, whole, grid, threads, st) : go<T, MT, 2, false>(a, whole, grid, threads, st);
+template <typename T, int MT, int CT, bool STATE> int go_staged(const LaArgs& a, bool staged, dim3 grid, int threads, hipStream_t st) {
+  return staged ? go<T, MT, CT, true, STATE>(a, grid, threads, st) : go<T, MT, CT, false, STATE>(a, grid, threads, st);
+}
+template <typename T, int MT> int go_mt(const LaArgs& a, bool staged, bool state, dim3 grid, int threads, hipStream_t st) {
+  // chunks of 32 tokens halve the work on the state per token; sequences of one chunk of 16 would waste half of them, and 128 fp32
+  // channels do not fit the registers twice
+  constexpr int CT = MT == 8 && sizeof(typename Mat<T>::Raw) == 16 ? 1 : 2;
+  if (state) return go_staged<T, MT, CT, true>(a, staged, grid, threads, st);
+  return a.T <= 16 ? go_staged<T, MT, 1, false>(a, staged, grid, threads, st) : go_staged<T, MT, CT, false>(a, staged, grid, threads, st);
 }
 // `roles` roles with the same number of m tiles in one launch
-template <typename T> int launch(const LaArgs& a, int roles, bool state, hipStream_t st) {
+template <typename T> int launch(LaArgs a, int roles, bool state, hipStream_t st) {
   int mt = 1, slices = 1;
-  bool whole = true;
+  bool staged = true;
   for (int i = 0; i < roles; ++i) {
     const Role& r = a.r[i];
     if (tiles(r.M) > mt) mt = tiles(r.M);
     if ((r.N + 15) / 16 > slices) slices = (r.N + 15) / 16;
   }
-  for (int i = 0; i < roles; ++i) whole = whole && a.r[i].wide && a.r[i].M == 16 * mt && a.r[i].N % 16 == 0;
-  const int per = kFold / a.group, threads = 64 * per * a.group;
-  const int64_t wgs = ((int64_t)a.B * (a.H / a.group) * slices + per - 1) / per;
-  if ((int64_t)a.B * a.H * slices > 0x7fffffff - 64) return TG_E_UNSUPPORTED;
-  const dim3 grid((unsigned)wgs, roles, state ? a.segments - 1 : a.segments);
-  if (mt == 1) return go_mt<T, 1>(a, whole, state, grid, threads, st);
-  if (mt == 2) return go_mt<T, 2>(a, whole, state, grid, threads, st);
-  if (mt == 4) return go_mt<T, 4>(a, whole, state, grid, threads, st);
-  return go_mt<T, 8>(a, whole, state, grid, threads, st);
+  for (int i = 0; i < roles; ++i) staged = staged && a.r[i].pieces;
+  // workgroups of up to kFold waves, as few idle ones among them as possible
+  const int64_t units = (int64_t)(a.H / a.group) * slices;
+  if (units > 0x7fffff00) return TG_E_UNSUPPORTED;
+  int per = 1;
+  for (int k = 2; k <= kFold / a.group; ++k)
+    if ((units + k - 1) / k * k <= (units + per - 1) / per * per) per = k;
+  a.columns = (int)((units + per - 1) / per);
+  const dim3 grid(1, roles, state ? a.segments - 1 : a.segments);
+  const int threads = 64 * per * a.group;
+  if (mt == 1) return go_mt<T, 1>(a, staged, state, grid, threads, st);
+  if (mt == 2) return go_mt<T, 2>(a, staged, state, grid, threads, st);
+  if (mt == 4) return go_mt<T, 4>(a, staged, state, grid, threads, st);
+  return go_mt<T, 8>(a, staged, state, grid, threads, st);
 }
 int launch_dt(int dtype, const LaArgs& a, int roles, bool state, hipStream_t st) {
   TG_DISPATCH_DTYPE(dtype, return launch<BF16>(a, roles, state, st), return launch<F16>(a, roles, state, st), return launch<F32>(a, roles, state, st));
 }
 
-struct Strided { Operand o; bool wide; };
+struct Strided { Operand o; bool wide, pieces; };   // aligned to 4 elements, to 16 bytes: the address and all strides
 Strided operand(int dtype, const void* p, const int64_t* stride, int shared) {
-  const int bytes = 4 * elem_bytes(dtype);
-  const bool wide = ((reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0) && stride[0] % 4 == 0 && stride[1] % 4 == 0 && stride[2] % 4 == 0;
-  return {Operand{p, stride[0], stride[2], (int)stride[1], shared}, wide};
+  auto aligned = [&](int n) {
+    return (reinterpret_cast<uintptr_t>(p) & (n * elem_bytes(dtype) - 1)) == 0 && stride[0] % n == 0 && stride[1] % n == 0 && stride[2] % n == 0;
+  };
+  return {Operand{p, stride[0], stride[2], (int)stride[1], shared}, aligned(4), aligned(16 / elem_bytes(dtype))};
 }
 
 int check(int dtype, const tg_la_desc* d) {
@@ -672,7 +844,9 @@ extern "C" int tg_linear_attention(int dtype, const tg_la_desc* d, const void* q
   a.group = 1;
   a.scale = d->scale;
   const bool wide = Q.wide && K.wide && V.wide && d->DK % 4 == 0 && d->DV % 4 == 0 && (reinterpret_cast<uintptr_t>(o) & (4 * elem_bytes(dtype) - 1)) == 0;
-  a.r[0] = Role{Q.o, K.o, V.o, o, state_in, state_out, scratch, d->DK, d->DV, d->DV, 1, d->scale, 1.f, 0, 0, 1, 0, wide};
+  const int piece = 16 / elem_bytes(dtype);
+  const bool pieces = wide && Q.pieces && K.pieces && V.pieces && d->DK % piece == 0 && d->DV % piece == 0;
+  a.r[0] = Role{Q.o, K.o, V.o, o, state_in, state_out, scratch, d->DK, d->DV, d->DV, 1, d->scale, 1.f, 0, 0, 1, 0, wide, pieces};
   if (a.segments > 1 && (rc = join_segments(dtype, a, 1, st)) != TG_OK) return rc;
   return launch_dt(dtype, a, 1, false, st);
 }
@@ -718,14 +892,16 @@ extern "C" int tg_linear_attention_bwd(int dtype, const tg_la_desc* d, const voi
   bool wide = Q.wide && K.wide && V.wide && D.wide && DK % 4 == 0 && DV % 4 == 0;
   for (const void* p : {(const void*)dq, (const void*)(apart ? part_k : dk), (const void*)(apart ? part_v : dv)})
     wide = wide && (reinterpret_cast<uintptr_t>(p) & 15) == 0;
+  const int piece = 16 / elem_bytes(dtype);
+  const bool pieces = wide && Q.pieces && K.pieces && V.pieces && D.pieces && DK % piece == 0 && DV % piece == 0;
   if (a.segments > 1) {
-    a.r[0] = Role{Q.o, K.o, V.o, nullptr, state_in, nullptr, seg_s, DK, DV, DV, 1, 0.f, 1.f, 0, 0, 1, 0, wide};
-    a.r[1] = Role{K.o, Q.o, D.o, nullptr, dstate_out, nullptr, seg_d, DK, DV, DV, 1, 0.f, d->scale, 1, 1, 1, 0, wide};
+    a.r[0] = Role{Q.o, K.o, V.o, nullptr, state_in, nullptr, seg_s, DK, DV, DV, 1, 0.f, 1.f, 0, 0, 1, 0, wide, pieces};
+    a.r[1] = Role{K.o, Q.o, D.o, nullptr, dstate_out, nullptr, seg_d, DK, DV, DV, 1, 0.f, d->scale, 1, 1, 1, 0, wide, pieces};
     if ((rc = join_segments(dtype, a, 2, st)) != TG_OK) return rc;
   }
-  const Role rq{D.o, V.o, K.o, dq, state_in, nullptr, seg_s, DV, DK, 1, DV, d->scale, 1.f, 0, 0, 1, 0, wide};
-  const Role rk{V.o, D.o, Q.o, apart ? (void*)part_k : dk, dstate_out, nullptr, seg_d, DV, DK, 1, DV, 1.f, d->scale, 1, 1, fold, apart, wide};
-  const Role rv{K.o, Q.o, D.o, apart ? (void*)part_v : dv, dstate_out, dstate_in, seg_d, DK, DV, DV, 1, 1.f, d->scale, 1, 1, fold, apart, wide};
+  const Role rq{D.o, V.o, K.o, dq, state_in, nullptr, seg_s, DV, DK, 1, DV, d->scale, 1.f, 0, 0, 1, 0, wide, pieces};
+  const Role rk{V.o, D.o, Q.o, apart ? (void*)part_k : dk, dstate_out, nullptr, seg_d, DV, DK, 1, DV, 1.f, d->scale, 1, 1, fold, apart, wide, pieces};
+  const Role rv{K.o, Q.o, D.o, apart ? (void*)part_v : dv, dstate_out, dstate_in, seg_d, DK, DV, DV, 1, 1.f, d->scale, 1, 1, fold, apart, wide, pieces};
   a.r[0] = rq;
   a.r[1] = rk;
   a.r[2] = rv;
