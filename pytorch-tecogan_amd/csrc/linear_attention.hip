@@ -242,6 +242,7 @@ template <typename T, int MT, int CT> struct Stage {
   static constexpr int kRow = 16 * kLanes + 16;                   // bytes between rows: 16 rows x 16 bytes hit every bank once
   static constexpr int kCRow = 16 * kBytes + 16;                  // the same for c: 16 columns
   static constexpr int kLoads = (C * kLanes + 63) / 64, kCLoads = (C * kBytes + 63) / 64;
+  static constexpr int kRows = C < 64 / kLanes ? C : 64 / kLanes, kCRows = C < 64 / kBytes ? C : 64 / kBytes;   // rows of one load
   static constexpr int kArea = C * (2 * kRow + kCRow);            // LDS of a wave
 };
 
@@ -315,33 +316,56 @@ template <typename T, int MT, int CT, bool STAGED, bool STATE> __global__ __laun
   Raw av[CT][MT], bv[CT][MT], cv[CT];
   const int piece = lane % G::kLanes * 16, piece_c = lane % kBytes * 16;                             // bytes into a row
   const bool piece_live = piece < r.M * kBytes, piece_c_live = slice * 16 * kBytes + piece_c < r.N * kBytes;   // channels behind M, N: zeros
+  const int row_a = lane / G::kLanes, row_c = lane / kBytes;                                          // of each load
+  const bool live_a = piece_live && row_a < C, live_c = piece_c_live && row_c < C;
+  // bytes from the lowest of a load's tokens to this lane's row
+  const int up_a = r.reverse ? G::kRows - 1 - row_a : row_a, up_c = r.reverse ? G::kCRows - 1 - row_c : row_c;
+  const unsigned va = (unsigned)(up_a * r.a.st * kBytes + piece), vb = (unsigned)(up_a * r.b.st * kBytes + piece), vc = (unsigned)(up_c * r.c.st * kBytes + piece_c);
   auto fetch = [&](int t0, int n) {
-    auto token = [&](int row) {
-      const int idx = min(t0 + row, n - 1);
-      return (int64_t)(r.reverse ? n - 1 - idx : idx);
-    };
     if constexpr (STAGED) {
 #pragma unroll
       for (int i = 0; i < G::kLoads; ++i) {
-        const int row = (64 * i + lane) / G::kLanes;
         if (!STATE) fa[i] = u32x4{0, 0, 0, 0};
         fb[i] = u32x4{0, 0, 0, 0};
-        if (piece_live && row < C) {
-          const int64_t tok = token(row);
-          if (!STATE) fa[i] = *reinterpret_cast<const u32x4*>(qa + tok * r.a.st * kBytes + piece);
-          fb[i] = *reinterpret_cast<const u32x4*>(qb + tok * r.b.st * kBytes + piece);
-        }
       }
 #pragma unroll
-      for (int i = 0; i < G::kCLoads; ++i) {
-        const int row = (64 * i + lane) / kBytes;
-        fc[i] = u32x4{0, 0, 0, 0};
-        if (piece_c_live && row < C) fc[i] = *reinterpret_cast<const u32x4*>(qc + token(row) * r.c.st * kBytes + piece_c);
+      for (int i = 0; i < G::kCLoads; ++i) fc[i] = u32x4{0, 0, 0, 0};
+      if (t0 + C <= n) {   // a whole chunk: uniform addresses, every lane its own fixed place
+        if (live_a)
+#pragma unroll
+          for (int i = 0; i < G::kLoads; ++i) {
+            const int64_t tok = r.reverse ? n - t0 - (i + 1) * G::kRows : t0 + i * G::kRows;
+            if (!STATE) fa[i] = *reinterpret_cast<const u32x4*>(qa + tok * r.a.st * kBytes + va);
+            fb[i] = *reinterpret_cast<const u32x4*>(qb + tok * r.b.st * kBytes + vb);
+          }
+        if (live_c)
+#pragma unroll
+          for (int i = 0; i < G::kCLoads; ++i) {
+            const int64_t tok = r.reverse ? n - t0 - (i + 1) * G::kCRows : t0 + i * G::kCRows;
+            fc[i] = *reinterpret_cast<const u32x4*>(qc + tok * r.c.st * kBytes + vc);
+          }
+      } else {
+        auto token = [&](int row) {
+          const int idx = min(t0 + row, n - 1);
+          return (int64_t)(r.reverse ? n - 1 - idx : idx);
+        };
+        if (live_a)
+#pragma unroll
+          for (int i = 0; i < G::kLoads; ++i) {
+            const int64_t tok = token(i * G::kRows + row_a);
+            if (!STATE) fa[i] = *reinterpret_cast<const u32x4*>(qa + tok * r.a.st * kBytes + piece);
+            fb[i] = *reinterpret_cast<const u32x4*>(qb + tok * r.b.st * kBytes + piece);
+          }
+        if (live_c)
+#pragma unroll
+          for (int i = 0; i < G::kCLoads; ++i)
+            fc[i] = *reinterpret_cast<const u32x4*>(qc + token(i * G::kCRows + row_c) * r.c.st * kBytes + piece_c);
       }
     } else {
 #pragma unroll
       for (int it = 0; it < CT; ++it) {
-        const int64_t tok = token(16 * it + c);
+        const int idx = min(t0 + 16 * it + c, n - 1);
+        const int64_t tok = r.reverse ? n - 1 - idx : idx;
 #pragma unroll
         for (int t = 0; t < MT; ++t) {
           const int m = 16 * t + 4 * g;
@@ -357,19 +381,15 @@ template <typename T, int MT, int CT, bool STAGED, bool STATE> __global__ __laun
     if constexpr (STAGED) {
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       __builtin_amdgcn_wave_barrier();
+      if (row_a < C)
 #pragma unroll
-      for (int i = 0; i < G::kLoads; ++i) {
-        const int row = (64 * i + lane) / G::kLanes;
-        if (row < C) {
-          if (!STATE) *reinterpret_cast<u32x4*>(area_a + row * G::kRow + piece) = fa[i];
-          *reinterpret_cast<u32x4*>(area_b + row * G::kRow + piece) = fb[i];
+        for (int i = 0; i < G::kLoads; ++i) {
+          if (!STATE) *reinterpret_cast<u32x4*>(area_a + (i * G::kRows + row_a) * G::kRow + piece) = fa[i];
+          *reinterpret_cast<u32x4*>(area_b + (i * G::kRows + row_a) * G::kRow + piece) = fb[i];
         }
-      }
+      if (row_c < C)
 #pragma unroll
-      for (int i = 0; i < G::kCLoads; ++i) {
-        const int row = (64 * i + lane) / kBytes;
-        if (row < C) *reinterpret_cast<u32x4*>(area_c + row * G::kCRow + piece_c) = fc[i];
-      }
+        for (int i = 0; i < G::kCLoads; ++i) *reinterpret_cast<u32x4*>(area_c + (i * G::kCRows + row_c) * G::kCRow + piece_c) = fc[i];
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       __builtin_amdgcn_wave_barrier();
     }
@@ -390,11 +410,12 @@ template <typename T, int MT, int CT, bool STAGED, bool STATE> __global__ __laun
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
       S[t] = zero;
-      if (s0 && has_col)
+      if (s0)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int m = 16 * t + 4 * g + e;
-          if (m < r.M) S[t][e] = s0[m * r.sm + col * r.sn];
+          const float v = s0[min(m, r.M - 1) * r.sm + min(col, r.N - 1) * r.sn];
+          S[t][e] = m < r.M && has_col ? v : 0.f;
         }
     }
     for (int t0 = begin; t0 < end; t0 += C, ++turn) {
@@ -549,27 +570,50 @@ template <typename T, int MT, int CT, bool STAGED, bool STATE> __global__ __laun
               for (int t = 0; t < CT; ++t) acc[t] += buf[((wave + k) * CT + t) * 64 + lane];
         }
         // (tokens behind the sequence's length get zeros)
-        char* const base = reinterpret_cast<char*>(r.out) + ((int64_t)bi * p.T * row_out + h / r.fold * r.N) * out_bytes;
+        char* const base = reinterpret_cast<char*>(r.out) + ((int64_t)bi * p.T * row_out + h / r.fold * r.N + slice * 16) * out_bytes;
+        auto place = [&](int idx) { return base + (int64_t)(r.reverse && idx < n ? n - 1 - idx : idx) * row_out * out_bytes; };
 #pragma unroll
-        for (int t = 0; t < CT; ++t) {
-          const int idx = t0 + 16 * t + c;
-          if (!writes || idx >= end || n0 >= r.N) continue;
-          if (idx >= n) acc[t] = zero;
-          const int tok = r.reverse && idx < n ? n - 1 - idx : idx;
-          char* const o = base + ((int64_t)tok * row_out + n0) * out_bytes;
-          if (kBytes == 4 || out_bytes == 4) {
-            if (STAGED || r.wide) *reinterpret_cast<f32x4*>(o) = acc[t];
-            else
+        for (int t = 0; t < CT; ++t)
+          if (t0 + 16 * t + c >= n) acc[t] = zero;
+        if (STAGED && (kBytes == 4 || out_bytes == kBytes)) {   // through c's place in the LDS: whole rows again, 16 bytes per lane
+          if (writes) {
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
 #pragma unroll
-              for (int e = 0; e < 4; ++e)
-                if (n0 + e < r.N) reinterpret_cast<float*>(o)[e] = acc[t][e];
-          } else if constexpr (kBytes == 2) {
-            const s16x4 v = X::to_out(acc[t]);
-            if (STAGED || r.wide) *reinterpret_cast<s16x4*>(o) = v;
-            else
+            for (int t = 0; t < CT; ++t) {
+              char* const o = area_c + (16 * t + c) * G::kCRow + 4 * g * kBytes;
+              if constexpr (kBytes == 4) *reinterpret_cast<f32x4*>(o) = acc[t];
+              else *reinterpret_cast<s16x4*>(o) = X::to_out(acc[t]);
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
 #pragma unroll
-              for (int e = 0; e < 4; ++e)
-                if (n0 + e < r.N) reinterpret_cast<short*>(o)[e] = v[e];
+            for (int i = 0; i < G::kCLoads; ++i) {
+              const int row = i * G::kCRows + row_c;
+              if (live_c && t0 + row < end)
+                *reinterpret_cast<u32x4*>(place(t0 + row) + piece_c) = *reinterpret_cast<const u32x4*>(area_c + row * G::kCRow + piece_c);
+            }
+          }
+        } else {
+#pragma unroll
+          for (int t = 0; t < CT; ++t) {
+            const int idx = t0 + 16 * t + c;
+            if (!writes || idx >= end || n0 >= r.N) continue;
+            char* const o = place(idx) + 4 * g * out_bytes;
+            if (kBytes == 4 || out_bytes == 4) {
+              if (r.wide) *reinterpret_cast<f32x4*>(o) = acc[t];
+              else
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                  if (n0 + e < r.N) reinterpret_cast<float*>(o)[e] = acc[t][e];
+            } else if constexpr (kBytes == 2) {
+              const s16x4 v = X::to_out(acc[t]);
+              if (r.wide) *reinterpret_cast<s16x4*>(o) = v;
+              else
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                  if (n0 + e < r.N) reinterpret_cast<short*>(o)[e] = v[e];
+            }
           }
         }
       }
@@ -590,44 +634,41 @@ template <typename T, int MT, int CT, bool STAGED, bool STATE> __global__ __laun
 // takes 64 elements of one state; 16 groups of threads take consecutive segments each and meet through LDS
 constexpr int kMaxSegments = 256;
 __global__ __launch_bounds__(1024) void la_scan_kernel(LaArgs p) {
-  __shared__ float total[16][64];
+  __shared__ float total[16][64], fades[16];
   const Role& r = p.r[blockIdx.z];
-  const int states = r.M * r.N, x = threadIdx.x & 63, z = threadIdx.x >> 6, at = blockIdx.x * 64 + x;
+  const int states = r.M * r.N, x = threadIdx.x & 63, z = threadIdx.x >> 6, at = blockIdx.x * 64 + x, h = blockIdx.y % p.H, bi = blockIdx.y / p.H;
   const int64_t pair = blockIdx.y;
-  const int h = (int)(pair % p.H);
-  const int64_t bi = pair / p.H;
   const int n = p.lengths ? min(max(p.lengths[bi], 0), p.T) : p.T;
   const Decay decay(p.log_decay[h]);
   const bool live = at < states;
-  float* seg = r.seg + pair * p.segments * states + at;
-  const int K = (p.segments - 1 + 15) / 16, s_begin = min(z * K, p.segments - 1), s_end = min(s_begin + K, p.segments - 1);
+  float* const seg = r.seg + pair * p.segments * states + at;
+  const int joins = p.segments - 1, K = (joins + 15) / 16, s0 = min(z * K, joins), s1 = min(s0 + K, joins);   // this group's segments
   // the decay over segment s: whole, the one that holds the sequence's end, or behind it
   const int last = n / p.seg;
   const float over = decay.pow(p.seg), part = decay.pow(n - last * p.seg);
-  auto fade = [&](int s) { return s < last ? over : s == last ? part : 1.f; };
-  auto count = [&](int a, int b) { return min(max(n - a * p.seg, 0), (b - a) * p.seg); };   // of segments a .. b - 1 (all but the last are whole)
   float own[kMaxSegments / 16], run = 0.f;
 #pragma unroll
   for (int k = 0; k < kMaxSegments / 16; ++k)
-    if (s_begin + k < s_end && live) own[k] = seg[(int64_t)(s_begin + k + 1) * states];
+    if (k < K) own[k] = s0 + k < s1 && live ? seg[(int64_t)(s0 + k + 1) * states] : 0.f;
+  const float first = r.s0 && live ? r.s0[pair * states + at] : 0.f;
+  auto fade = [&](int s) { return s >= s1 ? 1.f : s < last ? over : s == last ? part : 1.f; };
 #pragma unroll
   for (int k = 0; k < kMaxSegments / 16; ++k)
-    if (s_begin + k < s_end && live) run = fmaf(fade(s_begin + k), run, own[k]);
+    if (k < K) run = fmaf(fade(s0 + k), run, own[k]);
   total[z][x] = run;
+  if (x == 0) fades[z] = decay.pow(min(max(n - s0 * p.seg, 0), (s1 - s0) * p.seg));   // (all but the last segment are whole)
   __syncthreads();
-  const float first = r.s0 && live ? r.s0[pair * states + at] : 0.f;
   run = first;
-  for (int y = 0; y < z; ++y) {
-    const int a = min(y * K, p.segments - 1), b = min(a + K, p.segments - 1);
-    run = fmaf(decay.pow(count(a, b)), run, total[y][x]);
-  }
+#pragma unroll
+  for (int y = 0; y < 15; ++y)
+    if (y < z) run = fmaf(fades[y], run, total[y][x]);
   if (!live) return;
   if (z == 0) seg[0] = first;
 #pragma unroll
   for (int k = 0; k < kMaxSegments / 16; ++k)
-    if (s_begin + k < s_end) {
-      run = fmaf(fade(s_begin + k), run, own[k]);
-      seg[(int64_t)(s_begin + k + 1) * states] = run;
+    if (k < K && s0 + k < s1) {
+      run = fmaf(fade(s0 + k), run, own[k]);
+      seg[(int64_t)(s0 + k + 1) * states] = run;
     }
 }
 
@@ -743,15 +784,16 @@ template <typename T, int MT, int CT, bool STAGED, bool STATE> int go(LaArgs a, 
   kernel<<<grid, threads, lds, st>>>(a);
   return tg_launch_status();
 }
-template <typename T, int MT, int CT, bool STATE> int go_staged(const LaArgs& a, bool staged, dim3 grid, int threads, hipStream_t st) {
-  return staged ? go<T, MT, CT, true, STATE>(a, grid, threads, st) : go<T, MT, CT, false, STATE>(a, grid, threads, st);
-}
 template <typename T, int MT> int go_mt(const LaArgs& a, bool staged, bool state, dim3 grid, int threads, hipStream_t st) {
-  // chunks of 32 tokens halve the work on the state per token; sequences of one chunk of 16 would waste half of them, and 128 fp32
-  // channels do not fit the registers twice
-  constexpr int CT = MT == 8 && sizeof(typename Mat<T>::Raw) == 16 ? 1 : 2;
-  if (state) return go_staged<T, MT, CT, true>(a, staged, grid, threads, st);
-  return a.T <= 16 ? go_staged<T, MT, 1, false>(a, staged, grid, threads, st) : go_staged<T, MT, CT, false>(a, staged, grid, threads, st);
+  // chunks of 32 tokens halve the work on the state per token; sequences of one chunk of 16 would waste half of them, and two tiles of 128
+  // fp32 channels, or of 128 channels that every lane loads itself, do not fit the registers
+  constexpr int CT = MT == 8 && sizeof(typename Mat<T>::Raw) == 16 ? 1 : 2, CU = MT == 8 ? 1 : 2;
+  if (staged) {
+    if (state) return go<T, MT, CT, true, true>(a, grid, threads, st);
+    return a.T <= 16 ? go<T, MT, 1, true, false>(a, grid, threads, st) : go<T, MT, CT, true, false>(a, grid, threads, st);
+  }
+  if (state) return go<T, MT, CU, false, true>(a, grid, threads, st);
+  return a.T <= 16 ? go<T, MT, 1, false, false>(a, grid, threads, st) : go<T, MT, CU, false, false>(a, grid, threads, st);
 }
 // `roles` roles with the same number of m tiles in one launch
 template <typename T> int launch(LaArgs a, int roles, bool state, hipStream_t st) {
@@ -786,7 +828,8 @@ Strided operand(int dtype, const void* p, const int64_t* stride, int shared) {
   auto aligned = [&](int n) {
     return (reinterpret_cast<uintptr_t>(p) & (n * elem_bytes(dtype) - 1)) == 0 && stride[0] % n == 0 && stride[1] % n == 0 && stride[2] % n == 0;
   };
-  return {Operand{p, stride[0], stride[2], (int)stride[1], shared}, aligned(4), aligned(16 / elem_bytes(dtype))};
+  // (a chunk's rows are reached by 32-bit offsets: 32 tokens of up to 2^25 bytes)
+  return {Operand{p, stride[0], stride[2], (int)stride[1], shared}, aligned(4), aligned(16 / elem_bytes(dtype)) && stride[1] * elem_bytes(dtype) <= (1 << 25)};
 }
 
 int check(int dtype, const tg_la_desc* d) {

@@ -324,8 +324,8 @@ def linear_attention(q, k, v, log_decay, scale=None, state=None, lengths=None):
 
 
 def linear_attention_backward(do, q, k, v, log_decay, scale=None, state=None, lengths=None, dstate=None):
-    """(dq, dk, dv, gradient of the first state) of linear_attention from the gradients of o and, if given, of the last state.  The gradients
-    of shared key / value heads are summed in 32 bits."""
+    """(dq, dk, dv, gradient of the first state) of linear_attention from the gradients of o and, if given, of the last state; the gradient of
+    the first state is None where `state` is.  The gradients of shared key / value heads are summed in 32 bits."""
     with torch.no_grad():
         dt, d, q, k, v, log_decay = _desc(q, k, v, log_decay, scale, False)
     shape = (d.B, d.H, d.DK, d.DV)
@@ -335,11 +335,11 @@ def linear_attention_backward(do, q, k, v, log_decay, scale=None, state=None, le
     dstate = None if dstate is None else _f32(q, dstate, "dstate", shape)
     lengths = _lengths(q, lengths)
     dq, dk, dv = (torch.empty(t.shape, dtype=q.dtype, device=q.device) for t in (q, k, v))
-    first = torch.empty(shape, dtype=torch.float32, device=q.device)
+    first = None if state is None else torch.empty(shape, dtype=torch.float32, device=q.device)
     n = L.load().tg_linear_attention_bwd_scratch_floats(C.byref(d))
     scratch = torch.empty(n, dtype=torch.float32, device=q.device) if n else None
     _call(q.device, "tg_linear_attention_bwd", dt, C.byref(d), q.data_ptr(), k.data_ptr(), v.data_ptr(), do.data_ptr(), _Strides(*do.stride()[:3]),
-          log_decay.data_ptr(), _ptr(lengths), _ptr(state), _ptr(dstate), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), first.data_ptr(), _ptr(scratch))
+          log_decay.data_ptr(), _ptr(lengths), _ptr(state), _ptr(dstate), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _ptr(first), _ptr(scratch))
     return dq, dk, dv, first
 
 
