@@ -18,8 +18,7 @@
 // Layout: a wave owns 16 columns of c (and of S and out) of one head and walks the tokens in chunks of 16 CT.  Everything is
 // made of 16 x 16 tiles in the matrix instructions' own shape: lane (c = lane % 16, g = lane / 16) holds 4 consecutive values 4g .. 4g+3
 // of row / column c.  An accumulator tile X[k][c] has the shape of an operand with c along its free dimension and k along the summed one,
-// so the scores (b a^T, tile [j][i]) and the state (tiles [m][n]) go from accumulators to operands without leaving the registers, and a
-// product with the identity turns a tile that was loaded by rows into one by columns (exactly).
+// so the scores (b a^T, tile [j][i]) and the state (tiles [m][n]) go from accumulators to operands without leaving the registers.
 //
 // Long sequences: T is cut into segments of `seg` tokens so that a few heads fill the machine.  la_kernel<STATE> sums each segment's own state,
 // la_scan_kernel joins them into the state in front of every segment, and the segments then run side by side.
@@ -83,6 +82,7 @@ template <> struct Mat<F32> {
     return c;
   }
   __device__ __forceinline__ static Raw one(int d) { return Raw{d == 0 ? 1.f : 0.f, d == 1 ? 1.f : 0.f, d == 2 ? 1.f : 0.f, d == 3 ? 1.f : 0.f}; }
+  __device__ __forceinline__ static f32x4 to_float(Raw v) { return v; }
   __device__ __forceinline__ static Op op(Raw v) { return v; }
   __device__ __forceinline__ static Op op_of(f32x4 v) { return v; }
   __device__ __forceinline__ static Split split(f32x4 v) { return v; }
@@ -108,6 +108,7 @@ template <> struct Mat<BF16> {
   typedef Thirds Split3;
   __device__ __forceinline__ static Raw one(int d) { return Raw{(short)(d == 0 ? 0x3f80 : 0), (short)(d == 1 ? 0x3f80 : 0), (short)(d == 2 ? 0x3f80 : 0), (short)(d == 3 ? 0x3f80 : 0)}; }
   __device__ __forceinline__ static s16x4 to_out(f32x4 v) { return to_bf16(v); }
+  __device__ __forceinline__ static f32x4 to_float(Raw v) { return from_bf16(v); }
   __device__ __forceinline__ static Op op(Raw v) { return v; }
   __device__ __forceinline__ static Op op_of(f32x4 v) { return to_bf16(v); }   // (of values that are bf16)
   __device__ __forceinline__ static Split split(f32x4 v) { return halves(v); }
@@ -135,7 +136,8 @@ template <> struct Mat<F16> {
   typedef Thirds Split3;
   __device__ __forceinline__ static Raw one(int d) { return Raw{(short)(d == 0 ? 0x3c00 : 0), (short)(d == 1 ? 0x3c00 : 0), (short)(d == 2 ? 0x3c00 : 0), (short)(d == 3 ? 0x3c00 : 0)}; }
   __device__ __forceinline__ static s16x4 to_out(f32x4 v) { return __builtin_bit_cast(s16x4, __builtin_convertvector(v, f16x4)); }
-  __device__ __forceinline__ static Op op(Raw v) { return halves(__builtin_convertvector(__builtin_bit_cast(f16x4, v), f32x4)); }
+  __device__ __forceinline__ static f32x4 to_float(Raw v) { return __builtin_convertvector(__builtin_bit_cast(f16x4, v), f32x4); }
+  __device__ __forceinline__ static Op op(Raw v) { return halves(to_float(v)); }
   __device__ __forceinline__ static Op op_of(f32x4 v) { return halves(v); }
   __device__ __forceinline__ static Split split(f32x4 v) { return halves(v); }
   __device__ __forceinline__ static Split3 split3(f32x4 v) { return thirds(v); }
@@ -396,6 +398,18 @@ template <typename T, int MT, int CT, bool STAGED, bool STATE> __global__ __laun
   };
   auto A = [&](int it, int t) { if constexpr (STAGED) return *reinterpret_cast<const Raw*>(area_a + (16 * it + c) * G::kRow + (16 * t + 4 * g) * kBytes); else return av[it][t]; };
   auto Bt = [&](int it, int t) { if constexpr (STAGED) return *reinterpret_cast<const Raw*>(area_b + (16 * it + c) * G::kRow + (16 * t + 4 * g) * kBytes); else return bv[it][t]; };
+  // by columns: tokens 16 jt + 4g .. + 3 of channel 16 t + c: a transposing read (16-bit), or one channel of four rows
+  auto columns = [&](const char* area, int row_bytes, int jt, int t) {
+    if constexpr (kBytes == 2) {
+      typedef __attribute__((address_space(3))) s16x4* Lds;
+      return __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(area + (16 * jt + 4 * g + (c >> 2)) * row_bytes + (16 * t + 4 * (c & 3)) * 2));
+    } else {
+      Raw v;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = *reinterpret_cast<const float*>(area + (16 * jt + 4 * g + e) * row_bytes + (16 * t + c) * 4);
+      return v;
+    }
+  };
   auto Ct = [&](int it) { if constexpr (STAGED) return *reinterpret_cast<const Raw*>(area_c + (16 * it + c) * G::kCRow + 4 * g * kBytes); else return cv[it]; };
 
   int n = length(bgroup), n_next = 0;
@@ -405,6 +419,7 @@ template <typename T, int MT, int CT, bool STAGED, bool STATE> __global__ __laun
   for (int bi = bgroup; bi < p.B; bi += p.bgroups, n = n_next) {
     n_next = length(bi + p.bgroups);
     const int64_t pair = (int64_t)bi * p.H + h;
+    float* const s1 = STATE ? r.seg + (pair * p.segments + segment + 1) * states : segment == p.segments - 1 && r.s1 ? r.s1 + pair * states : nullptr;
     const float* s0 = STATE ? nullptr : p.segments > 1 ? r.seg + (pair * p.segments + segment) * states : r.s0 ? r.s0 + pair * states : nullptr;
     f32x4 S[MT];
 #pragma unroll
@@ -434,10 +449,14 @@ template <typename T, int MT, int CT, bool STAGED, bool STATE> __global__ __laun
         if (cnt > 0) stage();
         next();
       }
+      const bool from_state = s0 || t0 > begin, to_state = s1 || t0 + C < min(n, end);   // (nothing is read from a state of zeros, or added to one that nobody reads)
       if (cnt > 0) {
         // c by columns: tokens 4g .. 4g+3 of column `col`
 #pragma unroll
-        for (int t = 0; t < CT; ++t) cf[t] = X::raw(Ct(t), unit, zero);
+        for (int t = 0; t < CT; ++t) {
+          if constexpr (STAGED) cf[t] = X::to_float(columns(area_c, G::kCRow, t, 0));
+          else cf[t] = X::raw(Ct(t), unit, zero);
+        }
         if constexpr (!STATE) {
           // scores x[jt][it][j][i] = b_j . a_i, and acc[it][n][i] = sum_m S[m][n] a_i[m]
 #pragma unroll
@@ -445,32 +464,41 @@ template <typename T, int MT, int CT, bool STAGED, bool STATE> __global__ __laun
 #pragma unroll
             for (int jt = 0; jt <= it; ++jt) x[jt][it] = zero;
           if constexpr (MT == 1) {
-            Raw a[CT], b[CT];
-            const typename X::Split s = X::split(S[0]);
+            Raw b[CT];
 #pragma unroll
             for (int it = 0; it < CT; ++it) {
-              a[it] = A(it, 0);
               b[it] = Bt(it, 0);
 #pragma unroll
-              for (int jt = 0; jt <= it; ++jt) x[jt][it] = X::raw(b[jt], a[it], zero);
-              acc[it] = X::state(s, X::op(a[it]), zero);
+              for (int jt = 0; jt <= it; ++jt) x[jt][it] = X::raw(b[jt], A(it, 0), zero);
             }
           } else {
 #pragma unroll
             for (int t = 0; t < MT; t += 2) {
-              Raw a0[CT], a1[CT], b0[CT], b1[CT];
-              const typename X::Split s = X::split(S[t]), u = X::split(S[t + 1]);
+              Raw b0[CT], b1[CT];
 #pragma unroll
               for (int it = 0; it < CT; ++it) {
-                a0[it] = A(it, t);
-                a1[it] = A(it, t + 1);
                 b0[it] = Bt(it, t);
                 b1[it] = Bt(it, t + 1);
 #pragma unroll
-                for (int jt = 0; jt <= it; ++jt) x[jt][it] = X::raw2(b0[jt], b1[jt], a0[it], a1[it], x[jt][it]);
-                acc[it] = X::state2(s, u, X::op(a0[it]), X::op(a1[it]), acc[it]);
+                for (int jt = 0; jt <= it; ++jt) x[jt][it] = X::raw2(b0[jt], b1[jt], A(it, t), A(it, t + 1), x[jt][it]);
               }
             }
+          }
+          if (from_state) {
+            if constexpr (MT == 1) {
+              const typename X::Split s = X::split(S[0]);
+#pragma unroll
+              for (int it = 0; it < CT; ++it) acc[it] = X::state(s, X::op(A(it, 0)), zero);
+            } else {
+#pragma unroll
+              for (int t = 0; t < MT; t += 2) {
+                const typename X::Split s = X::split(S[t]), u = X::split(S[t + 1]);
+#pragma unroll
+                for (int it = 0; it < CT; ++it) acc[it] = X::state2(s, u, X::op(A(it, t)), X::op(A(it, t + 1)), acc[it]);
+              }
+            }
+#pragma unroll
+            for (int t = 0; t < CT; ++t) acc[t] *= from[t];
           }
         }
         if constexpr (!STAGED) {
@@ -496,7 +524,6 @@ template <typename T, int MT, int CT, bool STAGED, bool STATE> __global__ __laun
           float top = 0.f;
 #pragma unroll
           for (int t = 0; t < CT; ++t) {
-            acc[t] *= from[t];
             co[t] = X::op_of(cf[t]);
 #pragma unroll
             for (int e = 0; e < 4; ++e) top = __builtin_elementwise_maximum(top, __builtin_fabsf(cf[t][e]));   // (a NaN stays)
@@ -522,7 +549,7 @@ template <typename T, int MT, int CT, bool STAGED, bool STATE> __global__ __laun
             for (int it = 0; it < CT; ++it) acc[it] = inner(it, co[it], acc[it]);
           }
         }
-        if (cnt < C && cnt != tail) {
+        if (to_state && cnt < C && cnt != tail) {
           tail = cnt;
           tail_keep = expm1f(decay.la * (float)cnt);
 #pragma unroll
@@ -538,22 +565,24 @@ template <typename T, int MT, int CT, bool STAGED, bool STATE> __global__ __laun
           }
         }
         // S[m][n] = g^n S[m][n] + sum_j b_j[m] (into_j c_j[n]); S + (g^n - 1) S keeps a slow decay's last bits
-        typename X::Split3 ws[CT];
+        if (to_state) {
+          typename X::Split3 ws[CT];
 #pragma unroll
-        for (int t = 0; t < CT; ++t) ws[t] = X::split3(cf[t] * (cnt < C ? tail_into[t] : whole_into[t]));
-        const float keep = cnt < C ? tail_keep : whole_keep;
+          for (int t = 0; t < CT; ++t) ws[t] = X::split3(cf[t] * (cnt < C ? tail_into[t] : whole_into[t]));
+          const float keep = cnt < C ? tail_keep : whole_keep;
 #pragma unroll
-        for (int t = 0; t < MT; ++t) {
-          Op b[CT];   // b by columns: tokens 4g .. 4g+3 of column 16 t + c
+          for (int t = 0; t < MT; ++t) {
+            Op b[CT];   // b by columns: tokens 4g .. 4g+3 of column 16 t + c
 #pragma unroll
-          for (int jt = 0; jt < CT; ++jt) {
-            if constexpr (STAGED) b[jt] = X::op_of(X::raw(Bt(jt, t), unit, zero));
-            else b[jt] = bt[t][jt];
+            for (int jt = 0; jt < CT; ++jt) {
+              if constexpr (STAGED) b[jt] = X::op(columns(area_b, G::kRow, jt, t));
+              else b[jt] = bt[t][jt];
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) S[t][e] = fmaf(S[t][e], keep, S[t][e]);
+            if constexpr (CT == 1) S[t] = X::add(b[0], ws[0], S[t]);
+            else S[t] = X::add2(b[0], b[1], ws[0], ws[1], S[t]);
           }
-#pragma unroll
-          for (int e = 0; e < 4; ++e) S[t][e] = fmaf(S[t][e], keep, S[t][e]);
-          if constexpr (CT == 1) S[t] = X::add(b[0], ws[0], S[t]);
-          else S[t] = X::add2(b[0], b[1], ws[0], ws[1], S[t]);
         }
       }
       if constexpr (!STATE) {
@@ -618,7 +647,6 @@ template <typename T, int MT, int CT, bool STAGED, bool STATE> __global__ __laun
         }
       }
     }
-    float* s1 = STATE ? r.seg + (pair * p.segments + segment + 1) * states : segment == p.segments - 1 && r.s1 ? r.s1 + pair * states : nullptr;
     if (s1 && has_col)
 #pragma unroll
       for (int t = 0; t < MT; ++t)
