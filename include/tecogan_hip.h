@@ -590,7 +590,7 @@ int tg_rms_norm_bwd(int dtype, const void* dy, int64_t dy_stride, const void* x,
 int tg_dropout(int dtype, const void* x, const void* res, void* y, int64_t n, double p, const int64_t* rng, int layer, void* stream);
 
 /* S_t = exp(log_decay[h]) S_{t-1} + k_t v_t^T, o_t = scale q_t S_t per sequence and head; q [B][T][H][DK], k [B][T][HK][DK], v [B][T][HK][DV]
- * at the given strides of (sequence, token, head), H % HK == 0: head h reads stored head h / (H / HK); 1 <= DK, DV <= 128.
+ * at the given strides of (sequence, token, head), H % HK == 0: head h reads stored head h / (H / HK); 1 <= DK, DV <= 128, H <= 65536.
  * Outputs o, dq [B][T][H][..], dk, dv [B][T][HK][..] are contiguous; states [B][H][DK][DV] fp32; lengths [B] int32 or null: tokens at and
  * behind lengths[b] (clamped to 0 .. T) are not read, their rows of the outputs are zero and the last state is the one at the length.
  * state_in null: zeros.  tg_linear_attention_bwd: dstate_out null: zeros; dstate_in may be null.  scratch: *_scratch_floats floats (0: may

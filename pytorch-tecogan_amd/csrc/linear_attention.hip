@@ -658,6 +658,248 @@ template <typename T, int MT, int CT, bool STAGED, bool STATE> __global__ __laun
   }
 }
 
+// Sequences of at most 16 tokens (a training clip's frames): the same arithmetic for ONE chunk, straight through.  A wave walks its sequences with
+// addresses that move on by a constant, the next one's rows on their way; what depends on the length is made again only where it changes.
+// (la_kernel's loops over segments and chunks cost more scalar instructions and branches here than the chunk itself: 39 us for the gradients
+// of 16384 sequences of 10 tokens x 16 channels, 23 us here.)
+template <typename T, int MT> __global__ __launch_bounds__(256, 2) void la_short_kernel(LaArgs p) {
+  typedef Mat<T> X;
+  typedef Stage<T, MT, 1> G;
+  typedef typename X::Raw Raw;
+  typedef typename X::Op Op;
+  constexpr int kBytes = ElemTraits<T>::kBytes;
+  constexpr f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+  extern __shared__ __align__(16) char lds[];
+  const Role& r = p.r[blockIdx.y];
+  const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+  const int slices = (r.N + 15) >> 4, per = waves / p.group;
+  const int bgroup = blockIdx.x / p.columns, f = (blockIdx.x - bgroup * p.columns) * per + wave / p.group, member = wave % p.group;
+  const bool active = f < p.H / p.group * slices;
+  const int slice = f % slices, h = active ? f / slices * p.group + member : 0;
+  const Decay decay(p.log_decay[h]);
+  const int step = p.bgroups, B = p.B, Tn = p.T, M = r.M, N = r.N, reverse = r.reverse, fold = r.fold;
+  const int col = slice * 16 + c;
+  const bool has_col = active && col < N;
+  char* const area_a = lds + wave * G::kArea;
+  char* const area_b = area_a + 16 * G::kRow;
+  char* const area_c = area_b + 16 * G::kRow;
+  f32x4* const sums = reinterpret_cast<f32x4*>(lds + waves * G::kArea);
+  const int64_t states = (int64_t)M * N, next_states = (int64_t)step * p.H * states;
+  const float* s0 = r.s0 ? r.s0 + ((int64_t)bgroup * p.H + h) * states : nullptr;
+  float* s1 = r.s1 ? r.s1 + ((int64_t)bgroup * p.H + h) * states : nullptr;
+  const int row_bytes = p.H / fold * N * (r.out_f32 ? 4 : kBytes), cols_bytes = r.out_f32 ? 4 : kBytes;
+  char* out = reinterpret_cast<char*>(r.out) + (int64_t)bgroup * Tn * row_bytes + (h / fold * N + slice * 16) * cols_bytes;
+  const int64_t next_out = (int64_t)step * Tn * row_bytes;
+  const char* qa = reinterpret_cast<const char*>(r.a.p) + (bgroup * r.a.sb + (h / r.a.shared) * r.a.sh) * kBytes;
+  const char* qb = reinterpret_cast<const char*>(r.b.p) + (bgroup * r.b.sb + (h / r.b.shared) * r.b.sh) * kBytes;
+  const char* qc = reinterpret_cast<const char*>(r.c.p) + (bgroup * r.c.sb + (h / r.c.shared) * r.c.sh + slice * 16) * kBytes;
+  const int64_t next_a = step * r.a.sb * kBytes, next_b = step * r.b.sb * kBytes, next_c = step * r.c.sb * kBytes;
+  const int ta = r.a.st * kBytes, tb = r.b.st * kBytes, tc = r.c.st * kBytes;
+
+  const int piece = lane % G::kLanes * 16, piece_c = lane % kBytes * 16, row_a = lane / G::kLanes, row_c = lane / kBytes;
+  const bool live_a = piece < M * kBytes && row_a < 16, live_c = slice * 16 * kBytes + piece_c < N * kBytes && row_c < 16;
+  // lengths, and what goes by them: the lanes' places in a sequence, the weights in the state, the rows of out
+  auto length = [&](int bi) { return p.lengths ? min(max(p.lengths[bi], 0), Tn) : Tn; };
+  unsigned oa[G::kLoads], ob[G::kLoads], oc;
+  auto places = [&](int n) {
+    auto token = [&](int row) {
+      const int idx = min(row, max(n, 1) - 1);
+      return reverse ? max(n, 1) - 1 - idx : idx;
+    };
+#pragma unroll
+    for (int i = 0; i < G::kLoads; ++i) {
+      const int tok = token(i * G::kRows + row_a);
+      oa[i] = (unsigned)(tok * ta + piece);
+      ob[i] = (unsigned)(tok * tb + piece);
+    }
+    oc = (unsigned)(token(row_c) * tc + piece_c);
+  };
+  u32x4 fa[G::kLoads], fb[G::kLoads], fc;
+  auto fetch = [&]() {
+#pragma unroll
+    for (int i = 0; i < G::kLoads; ++i) fa[i] = fb[i] = u32x4{0, 0, 0, 0};
+    fc = u32x4{0, 0, 0, 0};
+    if (live_a)
+#pragma unroll
+      for (int i = 0; i < G::kLoads; ++i) {
+        fa[i] = *reinterpret_cast<const u32x4*>(qa + oa[i]);
+        fb[i] = *reinterpret_cast<const u32x4*>(qb + ob[i]);
+      }
+    if (live_c) fc = *reinterpret_cast<const u32x4*>(qc + oc);
+  };
+  auto columns = [&](const char* area, int row, int t) {
+    if constexpr (kBytes == 2) {
+      typedef __attribute__((address_space(3))) s16x4* Lds;
+      return __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(area + (4 * g + (c >> 2)) * row + (16 * t + 4 * (c & 3)) * 2));
+    } else {
+      Raw v;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = *reinterpret_cast<const float*>(area + (4 * g + e) * row + (16 * t + c) * 4);
+      return v;
+    }
+  };
+  f32x4 inside, into;
+  float keep = 0.f;
+  const float g1 = decay.pow(1), from = r.za * decay.pow(c + 1 - r.sh);
+  {
+    const int d = c - 4 * g;
+    inside[3] = p.scale * decay.pow(max(d - 3, 0));
+#pragma unroll
+    for (int e = 2; e >= 0; --e) inside[e] = d - e > 0 ? inside[e + 1] * g1 : p.scale;
+  }
+  auto weights = [&](int n) {
+    keep = expm1f(decay.la * (float)n);
+    const int d = n - 1 - 4 * g;
+    const float w0 = r.zs * decay.pow(r.sh);
+    float w = r.zs * decay.pow(max(d - 3, 0) + r.sh);
+#pragma unroll
+    for (int e = 3; e >= 0; --e) {
+      if (e < 3) w = d - e > 0 ? w * g1 : w0;
+      into[e] = d - e >= 0 ? w : 0.f;
+    }
+  };
+
+  int n = active && bgroup < B ? length(bgroup) : 0, placed = n, weighted = -1, turn = 0;
+  places(n);
+  if (n > 0) fetch();
+  for (int bi = bgroup; bi < B; bi += step, ++turn) {
+    f32x4 S[MT];
+    if (s0) {
+#pragma unroll
+      for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int m = 16 * t + 4 * g + e;
+          const float v = s0[min(m, M - 1) * r.sm + min(col, N - 1) * r.sn];
+          S[t][e] = m < M && has_col ? v : 0.f;
+        }
+      s0 += next_states;
+    }
+    if (n > 0) {   // into the wave's LDS
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      if (row_a < 16)
+#pragma unroll
+        for (int i = 0; i < G::kLoads; ++i) {
+          *reinterpret_cast<u32x4*>(area_a + (i * G::kRows + row_a) * G::kRow + piece) = fa[i];
+          *reinterpret_cast<u32x4*>(area_b + (i * G::kRows + row_a) * G::kRow + piece) = fb[i];
+        }
+      if (row_c < 16) *reinterpret_cast<u32x4*>(area_c + row_c * G::kCRow + piece_c) = fc;
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+    }
+    int n_next = 0;
+    if (active && bi + step < B) {
+      qa += next_a;
+      qb += next_b;
+      qc += next_c;
+      n_next = length(bi + step);
+      if (n_next != placed) {
+        placed = n_next;
+        places(n_next);
+      }
+      if (n_next > 0) fetch();
+    }
+    f32x4 acc = zero;
+    if (n > 0) {
+      auto A = [&](int t) { return *reinterpret_cast<const Raw*>(area_a + c * G::kRow + (16 * t + 4 * g) * kBytes); };
+      auto Bm = [&](int t) { return *reinterpret_cast<const Raw*>(area_b + c * G::kRow + (16 * t + 4 * g) * kBytes); };
+      const Raw craw = columns(area_c, G::kCRow, 0);
+      f32x4 x = zero;
+      if constexpr (MT == 1) {
+        x = X::raw(Bm(0), A(0), x);
+      } else {
+#pragma unroll
+        for (int t = 0; t < MT; t += 2) x = X::raw2(Bm(t), Bm(t + 1), A(t), A(t + 1), x);
+      }
+      if (s0) {
+#pragma unroll
+        for (int t = 0; t < MT; t += MT == 1 ? 1 : 2) {
+          if constexpr (MT == 1) acc = X::state(X::split(S[0]), X::op(A(0)), acc);
+          else acc = X::state2(X::split(S[t]), X::split(S[t + 1]), X::op(A(t)), X::op(A(t + 1)), acc);
+        }
+        acc *= from;
+      }
+      const f32x4 cf = X::to_float(craw);
+      const Op co = X::op(craw);
+      float top = 0.f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        x[e] = 4 * g + e <= c ? x[e] * inside[e] : 0.f;
+        top = __builtin_elementwise_maximum(top, __builtin_fabsf(cf[e]));
+      }
+      const typename X::Split ps = X::split(x);
+      if (__builtin_expect(__any(!(top <= 3.4028234e38f)), 0)) {   // (see la_kernel)
+        const f32x4 before = acc;
+#pragma unroll 1
+        for (int i = 0; i < 16; ++i) {
+          const f32x4 y = X::score(X::upto(co, i + 1 - 4 * g), ps, before);
+          if (c == i) acc = y;
+        }
+      } else {
+        acc = X::score(co, ps, acc);
+      }
+      if (s1) {
+        if (n != weighted) {
+          weighted = n;
+          weights(n);
+        }
+        const typename X::Split3 ws = X::split3(cf * into);
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+          f32x4 v = zero;
+          if (s0)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = fmaf(S[t][e], keep, S[t][e]);
+          S[t] = X::add(X::op(columns(area_b, G::kRow, t)), ws, v);
+        }
+      }
+    } else if (!s0) {
+#pragma unroll
+      for (int t = 0; t < MT; ++t) S[t] = zero;
+    }
+    if (s1) {
+      if (has_col)
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int m = 16 * t + 4 * g + e;
+            if (m < M) s1[m * r.sm + col * r.sn] = S[t][e];
+          }
+      s1 += next_states;
+    }
+    bool writes = active;
+    if (fold > 1) {   // (see la_kernel)
+      f32x4* const buf = sums + (turn & 1) * waves * 64;
+      buf[wave * 64 + lane] = acc;
+      __syncthreads();
+      writes = active && member == 0;
+      if (writes)
+        for (int k = 1; k < fold; ++k) acc += buf[(wave + k) * 64 + lane];
+    }
+    if (writes) {
+      if (c >= n) acc = zero;
+      if (kBytes == 4 || cols_bytes == kBytes) {
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        char* const o = area_c + c * G::kCRow + 4 * g * kBytes;
+        if constexpr (kBytes == 4) *reinterpret_cast<f32x4*>(o) = acc;
+        else *reinterpret_cast<s16x4*>(o) = X::to_out(acc);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        const int tok = reverse && row_c < n ? n - 1 - row_c : row_c;
+        if (live_c && row_c < Tn) *reinterpret_cast<u32x4*>(out + (unsigned)(tok * row_bytes + piece_c)) = *reinterpret_cast<const u32x4*>(area_c + row_c * G::kCRow + piece_c);
+      } else if (c < Tn && slice * 16 + 4 * g < N) {
+        const int tok = reverse && c < n ? n - 1 - c : c;
+        *reinterpret_cast<f32x4*>(out + (unsigned)(tok * row_bytes + 16 * g)) = acc;
+      }
+    }
+    out += next_out;
+    n = n_next;
+  }
+}
+
 // the state in front of every segment, from each segment's own (written one place further on) and the first state: in place.  A workgroup
 // takes 64 elements of one state; 16 groups of threads take consecutive segments each and meet through LDS
 constexpr int kMaxSegments = 256;
@@ -791,18 +1033,16 @@ void segmentation(int T, int64_t waves, int* seg, int* segments) {
 }
 
 // One launch.  Sequences are dealt out so that the grid fills the machine ONCE (a wave makes its decay's powers once, and no second round of
-// workgroups finds the machine half empty: 4096 waves where 3072 fit ran 338 us, 3072 run XXX us)
-template <typename T, int MT, int CT, bool STAGED, bool STATE> int go(LaArgs a, dim3 grid, int threads, hipStream_t st) {
-  const int waves = threads / 64, folds = !STATE && a.group > 1;
-  const int lds = (folds ? 2 * waves * CT * 64 * 16 : 0) + (STAGED ? waves * Stage<T, MT, CT>::kArea : 0);
-  const auto kernel = la_kernel<T, MT, CT, STAGED, STATE>;
-  static std::atomic<int> resident[2][kFold + 1];   // workgroups of a CU, by folds and waves; 0: not known yet
-  int per_cu = resident[folds][waves].load(std::memory_order_relaxed);
+// workgroups finds the machine half empty: 4096 waves where 3072 fit ran 338 us, 3072 ran 274)
+struct Resident { std::atomic<int> n[2][kFold + 1]; };   // a kernel's workgroups on a CU, by folds and waves; 0: not known yet
+int go(void (*kernel)(LaArgs), Resident& resident, int area, int ct, bool folds, LaArgs a, dim3 grid, int threads, hipStream_t st) {
+  const int waves = threads / 64, lds = (folds ? 2 * waves * ct * 64 * 16 : 0) + waves * area;
+  int per_cu = resident.n[folds][waves].load(std::memory_order_relaxed);
   if (per_cu == 0) {
     TG_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
     TG_CHECK_HIP(hipOccupancyMaxActiveBlocksPerMultiprocessor(&per_cu, reinterpret_cast<const void*>(kernel), threads, (size_t)lds));
     if (per_cu < 1) return TG_E_UNSUPPORTED;
-    resident[folds][waves].store(per_cu, std::memory_order_relaxed);
+    resident.n[folds][waves].store(per_cu, std::memory_order_relaxed);
   }
   const int64_t columns = a.columns, others = columns * grid.y * grid.z, room = (int64_t)per_cu * kCUs;
   const int64_t each = (a.B * others + room - 1) / room;             // sequences of a workgroup
@@ -812,16 +1052,24 @@ template <typename T, int MT, int CT, bool STAGED, bool STATE> int go(LaArgs a, 
   kernel<<<grid, threads, lds, st>>>(a);
   return tg_launch_status();
 }
+template <typename T, int MT, int CT, bool STAGED, bool STATE> int go_long(const LaArgs& a, dim3 grid, int threads, hipStream_t st) {
+  static Resident resident;
+  return go(la_kernel<T, MT, CT, STAGED, STATE>, resident, STAGED ? Stage<T, MT, CT>::kArea : 0, CT, !STATE && a.group > 1, a, grid, threads, st);
+}
+template <typename T, int MT> int go_short(const LaArgs& a, dim3 grid, int threads, hipStream_t st) {
+  static Resident resident;
+  return go(la_short_kernel<T, MT>, resident, Stage<T, MT, 1>::kArea, 1, a.group > 1, a, grid, threads, st);
+}
 template <typename T, int MT> int go_mt(const LaArgs& a, bool staged, bool state, dim3 grid, int threads, hipStream_t st) {
   // chunks of 32 tokens halve the work on the state per token; sequences of one chunk of 16 would waste half of them, and two tiles of 128
   // fp32 channels, or of 128 channels that every lane loads itself, do not fit the registers
   constexpr int CT = MT == 8 && sizeof(typename Mat<T>::Raw) == 16 ? 1 : 2, CU = MT == 8 ? 1 : 2;
   if (staged) {
-    if (state) return go<T, MT, CT, true, true>(a, grid, threads, st);
-    return a.T <= 16 ? go<T, MT, 1, true, false>(a, grid, threads, st) : go<T, MT, CT, true, false>(a, grid, threads, st);
+    if (state) return go_long<T, MT, CT, true, true>(a, grid, threads, st);
+    return a.T <= 16 ? go_short<T, MT>(a, grid, threads, st) : go_long<T, MT, CT, true, false>(a, grid, threads, st);
   }
-  if (state) return go<T, MT, CU, false, true>(a, grid, threads, st);
-  return a.T <= 16 ? go<T, MT, 1, false, false>(a, grid, threads, st) : go<T, MT, CU, false, false>(a, grid, threads, st);
+  if (state) return go_long<T, MT, CU, false, true>(a, grid, threads, st);
+  return a.T <= 16 ? go_long<T, MT, 1, false, false>(a, grid, threads, st) : go_long<T, MT, CU, false, false>(a, grid, threads, st);
 }
 // `roles` roles with the same number of m tiles in one launch
 template <typename T> int launch(LaArgs a, int roles, bool state, hipStream_t st) {
@@ -862,7 +1110,7 @@ Strided operand(int dtype, const void* p, const int64_t* stride, int shared) {
 
 int check(int dtype, const tg_la_desc* d) {
   if (!d || !known(dtype) || d->B < 0 || d->T < 0 || d->H <= 0 || d->HK <= 0 || d->DK <= 0 || d->DV <= 0) return TG_E_BADARG;
-  if (d->H % d->HK || d->DK > kMaxHead || d->DV > kMaxHead || d->T > 0x7fffff00) return TG_E_UNSUPPORTED;
+  if (d->H % d->HK || d->DK > kMaxHead || d->DV > kMaxHead || d->T > 0x7fffff00 || d->H > 65536) return TG_E_UNSUPPORTED;
   for (const int64_t* s : {d->q_stride, d->k_stride, d->v_stride})
     if (s[0] < 0 || s[1] < 0 || s[2] < 0) return TG_E_BADARG;
     else if (s[1] > 0x7fffffff) return TG_E_UNSUPPORTED;
