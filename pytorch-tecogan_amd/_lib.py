@@ -42,7 +42,7 @@ class WgradDesc(C.Structure):
                 ("taps_per_wg", C.c_int32), ("y_sum", C.c_int32)]
 
 
-class LaDesc(C.Structure):
+class LaDesc(C.Structure):   # tg_la_desc (sequence.py packs it as bytes: a third of a Structure's host time)
     _fields_ = [("B", C.c_int32), ("T", C.c_int32), ("H", C.c_int32), ("HK", C.c_int32), ("DK", C.c_int32), ("DV", C.c_int32),
                 ("q_stride", C.c_int64 * 3), ("k_stride", C.c_int64 * 3), ("v_stride", C.c_int64 * 3), ("scale", C.c_float)]
 
@@ -124,11 +124,11 @@ _PROTOS = {
     "tg_rms_norm_bwd_scratch_floats": (_L, [_L, _I]),
     "tg_rms_norm_bwd": (_I, [_I, _P, _L, _P, _L, _P, _L, _P, _P, _P, _L, _P, _P, _P, _L, _I, _P]),
     "tg_dropout": (_I, [_I, _P, _P, _P, _L, _D, _P, _I, _P]),
-    "tg_linear_attention_scratch_floats": (_L, [C.POINTER(LaDesc)]),
-    "tg_linear_attention": (_I, [_I, C.POINTER(LaDesc), _P, _P, _P, _P, _P, _P, _P, _P, _P, _P]),
-    "tg_linear_attention_bwd_scratch_floats": (_L, [C.POINTER(LaDesc)]),
-    "tg_linear_attention_bwd": (_I, [_I, C.POINTER(LaDesc), _P, _P, _P, _P, C.POINTER(C.c_int64), _P, _P, _P, _P, _P, _P, _P, _P, _P, _P]),
-    "tg_linear_attention_step": (_I, [_I, C.POINTER(LaDesc), _P, _P, _P, _P, _P, _P, _P]),
+    "tg_linear_attention_scratch_floats": (_L, [_P]),
+    "tg_linear_attention": (_I, [_I, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P]),
+    "tg_linear_attention_bwd_scratch_floats": (_L, [_P]),
+    "tg_linear_attention_bwd": (_I, [_I, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P]),
+    "tg_linear_attention_step": (_I, [_I, _P, _P, _P, _P, _P, _P, _P, _P]),
     "tg_stream_create_cumask": (_I, [_I, C.POINTER(C.c_void_p)]),
     "tg_stream_destroy": (_I, [_P]),
 }

@@ -7,7 +7,7 @@ allocates its outputs and workspaces like any torch operation; nothing synchroni
 carries one (first order).  The explicit forms - `stats=True` and the `*_backward` functions - are what a captured step uses: autograd
 itself is not captured (a backward pass recorded while an eager graph of the same leaves lives ends the process), so inside a capture a
 call that would build an autograd graph raises; use torch.no_grad() there, or the explicit forms on detached tensors."""
-import ctypes as C
+import struct
 
 import torch
 
@@ -24,22 +24,43 @@ def _fail(text):
     raise L.TecoganHipError(text)
 
 
+# Host time counts where a call is a few microseconds of GPU time: the device and the stream are asked for as plain integers (a Stream
+# object is 3 us), entry points are looked up once
+_device, _stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+_entry = {}
+
+
 def _call(dev, name, *args):
     """one entry point of the library on the current stream of `dev`"""
-    fn = getattr(L.load(), name)
-    if dev.index == torch.cuda.current_device():
-        rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+    fn = _entry.get(name)
+    if fn is None:
+        fn = _entry[name] = getattr(L.load(), name)
+    index = dev.index
+    if index == _device():
+        rc = fn(*args, _stream(index))
     else:
         with torch.cuda.device(dev):
-            rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+            rc = fn(*args, _stream(index))
     if rc:
         L.check(rc, name)
+
+
+_DTYPES = {torch.bfloat16: L.TG_BF16, torch.float16: L.TG_F16, torch.float32: L.TG_F32}
+
+
+def _floats_of(name, *args):
+    """a workspace's size"""
+    fn = _entry.get(name)
+    if fn is None:
+        fn = _entry[name] = getattr(L.load(), name)
+    return fn(*args)
 
 
 def _floats(x, what):
     if not isinstance(x, torch.Tensor) or not x.is_cuda:
         _fail(f"{what} must be a device tensor (no CPU fallback)")
-    return tg_dtype(x.dtype)   # raises for other element types
+    dt = _DTYPES.get(x.dtype)
+    return tg_dtype(x.dtype) if dt is None else dt   # (raises for other element types)
 
 
 def _like(x, t, what, shape=None):
@@ -50,9 +71,9 @@ def _like(x, t, what, shape=None):
 
 
 def _f32(x, t, what, shape):
-    if not isinstance(t, torch.Tensor) or t.device != x.device or t.dtype != torch.float32 or tuple(t.shape) != tuple(shape):
+    if not isinstance(t, torch.Tensor) or t.device != x.device or t.dtype != torch.float32 or t.shape != shape:
         _fail(f"{what} must be a float32 tensor of shape {tuple(shape)} on {x.device}")
-    return t.contiguous()
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def _grad(*tensors):
@@ -78,6 +99,10 @@ def _rows(x, channels):
     return x.contiguous(), channels
 
 
+def _rowmajor(x):
+    return torch.empty_like(x, memory_format=torch.contiguous_format)
+
+
 def _norm_args(x, weight, residual, eps):
     dt = _floats(x, "x")
     if x.dim() < 1 or x.shape[-1] < 1:
@@ -100,8 +125,8 @@ def _norm_fwd(x, weight, residual, eps, stats):
     dt, channels, weight = _norm_args(x, weight, residual, eps)
     xr, xs = _rows(x, channels)
     rr, rs = (None, 0) if residual is None else _rows(residual, channels)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    s = None if residual is None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = _rowmajor(x)
+    s = None if residual is None else _rowmajor(x)
     rstd = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device) if stats else None
     _call(x.device, "tg_rms_norm", dt, xr.data_ptr(), xs, _ptr(rr), rs, _ptr(weight), y.data_ptr(), _ptr(s), _ptr(rstd),
           x.numel() // channels, channels, eps)
@@ -155,11 +180,11 @@ def rms_norm_backward(dy, x, rstd, weight=None, residual=None, ds=None, dweight=
     xr, xs = _rows(x, channels)
     rr, rs = (None, 0) if residual is None else _rows(residual, channels)
     er, es = (None, 0) if ds is None else _rows(ds, channels)
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    dx = _rowmajor(x)
     dw = scratch = None
     if dweight:
         dw = torch.empty(channels, dtype=torch.float32, device=x.device)
-        scratch = torch.empty(L.load().tg_rms_norm_bwd_scratch_floats(rows, channels), dtype=torch.float32, device=x.device)
+        scratch = torch.empty(_floats_of("tg_rms_norm_bwd_scratch_floats", rows, channels), dtype=torch.float32, device=x.device)
     _call(x.device, "tg_rms_norm_bwd", dt, gr.data_ptr(), gs, xr.data_ptr(), xs, _ptr(rr), rs, rstd.data_ptr(), _ptr(weight), _ptr(er), es,
           dx.data_ptr(), _ptr(dw), _ptr(scratch), rows, channels)
     return dx, dw
@@ -175,7 +200,7 @@ def rms_norm_e4m3(x, weight=None, residual=None, eps=1e-6):
     rr, rs = (None, 0) if residual is None else _rows(residual, channels)
     q = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
     scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
-    s = None if residual is None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    s = None if residual is None else _rowmajor(x)
     _call(x.device, "tg_rms_norm_e4m3", dt, xr.data_ptr(), xs, _ptr(rr), rs, _ptr(weight), q.data_ptr(), scale.data_ptr(), _ptr(s),
           x.numel() // channels, channels, eps)
     return (q, scale) if s is None else (q, scale, s)
@@ -200,7 +225,7 @@ def _drop(x, p, rng, layer, residual):
         _like(x, residual, "residual")
         residual = residual.contiguous()
     x, rng = x.contiguous(), rng.contiguous()
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = torch.empty_like(x)
     _call(x.device, "tg_dropout", dt, x.data_ptr(), _ptr(residual), y.data_ptr(), x.numel(), p, rng.data_ptr(), layer)
     return y
 
@@ -233,7 +258,8 @@ def dropout_backward(dy, p, rng, layer=0):
 
 
 # ---------------------------------------------------------------------------------------------------- linear attention
-_Strides = C.c_int64 * 3
+_DESC = struct.Struct("6i9qf4x")   # tg_la_desc
+_STRIDES = struct.Struct("3q")
 
 
 def _channels_last(t):
@@ -241,31 +267,34 @@ def _channels_last(t):
     return t if (t.stride(-1) == 1 or t.shape[-1] == 1) and t.stride(1) < 1 << 31 else t.contiguous()
 
 
-def _desc(q, k, v, log_decay, scale, step):
-    """(dtype, descriptor, tensors) after the checks that the sequence and the single-token form share"""
+def _desc(q, k, v, log_decay, scale, step, recorded=True):
+    """(dtype, descriptor, (B, T, H, Dk, Dv), tensors) after the checks that the sequence and the single-token form share"""
     dt = _floats(q, "q")
     dims = 3 if step else 4
     for t, what in ((k, "k"), (v, "v")):
         if not isinstance(t, torch.Tensor) or t.device != q.device or t.dtype != q.dtype or t.dim() != dims:
             _fail(f"{what} must be a {q.dtype} tensor of {dims} dimensions on {q.device}")
-    form = "(B, heads, channels)" if step else "(B, T, heads, channels)"
-    if q.dim() != dims or k.shape[:-2] != q.shape[:-2] or v.shape[:-1] != k.shape[:-1] or k.shape[-1] != q.shape[-1]:
+    sq, sk, sv = q.shape, k.shape, v.shape
+    if len(sq) != dims or sk[:-2] != sq[:-2] or sv[:-1] != sk[:-1] or sk[-1] != sq[-1]:
+        form = "(B, heads, channels)" if step else "(B, T, heads, channels)"
         _fail(f"q, k, v must be {form} with q and k of the same channels, k and v of the same heads")
-    B, H, HK, DK, DV = q.shape[0], q.shape[-2], k.shape[-2], q.shape[-1], v.shape[-1]
+    B, H, HK, DK, DV = sq[0], sq[-2], sk[-2], sq[-1], sv[-1]
+    T = 1 if step else sq[1]
     if H < 1 or HK < 1 or H % HK:
         _fail(f"{H} query heads do not divide over {HK} key / value heads")
     if not (1 <= DK <= MAX_HEAD and 1 <= DV <= MAX_HEAD):
         _fail(f"head sizes must be 1 .. {MAX_HEAD}: got {DK} and {DV}")
-    if log_decay.requires_grad and torch.is_grad_enabled():
-        _fail("log_decay is a constant of the heads: it has no gradient")
     log_decay = _f32(q, log_decay, "log_decay", (H,))
-    q, k, v = (_channels_last(t) for t in (q, k, v))
-    strides = [t.stride() for t in (q, k, v)]
+    if recorded and log_decay.requires_grad and torch.is_grad_enabled():
+        _fail("log_decay is a constant of the heads: it has no gradient")
+    q, k, v = _channels_last(q), _channels_last(k), _channels_last(v)
+    scale = DK ** -0.5 if scale is None else float(scale)
+    tq, tk, tv = q.stride(), k.stride(), v.stride()
     if step:
-        strides = [(s[0], 0, s[1]) for s in strides]
-    d = L.LaDesc(B, 1 if step else q.shape[1], H, HK, DK, DV, strides[0][:3], strides[1][:3], strides[2][:3],
-                 DK ** -0.5 if scale is None else float(scale))
-    return dt, d, q, k, v, log_decay
+        d = _DESC.pack(B, T, H, HK, DK, DV, tq[0], 0, tq[1], tk[0], 0, tk[1], tv[0], 0, tv[1], scale)
+    else:
+        d = _DESC.pack(B, T, H, HK, DK, DV, *tq[:3], *tk[:3], *tv[:3], scale)
+    return dt, d, (B, T, H, DK, DV), q, k, v, log_decay
 
 
 def _lengths(q, lengths):
@@ -277,16 +306,16 @@ def _lengths(q, lengths):
 
 
 def _attention_fwd(q, k, v, log_decay, scale, state, lengths):
-    dt, d, q, k, v, log_decay = _desc(q, k, v, log_decay, scale, False)
-    shape = (d.B, d.H, d.DK, d.DV)
-    state = None if state is None else _f32(q, state, "state", shape)
+    dt, d, (B, T, H, DK, DV), q, k, v, log_decay = _desc(q, k, v, log_decay, scale, False)
+    dev = q.device
+    state = None if state is None else _f32(q, state, "state", (B, H, DK, DV))
     lengths = _lengths(q, lengths)
-    o = torch.empty((d.B, d.T, d.H, d.DV), dtype=q.dtype, device=q.device)
-    last = torch.empty(shape, dtype=torch.float32, device=q.device)
-    n = L.load().tg_linear_attention_scratch_floats(C.byref(d))
-    scratch = torch.empty(n, dtype=torch.float32, device=q.device) if n else None
-    _call(q.device, "tg_linear_attention", dt, C.byref(d), q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), _ptr(lengths),
-          _ptr(state), o.data_ptr(), last.data_ptr(), _ptr(scratch))
+    o = torch.empty((B, T, H, DV), dtype=q.dtype, device=dev)
+    last = torch.empty((B, H, DK, DV), dtype=torch.float32, device=dev)
+    n = _floats_of("tg_linear_attention_scratch_floats", d)
+    scratch = torch.empty(n, dtype=torch.float32, device=dev) if n else None
+    _call(dev, "tg_linear_attention", dt, d, q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), _ptr(lengths), _ptr(state), o.data_ptr(),
+          last.data_ptr(), _ptr(scratch))
     return o, last
 
 
@@ -326,19 +355,17 @@ def linear_attention(q, k, v, log_decay, scale=None, state=None, lengths=None):
 def linear_attention_backward(do, q, k, v, log_decay, scale=None, state=None, lengths=None, dstate=None):
     """(dq, dk, dv, gradient of the first state) of linear_attention from the gradients of o and, if given, of the last state; the gradient of
     the first state is None where `state` is.  The gradients of shared key / value heads are summed in 32 bits."""
-    with torch.no_grad():
-        dt, d, q, k, v, log_decay = _desc(q, k, v, log_decay, scale, False)
-    shape = (d.B, d.H, d.DK, d.DV)
-    _like(q, do, "do", torch.Size((d.B, d.T, d.H, d.DV)))
-    do = _channels_last(do)
+    dt, d, (B, T, H, DK, DV), q, k, v, log_decay = _desc(q, k, v, log_decay, scale, False, recorded=False)
+    dev, shape = q.device, (B, H, DK, DV)
+    do = _channels_last(_like(q, do, "do", (B, T, H, DV)))
     state = None if state is None else _f32(q, state, "state", shape)
     dstate = None if dstate is None else _f32(q, dstate, "dstate", shape)
     lengths = _lengths(q, lengths)
-    dq, dk, dv = (torch.empty(t.shape, dtype=q.dtype, device=q.device) for t in (q, k, v))
-    first = None if state is None else torch.empty(shape, dtype=torch.float32, device=q.device)
-    n = L.load().tg_linear_attention_bwd_scratch_floats(C.byref(d))
-    scratch = torch.empty(n, dtype=torch.float32, device=q.device) if n else None
-    _call(q.device, "tg_linear_attention_bwd", dt, C.byref(d), q.data_ptr(), k.data_ptr(), v.data_ptr(), do.data_ptr(), _Strides(*do.stride()[:3]),
+    dq, dk, dv = _rowmajor(q), _rowmajor(k), _rowmajor(v)
+    first = None if state is None else torch.empty(shape, dtype=torch.float32, device=dev)
+    n = _floats_of("tg_linear_attention_bwd_scratch_floats", d)
+    scratch = torch.empty(n, dtype=torch.float32, device=dev) if n else None
+    _call(dev, "tg_linear_attention_bwd", dt, d, q.data_ptr(), k.data_ptr(), v.data_ptr(), do.data_ptr(), _STRIDES.pack(*do.stride()[:3]),
           log_decay.data_ptr(), _ptr(lengths), _ptr(state), _ptr(dstate), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _ptr(first), _ptr(scratch))
     return dq, dk, dv, first
 
@@ -349,10 +376,10 @@ def linear_attention_step(q, k, v, log_decay, state, scale=None):
     gradient."""
     if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, state)):
         _fail("linear_attention_step has no gradient: call it under torch.no_grad(), or linear_attention with one token")
-    dt, d, q, k, v, log_decay = _desc(q, k, v, log_decay, scale, True)
-    _f32(q, state, "state", (d.B, d.H, d.DK, d.DV))
+    dt, d, (B, _, H, DK, DV), q, k, v, log_decay = _desc(q, k, v, log_decay, scale, True)
+    _f32(q, state, "state", (B, H, DK, DV))
     if not state.is_contiguous():
         _fail("state is updated in place: it must be contiguous")
-    o = torch.empty((d.B, d.H, d.DV), dtype=q.dtype, device=q.device)
-    _call(q.device, "tg_linear_attention_step", dt, C.byref(d), q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), o.data_ptr(), state.data_ptr())
+    o = torch.empty((B, H, DV), dtype=q.dtype, device=q.device)
+    _call(q.device, "tg_linear_attention_step", dt, d, q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), o.data_ptr(), state.data_ptr())
     return o
