@@ -556,7 +556,8 @@ def test_attention_gradient_against_differences():
 
 @pytest.mark.parametrize("dt", [F32, BF16, F16])
 @pytest.mark.parametrize("B,H,HK,DK,DV", [(1, 1, 1, 1, 1), (2, 4, 2, 16, 16), (5, 3, 1, 17, 31), (3, 4, 4, 64, 64), (2, 2, 2, 128, 128), (1, 2, 1, 7, 100),
-                                          (3, 2, 2, 33, 127), (70, 4, 4, 16, 16), (1, 2, 2, 128, 4)])
+                                          (3, 2, 2, 33, 127), (70, 4, 4, 16, 16), (1, 2, 2, 128, 4), (1100, 4, 2, 16, 16), (1367, 3, 3, 15, 12),
+                                          (600, 2, 1, 32, 64), (600, 2, 2, 5, 128), (9000, 2, 2, 8, 4)])
 def test_attention_step(B, H, HK, DK, DV, dt):
     q, k, v, state = randn(B, H, DK, dt=dt, seed=1), randn(B, HK, DK, dt=dt, seed=2), randn(B, HK, DV, dt=dt, seed=3), randn(B, H, DK, DV, seed=4)
     decay = -torch.rand(H, generator=torch.Generator().manual_seed(5)).to(DEV)
