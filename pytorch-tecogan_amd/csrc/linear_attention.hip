@@ -20,7 +20,7 @@
 // of row / column c.  An accumulator tile X[k][c] has the shape of an operand with c along its free dimension and k along the summed one,
 // so the scores (b a^T, tile [j][i]) and the state (tiles [m][n]) go from accumulators to operands without leaving the registers.
 //
-// Long sequences: T is cut into segments of `seg` tokens so that a few heads fill the machine.  la_kernel<STATE> sums each segment's own state,
+// Long sequences: T is cut into segments of `seg` tokens so that a few heads fill the machine.  la_kernel with STATE sums each segment's own state,
 // la_scan_kernel joins them into the state in front of every segment, and the segments then run side by side.
 //
 // Rounding: raw inputs are multiplied as they are (exact products, fp32 sums).  Scores and state are fp32; as operands beside 16-bit
@@ -95,6 +95,10 @@ template <> struct Mat<F32> {
   __device__ __forceinline__ static f32x4 score2(Op v0, Op v1, Split p0, Split p1, f32x4 c) { return mma(v1, p1, mma(v0, p0, c)); }
   __device__ __forceinline__ static f32x4 add(Op b, Split3 w, f32x4 c) { return mma(b, w, c); }
   __device__ __forceinline__ static f32x4 add2(Op b0, Op b1, Split3 w0, Split3 w1, f32x4 c) { return mma(b1, w1, mma(b0, w0, c)); }
+  template <int CT> __device__ __forceinline__ static f32x4 grown(f32x4 s, const Op* b, const Split3* w) {
+    if constexpr (CT == 1) return add(b[0], w[0], s);
+    else return add2(b[0], b[1], w[0], w[1], s);
+  }
   __device__ __forceinline__ static Op upto(Op v, int n) {   // the first n of the 4 values, zeros behind
 #pragma unroll
     for (int e = 0; e < 4; ++e) v[e] = e < n ? v[e] : 0.f;
@@ -122,6 +126,10 @@ template <> struct Mat<BF16> {
   __device__ __forceinline__ static f32x4 add(Op b, Split3 w, f32x4 c) { return mma_bf16(b, w.hi, mma_bf16(b, w.mid, mma_bf16(b, w.lo, c))); }
   __device__ __forceinline__ static f32x4 add2(Op b0, Op b1, Split3 w0, Split3 w1, f32x4 c) {
     return mma2_bf16(b0, b1, w0.hi, w1.hi, mma2_bf16(b0, b1, w0.mid, w1.mid, mma2_bf16(b0, b1, w0.lo, w1.lo, c)));
+  }
+  template <int CT> __device__ __forceinline__ static f32x4 grown(f32x4 s, const Op* b, const Split3* w) {
+    if constexpr (CT == 1) return add(b[0], w[0], s);
+    else return add2(b[0], b[1], w[0], w[1], s);
   }
   __device__ __forceinline__ static Op upto(Op v, int n) {
 #pragma unroll
@@ -164,6 +172,10 @@ template <> struct Mat<F16> {
     c = mma2_bf16(b0.hi, b1.hi, w0.mid, w1.mid, c);
     return mma2_bf16(b0.hi, b1.hi, w0.hi, w1.hi, c);
   }
+  template <int CT> __device__ __forceinline__ static f32x4 grown(f32x4 s, const Op* b, const Split3* w) {
+    if constexpr (CT == 1) return add(b[0], w[0], s);
+    else return add2(b[0], b[1], w[0], w[1], s);
+  }
   __device__ __forceinline__ static Op upto(Op v, int n) {
     v.hi = Mat<BF16>::upto(v.hi, n);
     v.lo = Mat<BF16>::upto(v.lo, n);
@@ -192,7 +204,7 @@ struct Operand {
   int shared;            // heads per stored head
 };
 
-// what one pass over the tokens computes (see the top): an output, or a gradient, or (la_kernel<STATE>) segments' states alone
+// what one pass over the tokens computes (see the top): an output, or a gradient, or (STATE) segments' states alone
 struct Role {
   Operand a, b, c;
   void* out;             // [B][T][H / fold][N]
@@ -232,11 +244,313 @@ struct Decay {
   }
 };
 
-// How a chunk's rows reach a wave.  STAGED (16-byte aligned operands whose channels fill 16-byte pieces): a wave reads whole rows, 16 bytes per
+__device__ __forceinline__ void wave_fence() {   // the wave's own LDS writes and reads keep their order
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+// What a wave works on: 16 columns (a slice) of one head, and the sequences bgroup, bgroup + bgroups, .. of it.  A wave without work does another's
+// and writes nothing (it meets the barriers of the summed roles).
+template <typename T, int MT> struct Wave {
+  int lane, c, g, wave, waves, member, bgroup, slice, h;
+  bool active;
+  Decay decay;
+  __device__ __forceinline__ explicit Wave(const LaArgs& p) : decay(0.f) {
+    const Role& r = p.r[blockIdx.y];
+    lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+    const int slices = (r.N + 15) >> 4, per = waves / p.group;       // (stored head, slice) pairs of a workgroup
+    bgroup = blockIdx.x / p.columns;
+    int f = (blockIdx.x - bgroup * p.columns) * per + wave / p.group;
+    member = wave % p.group;
+    active = f < p.H / p.group * slices;
+    if (!active) f = 0;
+    slice = f % slices;
+    h = f / slices * p.group + member;
+    decay = Decay(p.log_decay[h]);
+  }
+  __device__ __forceinline__ bool whole(const Role& r) const { return r.M == 16 * MT && (r.N & 15) == 0; }   // no part tiles
+  __device__ __forceinline__ bool has_col(const Role& r) const { return slice * 16 + c < r.N; }
+  // the state in front of the first token; false: there is none (zeros)
+  template <bool STATE> __device__ __forceinline__ bool first(const LaArgs& p, const Role& r, int bi, f32x4* S) const {
+    const int64_t pair = (int64_t)bi * p.H + h, states = (int64_t)r.M * r.N;
+    const float* s0 = STATE ? nullptr : p.segments > 1 ? r.seg + (pair * p.segments + blockIdx.z) * states : r.s0 ? r.s0 + pair * states : nullptr;
+#pragma unroll
+    for (int t = 0; t < MT; ++t) S[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (!s0) return false;
+    const int at = 4 * g * r.sm + (slice * 16 + c) * r.sn;
+    if (whole(r)) {
+#pragma unroll
+      for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) S[t][e] = s0[at + (16 * t + e) * r.sm];
+    } else if (has_col(r)) {
+#pragma unroll
+      for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (16 * t + 4 * g + e < r.M) S[t][e] = s0[at + (16 * t + e) * r.sm];
+    }
+    return true;
+  }
+  template <bool STATE> __device__ __forceinline__ void last(const LaArgs& p, const Role& r, int bi, const f32x4* S) const {
+    const int64_t pair = (int64_t)bi * p.H + h, states = (int64_t)r.M * r.N;
+    float* s1 = STATE ? r.seg + (pair * p.segments + blockIdx.z + 1) * states : (int)blockIdx.z == p.segments - 1 && r.s1 ? r.s1 + pair * states : nullptr;
+    if (!s1 || !active || !has_col(r)) return;
+    const int at = 4 * g * r.sm + (slice * 16 + c) * r.sn;
+    if (whole(r)) {
+#pragma unroll
+      for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s1[at + (16 * t + e) * r.sm] = S[t][e];
+    } else {
+#pragma unroll
+      for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (16 * t + 4 * g + e < r.M) s1[at + (16 * t + e) * r.sm] = S[t][e];
+    }
+  }
+  // the heads of one stored head add up, in order, in the first one's wave; whether this wave writes.  (Uniform over the launch's role.  Two
+  // buffers: who writes one again has passed the next barrier, and so have its readers.)
+  template <int CT> __device__ __forceinline__ bool fold(f32x4* acc, f32x4* sums, int heads, int turn) const {
+    if (heads == 1) return active;
+    f32x4* const buf = sums + (turn & 1) * waves * CT * 64;
+#pragma unroll
+    for (int t = 0; t < CT; ++t) buf[(wave * CT + t) * 64 + lane] = acc[t];
+    __syncthreads();
+    if (!writer(heads)) return false;
+    for (int k = 1; k < heads; ++k)
+#pragma unroll
+      for (int t = 0; t < CT; ++t) acc[t] += buf[((wave + k) * CT + t) * 64 + lane];
+    return true;
+  }
+  __device__ __forceinline__ bool writer(int heads) const { return active && (heads == 1 || member == 0); }
+};
+
+// The decay's powers for chunks of 16 CT tokens
+template <int CT> struct Weights {
+  static constexpr int C = 16 * CT;
+  f32x4 inside[CT], whole[CT], tail[CT];   // scale g^{i-j} by tile distance (i = c, j = 4g + e); zs g^{n-1-j+sh} of whole chunks, and of the one of `tokens` that ends a sequence
+  float from[CT], whole_keep, tail_keep, g1;   // za g^{i+1-sh}; g^n - 1; g
+  int tokens;
+  __device__ __forceinline__ Weights(const Decay& decay, int c, int g, float scale, float za, float zs, int sh) {
+    g1 = decay.pow(1);
+    whole_keep = expm1f(decay.la * (float)C);
+    tail_keep = 0.f;
+    tokens = 0;
+#pragma unroll
+    for (int t = 0; t < CT; ++t) {   // (the fourth of four neighbouring powers, the others by one more factor each)
+      const int d = 16 * t + c - 4 * g, j = 16 * t + 4 * g;
+      inside[t][3] = scale * decay.pow(max(d - 3, 0));
+      whole[t][3] = zs * decay.pow(C - 4 - j + sh);
+#pragma unroll
+      for (int e = 2; e >= 0; --e) {
+        inside[t][e] = d - e > 0 ? inside[t][e + 1] * g1 : scale;
+        whole[t][e] = whole[t][e + 1] * g1;
+      }
+      tail[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+      from[t] = za * decay.pow(16 * t + c + 1 - sh);
+    }
+  }
+  __device__ __forceinline__ void length(const Decay& decay, int cnt, int g, float zs, int sh) {   // a sequence's last chunk has cnt tokens
+    if (cnt >= C || cnt == tokens) return;
+    tokens = cnt;
+    tail_keep = expm1f(decay.la * (float)cnt);
+    const float w0 = zs * decay.pow(sh);
+#pragma unroll
+    for (int t = 0; t < CT; ++t) {
+      const int d = cnt - 1 - 16 * t - 4 * g;   // tokens behind the first of the four
+      float w = zs * decay.pow(max(d - 3, 0) + sh);
+#pragma unroll
+      for (int e = 3; e >= 0; --e) {
+        if (e < 3) w = d - e > 0 ? w * g1 : w0;
+        tail[t][e] = d - e >= 0 ? w : 0.f;
+      }
+    }
+  }
+  __device__ __forceinline__ f32x4 into(int cnt, int t) const { return cnt < C ? tail[t] : whole[t]; }
+  __device__ __forceinline__ f32x4 kept(f32x4 s, int cnt) const {   // g^n S as S + (g^n - 1) S: a slow decay's last bits stay
+    const float k = cnt < C ? tail_keep : whole_keep;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s[e] = fmaf(s[e], k, s[e]);
+    return s;
+  }
+  __device__ __forceinline__ f32x4 masked(f32x4 x, int it, int jt, int c, int g) const {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = jt < it || 4 * g + e <= c ? x[e] * inside[it - jt][e] : 0.f;
+    return x;
+  }
+};
+
+// acc[it][n][i] += sum_j c_j[n] scores[j][i].  A later token's infinity or NaN must not reach an earlier token's sum as 0 * inf: a chunk that
+// holds one goes token by token
+template <typename T, int CT>
+__device__ __forceinline__ void weighted_sum(f32x4* acc, const typename Mat<T>::Split (&ps)[CT][CT], const typename Mat<T>::Op* co, const f32x4* cf, int c, int g) {
+  typedef Mat<T> X;
+  float top = 0.f;
+#pragma unroll
+  for (int t = 0; t < CT; ++t)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) top = __builtin_elementwise_maximum(top, __builtin_fabsf(cf[t][e]));   // (a NaN stays)
+  auto inner = [&](int it, typename X::Op last, f32x4 y) {
+    if constexpr (CT == 1) return X::score(last, ps[0][0], y);
+    else return it == 0 ? X::score(last, ps[0][0], y) : X::score2(co[0], last, ps[0][1], ps[1][1], y);
+  };
+  if (__builtin_expect(__any(!(top <= 3.4028234e38f)), 0)) {
+#pragma unroll
+    for (int it = 0; it < CT; ++it) {
+      const f32x4 before = acc[it];
+#pragma unroll 1
+      for (int i = 0; i < 16; ++i) {
+        const f32x4 y = inner(it, X::upto(co[it], i + 1 - 4 * g), before);
+        if (c == i) acc[it] = y;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int it = 0; it < CT; ++it) acc[it] = inner(it, co[it], acc[it]);
+  }
+}
+
+// staged rows by columns: rows row0 + 4g .. + 3 of channel 16 t + c - a transposing read (16-bit), or one channel of four rows
+template <typename T> __device__ __forceinline__ typename Mat<T>::Raw columns(const char* area, int row_bytes, int row0, int t, int c, int g) {
+  if constexpr (ElemTraits<T>::kBytes == 2) {
+    typedef __attribute__((address_space(3))) s16x4* Lds;
+    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(area + (row0 + 4 * g + (c >> 2)) * row_bytes + (16 * t + 4 * (c & 3)) * 2));
+  } else {
+    f32x4 v;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = *reinterpret_cast<const float*>(area + (row0 + 4 * g + e) * row_bytes + (16 * t + c) * 4);
+    return v;
+  }
+}
+
+// Operands that are not aligned to 16 bytes, or whose channels do not fill them: every lane loads its tiles' elements itself.
+template <typename T, int MT, int CT, bool STATE> __global__ __launch_bounds__(256, 2) void la_plain_kernel(LaArgs p) {
+  typedef Mat<T> X;
+  typedef typename X::Raw Raw;
+  typedef typename X::Op Op;
+  constexpr int kBytes = ElemTraits<T>::kBytes;
+  constexpr int C = 16 * CT;
+  constexpr f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+  extern __shared__ __align__(16) char lds[];           // [2][waves][CT][64] sums of 4 floats if a role folds
+  const Wave<T, MT> w(p);
+  const Role& r = p.r[blockIdx.y];
+  const int lane = w.lane, c = w.c, g = w.g;
+  const int begin = blockIdx.z * p.seg, end = min(begin + p.seg, p.T);
+  const char* pa = reinterpret_cast<const char*>(r.a.p) + (w.h / r.a.shared) * r.a.sh * kBytes;
+  const char* pb = reinterpret_cast<const char*>(r.b.p) + (w.h / r.b.shared) * r.b.sh * kBytes;
+  const char* pc = reinterpret_cast<const char*>(r.c.p) + ((w.h / r.c.shared) * r.c.sh + w.slice * 16) * kBytes;
+  const int n0 = w.slice * 16 + 4 * g;                  // this lane's 4 columns of c's rows and of out
+  const int row_out = p.H / r.fold * r.N, out_bytes = r.out_f32 ? 4 : kBytes;
+  const Raw unit = X::one(c - 4 * g);
+  f32x4* const sums = reinterpret_cast<f32x4*>(lds);
+  Weights<CT> k(w.decay, c, g, p.scale, r.za, r.zs, r.sh);
+  int turn = 0;
+  for (int bi = w.bgroup; bi < p.B; bi += p.bgroups) {
+    const int n = p.lengths ? min(max(p.lengths[bi], 0), p.T) : p.T;
+    const char *qa = pa + bi * r.a.sb * kBytes, *qb = pb + bi * r.b.sb * kBytes, *qc = pc + bi * r.c.sb * kBytes;
+    f32x4 S[MT];
+    const bool s0 = w.template first<STATE>(p, r, bi, S);
+    for (int t0 = begin; t0 < end; t0 += C, ++turn) {
+      const int cnt = min(C, n - t0);
+      f32x4 acc[CT];
+#pragma unroll
+      for (int t = 0; t < CT; ++t) acc[t] = zero;
+      if (cnt > 0) {
+        // (behind the last token its row again: those scores lie above every valid token's diagonal and their weights in the state are 0)
+        Raw av[CT][MT], bv[CT][MT];
+        f32x4 cf[CT];
+#pragma unroll
+        for (int it = 0; it < CT; ++it) {
+          const int idx = min(t0 + 16 * it + c, n - 1);
+          const int64_t tok = r.reverse ? n - 1 - idx : idx;
+#pragma unroll
+          for (int t = 0; t < MT; ++t) {
+            const int m = 16 * t + 4 * g;
+            if (!STATE) av[it][t] = load4<T>(qa + (tok * r.a.st + m) * kBytes, r.M - m, r.wide);
+            bv[it][t] = load4<T>(qb + (tok * r.b.st + m) * kBytes, r.M - m, r.wide);
+          }
+          // by columns: a product with the identity turns a tile (exactly)
+          cf[it] = X::raw(load4<T>(qc + (tok * r.c.st + 4 * g) * kBytes, r.N - n0, r.wide), unit, zero);
+        }
+        if constexpr (!STATE) {
+          typename X::Split ps[CT][CT];
+#pragma unroll
+          for (int it = 0; it < CT; ++it)
+#pragma unroll
+            for (int jt = 0; jt <= it; ++jt) {
+              f32x4 x = zero;
+              if constexpr (MT == 1) x = X::raw(bv[jt][0], av[it][0], x);
+              else
+#pragma unroll
+                for (int t = 0; t < MT; t += 2) x = X::raw2(bv[jt][t], bv[jt][t + 1], av[it][t], av[it][t + 1], x);
+              ps[jt][it] = X::split(k.masked(x, it, jt, c, g));
+            }
+          if (s0 || t0 > begin) {
+#pragma unroll
+            for (int t = 0; t < MT; t += MT == 1 ? 1 : 2)
+#pragma unroll
+              for (int it = 0; it < CT; ++it) {
+                if constexpr (MT == 1) acc[it] = X::state(X::split(S[0]), X::op(av[it][0]), acc[it]);
+                else acc[it] = X::state2(X::split(S[t]), X::split(S[t + 1]), X::op(av[it][t]), X::op(av[it][t + 1]), acc[it]);
+              }
+#pragma unroll
+            for (int t = 0; t < CT; ++t) acc[t] *= k.from[t];
+          }
+          Op co[CT];
+#pragma unroll
+          for (int t = 0; t < CT; ++t) co[t] = X::op_of(cf[t]);
+          weighted_sum<T, CT>(acc, ps, co, cf, c, g);
+        }
+        k.length(w.decay, cnt, g, r.zs, r.sh);
+        typename X::Split3 ws[CT];
+#pragma unroll
+        for (int t = 0; t < CT; ++t) ws[t] = X::split3(cf[t] * k.into(cnt, t));
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+          Op b[CT];
+#pragma unroll
+          for (int jt = 0; jt < CT; ++jt) b[jt] = X::op_of(X::raw(bv[jt][t], unit, zero));
+          S[t] = X::template grown<CT>(k.kept(S[t], cnt), b, ws);
+        }
+      }
+      if constexpr (!STATE) {
+        const bool writes = w.template fold<CT>(acc, sums, r.fold, turn);
+        // (tokens behind the sequence's length get zeros)
+        char* const base = reinterpret_cast<char*>(r.out) + ((int64_t)bi * p.T * row_out + w.h / r.fold * r.N + n0) * out_bytes;
+#pragma unroll
+        for (int t = 0; t < CT; ++t) {
+          const int idx = t0 + 16 * t + c;
+          if (!writes || idx >= end || n0 >= r.N) continue;
+          if (idx >= n) acc[t] = zero;
+          char* const o = base + (int64_t)(r.reverse && idx < n ? n - 1 - idx : idx) * row_out * out_bytes;
+          if (kBytes == 4 || out_bytes == 4) {
+            if (r.wide) *reinterpret_cast<f32x4*>(o) = acc[t];
+            else
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (n0 + e < r.N) reinterpret_cast<float*>(o)[e] = acc[t][e];
+          } else if constexpr (kBytes == 2) {
+            const s16x4 v = X::to_out(acc[t]);
+            if (r.wide) *reinterpret_cast<s16x4*>(o) = v;
+            else
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (n0 + e < r.N) reinterpret_cast<short*>(o)[e] = v[e];
+          }
+        }
+      }
+    }
+    w.template last<STATE>(p, r, bi, S);
+  }
+}
+
+// How a chunk's rows reach a wave.  Where operands are aligned to 16 bytes and their channels fill 16-byte pieces, a wave reads whole rows, 16 bytes per
 // lane and neighbouring lanes side by side, into its own part of the LDS and takes the tiles from there.  (Tiles straight from memory -
 // 16 rows at a time, 8 bytes per lane - cost one L1 access per LANE: 54 per load instruction, and the L1s became the bound: 370 us
-// instead of 311 for 65536 sequences of 120 tokens, the more waves the worse.)  Otherwise every lane loads its tiles' elements itself.
-// The next chunk's rows are on their way, in registers, while this one is worked on.
+// instead of 311 for 65536 sequences of 120 tokens, the more waves the worse.)  The next chunk's rows are on their way, in registers,
+// while this one is worked on.
 template <typename T, int MT, int CT> struct Stage {
   static constexpr int kBytes = ElemTraits<T>::kBytes;
   static constexpr int C = 16 * CT;
@@ -248,9 +562,9 @@ template <typename T, int MT, int CT> struct Stage {
   static constexpr int kArea = C * (2 * kRow + kCRow);            // LDS of a wave
 };
 
-// A wave keeps one head's slice and walks the sequences bgroup, bgroup + bgroups, .. (the decay's powers are made once), every sequence's
-// tokens in chunks.
-template <typename T, int MT, int CT, bool STAGED, bool STATE> __global__ __launch_bounds__(256, 2) void la_kernel(LaArgs p) {
+// The staged form.  Addresses are a uniform pointer to the chunk's lowest token, which moves on by a constant, and every lane's own offset:
+// the loop holds no multiplication and no scalar load (with both, 187 scalar instructions and 7 loads stood beside 325 vector ones a chunk).
+template <typename T, int MT, int CT, bool STATE> __global__ __launch_bounds__(256, 2) void la_kernel(LaArgs p) {
   typedef Mat<T> X;
   typedef Stage<T, MT, CT> G;
   typedef typename X::Raw Raw;
@@ -258,403 +572,221 @@ template <typename T, int MT, int CT, bool STAGED, bool STATE> __global__ __laun
   constexpr int kBytes = ElemTraits<T>::kBytes;
   constexpr int C = 16 * CT;
   constexpr f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-  extern __shared__ __align__(16) char lds[];           // [waves][kArea] if STAGED, then [2][waves][CT][64] sums of 4 floats if a role folds
+  extern __shared__ __align__(16) char lds[];           // [waves][kArea], then [2][waves][CT][64] sums of 4 floats if a role folds
+  const Wave<T, MT> w(p);
   const Role& r = p.r[blockIdx.y];
-  const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
-  const int slices = (r.N + 15) >> 4;
-  const int per = waves / p.group;                                   // (stored head, slice) pairs of a workgroup
-  const int f = blockIdx.x % p.columns * per + wave / p.group, member = wave % p.group, bgroup = blockIdx.x / p.columns;
-  const bool active = f < p.H / p.group * slices;                   // (a wave without work still meets the barriers of the summed roles)
-  const int slice = f % slices, h = active ? f / slices * p.group + member : 0;
-  const int segment = blockIdx.z;
-  const int begin = segment * p.seg, end = min(begin + p.seg, p.T);
-  const Decay decay(p.log_decay[h]);
-  const char* pa = reinterpret_cast<const char*>(r.a.p) + (h / r.a.shared) * r.a.sh * kBytes;
-  const char* pb = reinterpret_cast<const char*>(r.b.p) + (h / r.b.shared) * r.b.sh * kBytes;
-  const char* pc = reinterpret_cast<const char*>(r.c.p) + ((h / r.c.shared) * r.c.sh + slice * 16) * kBytes;
-  const int col = slice * 16 + c;                       // this lane's column of S and of c's transposed tile
-  const int n0 = slice * 16 + 4 * g;                    // its 4 columns of c's rows and of out
-  const bool has_col = active && col < r.N;
-  const int64_t states = (int64_t)r.M * r.N;
-  const int row_out = p.H / r.fold * r.N, out_bytes = r.out_f32 ? 4 : kBytes;   // elements of one token of out
-  const Raw unit = X::one(c - 4 * g);
-  char* const area_a = lds + wave * (STAGED ? G::kArea : 0);
+  const int lane = w.lane, c = w.c, g = w.g, reverse = r.reverse, N = r.N, B = p.B, step = p.bgroups;
+  const int begin = blockIdx.z * p.seg, end = min(begin + p.seg, p.T);
+  char* const area_a = lds + w.wave * G::kArea;
   char* const area_b = area_a + C * G::kRow;
   char* const area_c = area_b + C * G::kRow;
-  f32x4* const sums = reinterpret_cast<f32x4*>(lds + (STAGED ? waves * G::kArea : 0));
+  f32x4* const sums = reinterpret_cast<f32x4*>(lds + w.waves * G::kArea);
+  const int cols_bytes = r.out_f32 ? 4 : kBytes, to = p.H / r.fold * N * cols_bytes;   // bytes of a column, and of a token of out
+  const int ta = r.a.st * kBytes, tb = r.b.st * kBytes, tc = r.c.st * kBytes;
+  Weights<CT> k(w.decay, c, g, p.scale, r.za, r.zs, r.sh);
 
-  // scale g^{i-j} (i = 16 it + c, j = 16 jt + 4g + e; used on and below the diagonal) by it - jt, za g^{i+1-sh}; zs g^{n-1-j+sh} and g^n - 1 for
-  // whole chunks and for the one of `tail` tokens that ends a sequence
-  f32x4 inside[CT], whole_into[CT], tail_into[CT];
-  float from[CT];
-  const float whole_keep = expm1f(decay.la * (float)C);
-  float tail_keep = 0.f;
-  int tail = 0;
-  const float g1 = decay.pow(1);
-#pragma unroll
-  for (int t = 0; t < CT; ++t) {   // (the fourth of four neighbouring powers, the others by one more factor each)
-    tail_into[t] = zero;
-    const int d = 16 * t + c - 4 * g, j = 16 * t + 4 * g;
-    if (!STATE) inside[t][3] = p.scale * decay.pow(max(d - 3, 0));
-    whole_into[t][3] = r.zs * decay.pow(C - 4 - j + r.sh);
-#pragma unroll
-    for (int e = 2; e >= 0; --e) {
-      if (!STATE) inside[t][e] = d - e > 0 ? inside[t][e + 1] * g1 : p.scale;
-      whole_into[t][e] = whole_into[t][e + 1] * g1;
-    }
-    from[t] = r.za * decay.pow(16 * t + c + 1 - r.sh);
-  }
-
-  auto length = [&](int bi) { return !active || bi >= p.B ? 0 : p.lengths ? min(max(p.lengths[bi], 0), p.T) : p.T; };
-  const char *qa = nullptr, *qb = nullptr, *qc = nullptr;   // of the sequence that is fetched from
-  auto sequence = [&](int bi) {
-    qa = pa + bi * r.a.sb * kBytes;
-    qb = pb + bi * r.b.sb * kBytes;
-    qc = pc + bi * r.c.sb * kBytes;
+  // this lane's piece of a row, its row of a load, and its place in one of a whole chunk's loads
+  const int piece = lane % G::kLanes * 16, piece_c = lane % kBytes * 16, row_a = lane / G::kLanes, row_c = lane / kBytes;
+  const bool live_a = piece < r.M * kBytes && row_a < C, live_c = w.slice * 16 * kBytes + piece_c < N * kBytes && row_c < C;
+  const int up_a = reverse ? G::kRows - 1 - row_a : row_a, up_c = reverse ? G::kCRows - 1 - row_c : row_c;
+  const unsigned va = (unsigned)(up_a * ta + piece), vb = (unsigned)(up_a * tb + piece), vc = (unsigned)(up_c * tc + piece_c), vo = (unsigned)(up_c * to + piece_c);
+  // uniform: the lowest token of the next load of a, b, c, and of the next store of out; from load to load; back from a chunk's first load to its
+  // lowest token
+  const char *ca = nullptr, *cb = nullptr, *cc = nullptr;
+  char* co_at = nullptr;
+  const int64_t sign = reverse ? -1 : 1, da = sign * G::kRows * ta, db = sign * G::kRows * tb, dc = sign * G::kCRows * tc, d_out = sign * G::kCRows * to;
+  auto place = [&](int bi, int n) {   // at a sequence's first chunk
+    const int64_t tok = reverse ? n - begin - G::kRows : begin, tok_c = reverse ? n - begin - G::kCRows : begin;
+    ca = reinterpret_cast<const char*>(r.a.p) + (bi * r.a.sb + (w.h / r.a.shared) * r.a.sh + tok * r.a.st) * kBytes;
+    cb = reinterpret_cast<const char*>(r.b.p) + (bi * r.b.sb + (w.h / r.b.shared) * r.b.sh + tok * r.b.st) * kBytes;
+    cc = reinterpret_cast<const char*>(r.c.p) + (bi * r.c.sb + (w.h / r.c.shared) * r.c.sh + w.slice * 16 + tok_c * r.c.st) * kBytes;
   };
-  // The chunk at t0, on its way (behind the last token its row again: those scores lie above every valid token's diagonal and their weights in
-  // the state are 0)
   u32x4 fa[G::kLoads], fb[G::kLoads], fc[G::kCLoads];
-  Raw av[CT][MT], bv[CT][MT], cv[CT];
-  const int piece = lane % G::kLanes * 16, piece_c = lane % kBytes * 16;                             // bytes into a row
-  const bool piece_live = piece < r.M * kBytes, piece_c_live = slice * 16 * kBytes + piece_c < r.N * kBytes;   // channels behind M, N: zeros
-  const int row_a = lane / G::kLanes, row_c = lane / kBytes;                                          // of each load
-  const bool live_a = piece_live && row_a < C, live_c = piece_c_live && row_c < C;
-  // bytes from the lowest of a load's tokens to this lane's row
-  const int up_a = r.reverse ? G::kRows - 1 - row_a : row_a, up_c = r.reverse ? G::kCRows - 1 - row_c : row_c;
-  const unsigned va = (unsigned)(up_a * r.a.st * kBytes + piece), vb = (unsigned)(up_a * r.b.st * kBytes + piece), vc = (unsigned)(up_c * r.c.st * kBytes + piece_c);
-  auto fetch = [&](int t0, int n) {
-    if constexpr (STAGED) {
-#pragma unroll
-      for (int i = 0; i < G::kLoads; ++i) {
-        if (!STATE) fa[i] = u32x4{0, 0, 0, 0};
-        fb[i] = u32x4{0, 0, 0, 0};
-      }
-#pragma unroll
-      for (int i = 0; i < G::kCLoads; ++i) fc[i] = u32x4{0, 0, 0, 0};
-      if (t0 + C <= n) {   // a whole chunk: uniform addresses, every lane its own fixed place
-        if (live_a)
-#pragma unroll
-          for (int i = 0; i < G::kLoads; ++i) {
-            const int64_t tok = r.reverse ? n - t0 - (i + 1) * G::kRows : t0 + i * G::kRows;
-            if (!STATE) fa[i] = *reinterpret_cast<const u32x4*>(qa + tok * r.a.st * kBytes + va);
-            fb[i] = *reinterpret_cast<const u32x4*>(qb + tok * r.b.st * kBytes + vb);
-          }
-        if (live_c)
-#pragma unroll
-          for (int i = 0; i < G::kCLoads; ++i) {
-            const int64_t tok = r.reverse ? n - t0 - (i + 1) * G::kCRows : t0 + i * G::kCRows;
-            fc[i] = *reinterpret_cast<const u32x4*>(qc + tok * r.c.st * kBytes + vc);
-          }
-      } else {
-        auto token = [&](int row) {
-          const int idx = min(t0 + row, n - 1);
-          return (int64_t)(r.reverse ? n - 1 - idx : idx);
-        };
-        if (live_a)
-#pragma unroll
-          for (int i = 0; i < G::kLoads; ++i) {
-            const int64_t tok = token(i * G::kRows + row_a);
-            if (!STATE) fa[i] = *reinterpret_cast<const u32x4*>(qa + tok * r.a.st * kBytes + piece);
-            fb[i] = *reinterpret_cast<const u32x4*>(qb + tok * r.b.st * kBytes + piece);
-          }
-        if (live_c)
-#pragma unroll
-          for (int i = 0; i < G::kCLoads; ++i)
-            fc[i] = *reinterpret_cast<const u32x4*>(qc + token(i * G::kCRows + row_c) * r.c.st * kBytes + piece_c);
-      }
-    } else {
-#pragma unroll
-      for (int it = 0; it < CT; ++it) {
-        const int idx = min(t0 + 16 * it + c, n - 1);
-        const int64_t tok = r.reverse ? n - 1 - idx : idx;
-#pragma unroll
-        for (int t = 0; t < MT; ++t) {
-          const int m = 16 * t + 4 * g;
-          if (!STATE) av[it][t] = load4<T>(qa + (tok * r.a.st + m) * kBytes, r.M - m, r.wide);
-          bv[it][t] = load4<T>(qb + (tok * r.b.st + m) * kBytes, r.M - m, r.wide);
-        }
-        cv[it] = load4<T>(qc + (tok * r.c.st + 4 * g) * kBytes, r.N - n0, r.wide);
-      }
-    }
-  };
-  // from the registers into the wave's LDS (which the wave alone reads; its LDS operations run in order)
-  auto stage = [&]() {
-    if constexpr (STAGED) {
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      __builtin_amdgcn_wave_barrier();
-      if (row_a < C)
+  auto fetch = [&](int cnt) {
+    if (cnt >= C) {
+      if (live_a)
 #pragma unroll
         for (int i = 0; i < G::kLoads; ++i) {
-          if (!STATE) *reinterpret_cast<u32x4*>(area_a + (i * G::kRows + row_a) * G::kRow + piece) = fa[i];
-          *reinterpret_cast<u32x4*>(area_b + (i * G::kRows + row_a) * G::kRow + piece) = fb[i];
+          if (!STATE) fa[i] = *reinterpret_cast<const u32x4*>(ca + i * da + va);
+          fb[i] = *reinterpret_cast<const u32x4*>(cb + i * db + vb);
         }
-      if (row_c < C)
+      if (live_c)
 #pragma unroll
-        for (int i = 0; i < G::kCLoads; ++i) *reinterpret_cast<u32x4*>(area_c + (i * G::kCRows + row_c) * G::kCRow + piece_c) = fc[i];
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      __builtin_amdgcn_wave_barrier();
-    }
-  };
-  auto A = [&](int it, int t) { if constexpr (STAGED) return *reinterpret_cast<const Raw*>(area_a + (16 * it + c) * G::kRow + (16 * t + 4 * g) * kBytes); else return av[it][t]; };
-  auto Bt = [&](int it, int t) { if constexpr (STAGED) return *reinterpret_cast<const Raw*>(area_b + (16 * it + c) * G::kRow + (16 * t + 4 * g) * kBytes); else return bv[it][t]; };
-  // by columns: tokens 16 jt + 4g .. + 3 of channel 16 t + c: a transposing read (16-bit), or one channel of four rows
-  auto columns = [&](const char* area, int row_bytes, int jt, int t) {
-    if constexpr (kBytes == 2) {
-      typedef __attribute__((address_space(3))) s16x4* Lds;
-      return __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(area + (16 * jt + 4 * g + (c >> 2)) * row_bytes + (16 * t + 4 * (c & 3)) * 2));
-    } else {
-      Raw v;
+        for (int i = 0; i < G::kCLoads; ++i) fc[i] = *reinterpret_cast<const u32x4*>(cc + i * dc + vc);
+    } else {   // cnt tokens (behind the last one its row again: those scores lie above every valid token's diagonal and their weights in the state are 0)
+      auto at = [&](int row, int rows) { return (int64_t)(reverse ? rows - 1 - min(row, cnt - 1) : min(row, cnt - 1)); };
+      if (live_a)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = *reinterpret_cast<const float*>(area + (16 * jt + 4 * g + e) * row_bytes + (16 * t + c) * 4);
-      return v;
+        for (int i = 0; i < G::kLoads; ++i) {
+          const int64_t row = at(i * G::kRows + row_a, G::kRows);
+          if (!STATE) fa[i] = *reinterpret_cast<const u32x4*>(ca + row * ta + piece);
+          fb[i] = *reinterpret_cast<const u32x4*>(cb + row * tb + piece);
+        }
+      if (live_c)
+#pragma unroll
+        for (int i = 0; i < G::kCLoads; ++i) fc[i] = *reinterpret_cast<const u32x4*>(cc + at(i * G::kCRows + row_c, G::kCRows) * tc + piece_c);
     }
+    ca += G::kLoads * da;
+    cb += G::kLoads * db;
+    cc += G::kCLoads * dc;
   };
-  auto Ct = [&](int it) { if constexpr (STAGED) return *reinterpret_cast<const Raw*>(area_c + (16 * it + c) * G::kCRow + 4 * g * kBytes); else return cv[it]; };
+  // into the wave's LDS, which the wave alone reads (its LDS operations run in order).  Channels behind M and N were cleared once
+  auto stage = [&]() {
+    wave_fence();
+    if (live_a)
+#pragma unroll
+      for (int i = 0; i < G::kLoads; ++i) {
+        if (!STATE) *reinterpret_cast<u32x4*>(area_a + (i * G::kRows + row_a) * G::kRow + piece) = fa[i];
+        *reinterpret_cast<u32x4*>(area_b + (i * G::kRows + row_a) * G::kRow + piece) = fb[i];
+      }
+    if (live_c)
+#pragma unroll
+      for (int i = 0; i < G::kCLoads; ++i) *reinterpret_cast<u32x4*>(area_c + (i * G::kCRows + row_c) * G::kCRow + piece_c) = fc[i];
+    wave_fence();
+  };
+  if (!w.whole(r))
+    for (int i = lane * 16; i < G::kArea; i += 1024) *reinterpret_cast<u32x4*>(area_a + i) = u32x4{0, 0, 0, 0};
+  auto A = [&](int it, int t) { return *reinterpret_cast<const Raw*>(area_a + (16 * it + c) * G::kRow + (16 * t + 4 * g) * kBytes); };
+  auto Bm = [&](int it, int t) { return *reinterpret_cast<const Raw*>(area_b + (16 * it + c) * G::kRow + (16 * t + 4 * g) * kBytes); };
 
-  int n = length(bgroup), n_next = 0;
-  sequence(bgroup);
-  if (begin < n) fetch(begin, n);
-  int turn = 0;
-  for (int bi = bgroup; bi < p.B; bi += p.bgroups, n = n_next) {
-    n_next = length(bi + p.bgroups);
-    const int64_t pair = (int64_t)bi * p.H + h;
-    float* const s1 = STATE ? r.seg + (pair * p.segments + segment + 1) * states : segment == p.segments - 1 && r.s1 ? r.s1 + pair * states : nullptr;
-    const float* s0 = STATE ? nullptr : p.segments > 1 ? r.seg + (pair * p.segments + segment) * states : r.s0 ? r.s0 + pair * states : nullptr;
+  auto length = [&](int bi) { return bi >= B ? 0 : p.lengths ? min(max(p.lengths[bi], 0), p.T) : p.T; };
+  int n = length(w.bgroup), n_next = length(w.bgroup + step), turn = 0;
+  if (begin < n) {
+    place(w.bgroup, n);
+    fetch(n - begin);
+  }
+  for (int bi = w.bgroup; bi < B; bi += step, n = n_next, n_next = length(bi + step)) {
+    const int stop = min(n, end);
     f32x4 S[MT];
-#pragma unroll
-    for (int t = 0; t < MT; ++t) {
-      S[t] = zero;
-      if (s0)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int m = 16 * t + 4 * g + e;
-          const float v = s0[min(m, r.M - 1) * r.sm + min(col, r.N - 1) * r.sn];
-          S[t][e] = m < r.M && has_col ? v : 0.f;
-        }
-    }
-    for (int t0 = begin; t0 < end; t0 += C, ++turn) {
-      const int cnt = min(C, n - t0);
-      f32x4 acc[CT], cf[CT], x[CT][CT];
-      Op bt[STAGED ? 1 : MT][CT];
-#pragma unroll
-      for (int t = 0; t < CT; ++t) acc[t] = zero;
-      auto next = [&]() {   // the next chunk, of this sequence or of the wave's next one
-        const bool more = t0 + C < end;
-        const int t1 = more ? t0 + C : begin, n1 = more ? n : n_next;
-        if (!more) sequence(bi + p.bgroups);
-        if (t1 < n1) fetch(t1, n1);
-      };
-      if (STAGED) {
-        if (cnt > 0) stage();
-        next();
+    const bool s0 = w.template first<STATE>(p, r, bi, S), s1 = STATE || (blockIdx.z == (unsigned)p.segments - 1 && r.s1);
+    char* const out = reinterpret_cast<char*>(r.out) + ((int64_t)bi * p.T * (p.H / r.fold) * N + w.h / r.fold * N + w.slice * 16) * cols_bytes;
+    co_at = out + (int64_t)(reverse ? n - begin - G::kCRows : begin) * to;
+    auto next_sequence = [&]() {
+      if (begin < n_next) {
+        place(bi + step, n_next);
+        fetch(n_next - begin);
       }
-      const bool from_state = s0 || t0 > begin, to_state = s1 || t0 + C < min(n, end);   // (nothing is read from a state of zeros, or added to one that nobody reads)
-      if (cnt > 0) {
-        // c by columns: tokens 4g .. 4g+3 of column `col`
+    };
+    if (begin >= n) next_sequence();
+    for (int t0 = begin; t0 < stop; t0 += C, ++turn) {
+      const int cnt = min(C, stop - t0);
+      stage();
+      if (t0 + C < stop) fetch(stop - t0 - C);
+      else next_sequence();
+      f32x4 acc[CT], cf[CT];
+      Raw craw[CT];
 #pragma unroll
-        for (int t = 0; t < CT; ++t) {
-          if constexpr (STAGED) cf[t] = X::to_float(columns(area_c, G::kCRow, t, 0));
-          else cf[t] = X::raw(Ct(t), unit, zero);
-        }
-        if constexpr (!STATE) {
-          // scores x[jt][it][j][i] = b_j . a_i, and acc[it][n][i] = sum_m S[m][n] a_i[m]
-#pragma unroll
-          for (int it = 0; it < CT; ++it)
-#pragma unroll
-            for (int jt = 0; jt <= it; ++jt) x[jt][it] = zero;
-          if constexpr (MT == 1) {
-            Raw b[CT];
-#pragma unroll
-            for (int it = 0; it < CT; ++it) {
-              b[it] = Bt(it, 0);
-#pragma unroll
-              for (int jt = 0; jt <= it; ++jt) x[jt][it] = X::raw(b[jt], A(it, 0), zero);
-            }
-          } else {
-#pragma unroll
-            for (int t = 0; t < MT; t += 2) {
-              Raw b0[CT], b1[CT];
-#pragma unroll
-              for (int it = 0; it < CT; ++it) {
-                b0[it] = Bt(it, t);
-                b1[it] = Bt(it, t + 1);
-#pragma unroll
-                for (int jt = 0; jt <= it; ++jt) x[jt][it] = X::raw2(b0[jt], b1[jt], A(it, t), A(it, t + 1), x[jt][it]);
-              }
-            }
-          }
-          if (from_state) {
-            if constexpr (MT == 1) {
-              const typename X::Split s = X::split(S[0]);
-#pragma unroll
-              for (int it = 0; it < CT; ++it) acc[it] = X::state(s, X::op(A(it, 0)), zero);
-            } else {
-#pragma unroll
-              for (int t = 0; t < MT; t += 2) {
-                const typename X::Split s = X::split(S[t]), u = X::split(S[t + 1]);
-#pragma unroll
-                for (int it = 0; it < CT; ++it) acc[it] = X::state2(s, u, X::op(A(it, t)), X::op(A(it, t + 1)), acc[it]);
-              }
-            }
-#pragma unroll
-            for (int t = 0; t < CT; ++t) acc[t] *= from[t];
-          }
-        }
-        if constexpr (!STAGED) {
-#pragma unroll
-          for (int t = 0; t < MT; ++t)
-#pragma unroll
-            for (int jt = 0; jt < CT; ++jt) bt[t][jt] = X::op_of(X::raw(bv[jt][t], unit, zero));
-        }
-      }
-      if (!STAGED) next();   // (a, b, c are used up)
-      if (cnt > 0) {
-        if constexpr (!STATE) {
-          typename X::Split ps[CT][CT];
-#pragma unroll
-          for (int it = 0; it < CT; ++it)
-#pragma unroll
-            for (int jt = 0; jt <= it; ++jt) {
-#pragma unroll
-              for (int e = 0; e < 4; ++e) x[jt][it][e] = jt < it || 4 * g + e <= c ? x[jt][it][e] * inside[it - jt][e] : 0.f;
-              ps[jt][it] = X::split(x[jt][it]);
-            }
-          Op co[CT];
-          float top = 0.f;
-#pragma unroll
-          for (int t = 0; t < CT; ++t) {
-            co[t] = X::op_of(cf[t]);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) top = __builtin_elementwise_maximum(top, __builtin_fabsf(cf[t][e]));   // (a NaN stays)
-          }
-          // acc[it][n][i] += sum_j c_j[n] scores[j][i].  A later token's infinity or NaN must not reach an earlier token's sum as 0 * inf: a
-          // chunk that holds one goes token by token
-          auto inner = [&](int it, Op last, f32x4 y) {
-            if constexpr (CT == 1) return X::score(last, ps[0][0], y);
-            else return it == 0 ? X::score(last, ps[0][0], y) : X::score2(co[0], last, ps[0][1], ps[1][1], y);
-          };
-          if (__builtin_expect(__any(!(top <= 3.4028234e38f)), 0)) {
-#pragma unroll
-            for (int it = 0; it < CT; ++it) {
-              const f32x4 before = acc[it];
-#pragma unroll 1
-              for (int i = 0; i < 16; ++i) {
-                const f32x4 y = inner(it, X::upto(co[it], i + 1 - 4 * g), before);
-                if (c == i) acc[it] = y;
-              }
-            }
-          } else {
-#pragma unroll
-            for (int it = 0; it < CT; ++it) acc[it] = inner(it, co[it], acc[it]);
-          }
-        }
-        if (to_state && cnt < C && cnt != tail) {
-          tail = cnt;
-          tail_keep = expm1f(decay.la * (float)cnt);
-#pragma unroll
-          for (int t = 0; t < CT; ++t) {
-            const int d = cnt - 1 - 16 * t - 4 * g;   // tokens behind the first of the four
-            const float w0 = r.zs * decay.pow(r.sh);
-            float w = r.zs * decay.pow(max(d - 3, 0) + r.sh);
-#pragma unroll
-            for (int e = 3; e >= 0; --e) {
-              if (e < 3) w = d - e > 0 ? w * g1 : w0;
-              tail_into[t][e] = d - e >= 0 ? w : 0.f;
-            }
-          }
-        }
-        // S[m][n] = g^n S[m][n] + sum_j b_j[m] (into_j c_j[n]); S + (g^n - 1) S keeps a slow decay's last bits
-        if (to_state) {
-          typename X::Split3 ws[CT];
-#pragma unroll
-          for (int t = 0; t < CT; ++t) ws[t] = X::split3(cf[t] * (cnt < C ? tail_into[t] : whole_into[t]));
-          const float keep = cnt < C ? tail_keep : whole_keep;
-#pragma unroll
-          for (int t = 0; t < MT; ++t) {
-            Op b[CT];   // b by columns: tokens 4g .. 4g+3 of column 16 t + c
-#pragma unroll
-            for (int jt = 0; jt < CT; ++jt) {
-              if constexpr (STAGED) b[jt] = X::op(columns(area_b, G::kRow, jt, t));
-              else b[jt] = bt[t][jt];
-            }
-#pragma unroll
-            for (int e = 0; e < 4; ++e) S[t][e] = fmaf(S[t][e], keep, S[t][e]);
-            if constexpr (CT == 1) S[t] = X::add(b[0], ws[0], S[t]);
-            else S[t] = X::add2(b[0], b[1], ws[0], ws[1], S[t]);
-          }
-        }
+      for (int t = 0; t < CT; ++t) {
+        craw[t] = columns<T>(area_c, G::kCRow, 16 * t, 0, c, g);
+        acc[t] = zero;
       }
       if constexpr (!STATE) {
-        bool writes = active;
-        if (r.fold > 1) {   // (uniform over the launch's role) the heads of one stored head add up in the first one's wave
-          f32x4* const buf = sums + (turn & 1) * waves * CT * 64;
+        // scores x[jt][it][j][i] = b_j . a_i
+        f32x4 x[CT][CT];
 #pragma unroll
-          for (int t = 0; t < CT; ++t) buf[(wave * CT + t) * 64 + lane] = acc[t];
-          __syncthreads();   // (two buffers: who writes this one again has passed the next barrier, and so have its readers)
-          writes = active && member == 0;
-          if (writes)
-            for (int k = 1; k < r.fold; ++k)
+        for (int it = 0; it < CT; ++it)
 #pragma unroll
-              for (int t = 0; t < CT; ++t) acc[t] += buf[((wave + k) * CT + t) * 64 + lane];
-        }
-        // (tokens behind the sequence's length get zeros)
-        char* const base = reinterpret_cast<char*>(r.out) + ((int64_t)bi * p.T * row_out + h / r.fold * r.N + slice * 16) * out_bytes;
-        auto place = [&](int idx) { return base + (int64_t)(r.reverse && idx < n ? n - 1 - idx : idx) * row_out * out_bytes; };
+          for (int jt = 0; jt <= it; ++jt) x[jt][it] = zero;
+        if constexpr (MT == 1) {
+          Raw b[CT];
 #pragma unroll
-        for (int t = 0; t < CT; ++t)
-          if (t0 + 16 * t + c >= n) acc[t] = zero;
-        if (STAGED && (kBytes == 4 || out_bytes == kBytes)) {   // through c's place in the LDS: whole rows again, 16 bytes per lane
-          if (writes) {
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            __builtin_amdgcn_wave_barrier();
+          for (int it = 0; it < CT; ++it) {
+            b[it] = Bm(it, 0);
 #pragma unroll
-            for (int t = 0; t < CT; ++t) {
-              char* const o = area_c + (16 * t + c) * G::kCRow + 4 * g * kBytes;
-              if constexpr (kBytes == 4) *reinterpret_cast<f32x4*>(o) = acc[t];
-              else *reinterpret_cast<s16x4*>(o) = X::to_out(acc[t]);
-            }
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            __builtin_amdgcn_wave_barrier();
-#pragma unroll
-            for (int i = 0; i < G::kCLoads; ++i) {
-              const int row = i * G::kCRows + row_c;
-              if (live_c && t0 + row < end)
-                *reinterpret_cast<u32x4*>(place(t0 + row) + piece_c) = *reinterpret_cast<const u32x4*>(area_c + row * G::kCRow + piece_c);
-            }
+            for (int jt = 0; jt <= it; ++jt) x[jt][it] = X::raw(b[jt], A(it, 0), zero);
           }
         } else {
 #pragma unroll
-          for (int t = 0; t < CT; ++t) {
-            const int idx = t0 + 16 * t + c;
-            if (!writes || idx >= end || n0 >= r.N) continue;
-            char* const o = place(idx) + 4 * g * out_bytes;
-            if (kBytes == 4 || out_bytes == 4) {
-              if (r.wide) *reinterpret_cast<f32x4*>(o) = acc[t];
-              else
+          for (int t = 0; t < MT; t += 2) {
+            Raw b0[CT], b1[CT];
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                  if (n0 + e < r.N) reinterpret_cast<float*>(o)[e] = acc[t][e];
-            } else if constexpr (kBytes == 2) {
-              const s16x4 v = X::to_out(acc[t]);
-              if (r.wide) *reinterpret_cast<s16x4*>(o) = v;
-              else
+            for (int it = 0; it < CT; ++it) {
+              b0[it] = Bm(it, t);
+              b1[it] = Bm(it, t + 1);
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                  if (n0 + e < r.N) reinterpret_cast<short*>(o)[e] = v[e];
+              for (int jt = 0; jt <= it; ++jt) x[jt][it] = X::raw2(b0[jt], b1[jt], A(it, t), A(it, t + 1), x[jt][it]);
             }
           }
         }
+        if (s0 || t0 > begin) {   // acc[it][n][i] = za g^{i+1-sh} sum_m S[m][n] a_i[m]; nothing is read from a state of zeros
+          if constexpr (MT == 1) {
+            const typename X::Split s = X::split(S[0]);
+#pragma unroll
+            for (int it = 0; it < CT; ++it) acc[it] = X::state(s, X::op(A(it, 0)), zero);
+          } else {
+#pragma unroll
+            for (int t = 0; t < MT; t += 2) {
+              const typename X::Split s = X::split(S[t]), u = X::split(S[t + 1]);
+#pragma unroll
+              for (int it = 0; it < CT; ++it) acc[it] = X::state2(s, u, X::op(A(it, t)), X::op(A(it, t + 1)), acc[it]);
+            }
+          }
+#pragma unroll
+          for (int t = 0; t < CT; ++t) acc[t] *= k.from[t];
+        }
+        typename X::Split ps[CT][CT];
+        Op co[CT];
+#pragma unroll
+        for (int it = 0; it < CT; ++it) {
+#pragma unroll
+          for (int jt = 0; jt <= it; ++jt) ps[jt][it] = X::split(k.masked(x[jt][it], it, jt, c, g));
+          cf[it] = X::to_float(craw[it]);
+          co[it] = X::op(craw[it]);
+        }
+        weighted_sum<T, CT>(acc, ps, co, cf, c, g);
+      } else {
+#pragma unroll
+        for (int t = 0; t < CT; ++t) cf[t] = X::to_float(craw[t]);
+      }
+      if (s1 || t0 + C < stop) {   // (nothing is added to a state that nobody reads)
+        k.length(w.decay, cnt, g, r.zs, r.sh);
+        typename X::Split3 ws[CT];
+#pragma unroll
+        for (int t = 0; t < CT; ++t) ws[t] = X::split3(cf[t] * k.into(cnt, t));
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+          Op b[CT];
+#pragma unroll
+          for (int jt = 0; jt < CT; ++jt) b[jt] = X::op(columns<T>(area_b, G::kRow, 16 * jt, t, c, g));
+          S[t] = X::template grown<CT>(k.kept(S[t], cnt), b, ws);
+        }
+      }
+      if constexpr (!STATE) {
+        const bool writes = w.template fold<CT>(acc, sums, r.fold, turn);
+        if (writes && cols_bytes == kBytes) {   // through c's place in the LDS: whole rows again, 16 bytes per lane
+          wave_fence();
+#pragma unroll
+          for (int t = 0; t < CT; ++t) {
+            char* const o = area_c + (16 * t + c) * G::kCRow + 4 * g * kBytes;
+            if constexpr (kBytes == 4) *reinterpret_cast<f32x4*>(o) = acc[t];
+            else *reinterpret_cast<s16x4*>(o) = X::to_out(acc[t]);
+          }
+          wave_fence();
+          if (live_c)
+#pragma unroll
+            for (int i = 0; i < G::kCLoads; ++i) {
+              const int row = i * G::kCRows + row_c;
+              if (row < cnt)
+                *reinterpret_cast<u32x4*>(co_at + i * d_out + vo) = *reinterpret_cast<const u32x4*>(area_c + row * G::kCRow + piece_c);
+            }
+        } else if (writes) {
+#pragma unroll
+          for (int t = 0; t < CT; ++t) {
+            const int row = 16 * t + c;
+            if (row < cnt && w.slice * 16 + 4 * g < N) *reinterpret_cast<f32x4*>(co_at + (int64_t)(reverse ? G::kCRows - 1 - row : row) * to + 16 * g) = acc[t];
+          }
+        }
+        co_at += G::kCLoads * d_out;
       }
     }
-    if (s1 && has_col)
-#pragma unroll
-      for (int t = 0; t < MT; ++t)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int m = 16 * t + 4 * g + e;
-          if (m < r.M) s1[m * r.sm + col * r.sn] = S[t][e];
-        }
+    if (!STATE && w.writer(r.fold)) {   // tokens behind the sequence's length get zeros
+      const int wide = 16 * cols_bytes;   // bytes of the slice in a row: pieces of 16
+      for (int i = lane; i < max(end - max(n, begin), 0) * (wide / 16); i += 64) {
+        const int at = i % (wide / 16) * 16, tok = max(n, begin) + i / (wide / 16);
+        if (w.slice * wide + at < N * cols_bytes) *reinterpret_cast<u32x4*>(out + (int64_t)tok * to + at) = u32x4{0, 0, 0, 0};
+      }
+    }
+    w.template last<STATE>(p, r, bi, S);
   }
 }
 
@@ -1149,9 +1281,13 @@ int go(void (*kernel)(LaArgs), Resident& resident, int area, int ct, bool folds,
   kernel<<<grid, threads, lds, st>>>(a);
   return tg_launch_status();
 }
-template <typename T, int MT, int CT, bool STAGED, bool STATE> int go_long(const LaArgs& a, dim3 grid, int threads, hipStream_t st) {
+template <typename T, int MT, int CT, bool STATE> int go_long(const LaArgs& a, dim3 grid, int threads, hipStream_t st) {
   static Resident resident;
-  return go(la_kernel<T, MT, CT, STAGED, STATE>, resident, STAGED ? Stage<T, MT, CT>::kArea : 0, CT, !STATE && a.group > 1, a, grid, threads, st);
+  return go(la_kernel<T, MT, CT, STATE>, resident, Stage<T, MT, CT>::kArea, CT, !STATE && a.group > 1, a, grid, threads, st);
+}
+template <typename T, int MT, int CT, bool STATE> int go_plain(const LaArgs& a, dim3 grid, int threads, hipStream_t st) {
+  static Resident resident;
+  return go(la_plain_kernel<T, MT, CT, STATE>, resident, 0, CT, !STATE && a.group > 1, a, grid, threads, st);
 }
 template <typename T, int MT> int go_short(const LaArgs& a, dim3 grid, int threads, hipStream_t st) {
   static Resident resident;
@@ -1162,11 +1298,11 @@ template <typename T, int MT> int go_mt(const LaArgs& a, bool staged, bool state
   // fp32 channels, or of 128 channels that every lane loads itself, do not fit the registers
   constexpr int CT = MT == 8 && sizeof(typename Mat<T>::Raw) == 16 ? 1 : 2, CU = MT == 8 ? 1 : 2;
   if (staged) {
-    if (state) return go_long<T, MT, CT, true, true>(a, grid, threads, st);
-    return a.T <= 16 ? go_short<T, MT>(a, grid, threads, st) : go_long<T, MT, CT, true, false>(a, grid, threads, st);
+    if (state) return go_long<T, MT, CT, true>(a, grid, threads, st);
+    return a.T <= 16 ? go_short<T, MT>(a, grid, threads, st) : go_long<T, MT, CT, false>(a, grid, threads, st);
   }
-  if (state) return go_long<T, MT, CU, false, true>(a, grid, threads, st);
-  return a.T <= 16 ? go_long<T, MT, 1, false, false>(a, grid, threads, st) : go_long<T, MT, CU, false, false>(a, grid, threads, st);
+  if (state) return go_plain<T, MT, CU, true>(a, grid, threads, st);
+  return a.T <= 16 ? go_plain<T, MT, 1, false>(a, grid, threads, st) : go_plain<T, MT, CU, false>(a, grid, threads, st);
 }
 // `roles` roles with the same number of m tiles in one launch
 template <typename T> int launch(LaArgs a, int roles, bool state, hipStream_t st) {
