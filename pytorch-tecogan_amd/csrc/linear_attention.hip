@@ -225,7 +225,7 @@ struct LaArgs {
   int B, T, H;
   int group;               // waves of a workgroup that belong to one (stored head, slice)
   int columns, bgroups;    // blockIdx.x = bgroup * columns + column: workgroups over (stored head, slice), and over the sequences
-  int seg, segments;       // tokens in a segment (a multiple of 64)
+  int seg, segments;       // tokens in a segment (a multiple of 32)
   float scale;
   Role r[3];
 };
@@ -1246,7 +1246,7 @@ inline int tiles(int m) { return m <= 16 ? 1 : m <= 32 ? 2 : m <= 64 ? 4 : 8; }
 
 // Segments: as many as two waves per SIMD need, each of at least kMinSegment tokens
 constexpr int64_t kWaves = 2048;
-constexpr int kMinSegment = 128;
+constexpr int kMinSegment = 32;
 constexpr int kCUs = 256;
 
 // (tokens in a segment, segments) for `waves` waves per segment
@@ -1254,9 +1254,9 @@ void segmentation(int T, int64_t waves, int* seg, int* segments) {
   int64_t want = waves > 0 ? kWaves / waves : 1, most = T / kMinSegment;
   if (want > most) want = most;
   if (want > kMaxSegments) want = kMaxSegments;
-  if (want < 2) { *seg = (T + 63) / 64 * 64; *segments = 1; return; }
+  if (want < 2) { *seg = (T + 31) / 32 * 32; *segments = 1; return; }
   int64_t s = (T + want - 1) / want;
-  s = (s + 63) / 64 * 64;
+  s = (s + 31) / 32 * 32;
   *seg = (int)s;
   *segments = (int)((T + s - 1) / s);
 }
