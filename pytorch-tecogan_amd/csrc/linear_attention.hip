@@ -270,13 +270,25 @@ template <typename T, int MT> struct Wave {
   }
   __device__ __forceinline__ bool whole(const Role& r) const { return r.M == 16 * MT && (r.N & 15) == 0; }   // no part tiles
   __device__ __forceinline__ bool has_col(const Role& r) const { return slice * 16 + c < r.N; }
-  // the state in front of the first token; false: there is none (zeros)
-  template <bool STATE> __device__ __forceinline__ bool first(const LaArgs& p, const Role& r, int bi, f32x4* S) const {
-    const int64_t pair = (int64_t)bi * p.H + h, states = (int64_t)r.M * r.N;
-    const float* s0 = STATE ? nullptr : p.segments > 1 ? r.seg + (pair * p.segments + blockIdx.z) * states : r.s0 ? r.s0 + pair * states : nullptr;
+  // sequence bgroup's states of this wave's head, and how far it is to the next sequence's: in front of the first token (null: zeros), and
+  // behind the last one (null: not wanted)
+  template <bool STATE> __device__ __forceinline__ const float* first_at(const LaArgs& p, const Role& r, int64_t* next) const {
+    const int64_t pair = (int64_t)bgroup * p.H + h, states = (int64_t)r.M * r.N;
+    *next = (int64_t)p.bgroups * p.H * p.segments * states;
+    if (STATE) return nullptr;
+    if (p.segments > 1) return r.seg + (pair * p.segments + blockIdx.z) * states;
+    return r.s0 ? r.s0 + pair * states : nullptr;
+  }
+  template <bool STATE> __device__ __forceinline__ float* last_at(const LaArgs& p, const Role& r, int64_t* next) const {
+    const int64_t pair = (int64_t)bgroup * p.H + h, states = (int64_t)r.M * r.N;
+    *next = (int64_t)p.bgroups * p.H * (STATE ? p.segments : 1) * states;
+    if (STATE) return r.seg + (pair * p.segments + blockIdx.z + 1) * states;
+    return (int)blockIdx.z == p.segments - 1 && r.s1 ? r.s1 + pair * states : nullptr;
+  }
+  __device__ __forceinline__ void load(const Role& r, const float* s0, f32x4* S) const {
 #pragma unroll
     for (int t = 0; t < MT; ++t) S[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-    if (!s0) return false;
+    if (!s0) return;
     const int at = 4 * g * r.sm + (slice * 16 + c) * r.sn;
     if (whole(r)) {
 #pragma unroll
@@ -290,11 +302,8 @@ template <typename T, int MT> struct Wave {
         for (int e = 0; e < 4; ++e)
           if (16 * t + 4 * g + e < r.M) S[t][e] = s0[at + (16 * t + e) * r.sm];
     }
-    return true;
   }
-  template <bool STATE> __device__ __forceinline__ void last(const LaArgs& p, const Role& r, int bi, const f32x4* S) const {
-    const int64_t pair = (int64_t)bi * p.H + h, states = (int64_t)r.M * r.N;
-    float* s1 = STATE ? r.seg + (pair * p.segments + blockIdx.z + 1) * states : (int)blockIdx.z == p.segments - 1 && r.s1 ? r.s1 + pair * states : nullptr;
+  __device__ __forceinline__ void store(const Role& r, float* s1, const f32x4* S) const {
     if (!s1 || !active || !has_col(r)) return;
     const int at = 4 * g * r.sm + (slice * 16 + c) * r.sn;
     if (whole(r)) {
@@ -446,12 +455,15 @@ template <typename T, int MT, int CT, bool STATE> __global__ __launch_bounds__(2
   const Raw unit = X::one(c - 4 * g);
   f32x4* const sums = reinterpret_cast<f32x4*>(lds);
   Weights<CT> k(w.decay, c, g, p.scale, r.za, r.zs, r.sh);
+  int64_t next0, next1;
+  const float* s0 = w.template first_at<STATE>(p, r, &next0);
+  float* s1 = w.template last_at<STATE>(p, r, &next1);
   int turn = 0;
-  for (int bi = w.bgroup; bi < p.B; bi += p.bgroups) {
+  for (int bi = w.bgroup; bi < p.B; bi += p.bgroups, s0 += s0 ? next0 : 0, s1 += s1 ? next1 : 0) {
     const int n = p.lengths ? min(max(p.lengths[bi], 0), p.T) : p.T;
     const char *qa = pa + bi * r.a.sb * kBytes, *qb = pb + bi * r.b.sb * kBytes, *qc = pc + bi * r.c.sb * kBytes;
     f32x4 S[MT];
-    const bool s0 = w.template first<STATE>(p, r, bi, S);
+    w.load(r, s0, S);
     for (int t0 = begin; t0 < end; t0 += C, ++turn) {
       const int cnt = min(C, n - t0);
       f32x4 acc[CT];
@@ -542,7 +554,7 @@ template <typename T, int MT, int CT, bool STATE> __global__ __launch_bounds__(2
         }
       }
     }
-    w.template last<STATE>(p, r, bi, S);
+    w.store(r, s1, S);
   }
 }
 
@@ -595,11 +607,17 @@ template <typename T, int MT, int CT, bool STATE> __global__ __launch_bounds__(2
   const char *ca = nullptr, *cb = nullptr, *cc = nullptr;
   char* co_at = nullptr;
   const int64_t sign = reverse ? -1 : 1, da = sign * G::kRows * ta, db = sign * G::kRows * tb, dc = sign * G::kCRows * tc, d_out = sign * G::kCRows * to;
-  auto place = [&](int bi, int n) {   // at a sequence's first chunk
-    const int64_t tok = reverse ? n - begin - G::kRows : begin, tok_c = reverse ? n - begin - G::kCRows : begin;
-    ca = reinterpret_cast<const char*>(r.a.p) + (bi * r.a.sb + (w.h / r.a.shared) * r.a.sh + tok * r.a.st) * kBytes;
-    cb = reinterpret_cast<const char*>(r.b.p) + (bi * r.b.sb + (w.h / r.b.shared) * r.b.sh + tok * r.b.st) * kBytes;
-    cc = reinterpret_cast<const char*>(r.c.p) + (bi * r.c.sb + (w.h / r.c.shared) * r.c.sh + w.slice * 16 + tok_c * r.c.st) * kBytes;
+  // a sequence's rows, and how far it is to the wave's next one
+  const char *qa = reinterpret_cast<const char*>(r.a.p) + (w.bgroup * r.a.sb + (w.h / r.a.shared) * r.a.sh) * kBytes;
+  const char *qb = reinterpret_cast<const char*>(r.b.p) + (w.bgroup * r.b.sb + (w.h / r.b.shared) * r.b.sh) * kBytes;
+  const char *qc = reinterpret_cast<const char*>(r.c.p) + (w.bgroup * r.c.sb + (w.h / r.c.shared) * r.c.sh + w.slice * 16) * kBytes;
+  char* out = reinterpret_cast<char*>(r.out) + (int64_t)w.bgroup * p.T * to + (w.h / r.fold * N + w.slice * 16) * cols_bytes;
+  const int64_t next_a = step * r.a.sb * kBytes, next_b = step * r.b.sb * kBytes, next_c = step * r.c.sb * kBytes, next_out = (int64_t)step * p.T * to;
+  auto place = [&](int n) {   // at a sequence's first chunk
+    const int tok = reverse ? n - begin - G::kRows : begin, tok_c = reverse ? n - begin - G::kCRows : begin;
+    ca = qa + (int64_t)tok * ta;
+    cb = qb + (int64_t)tok * tb;
+    cc = qc + (int64_t)tok_c * tc;
   };
   u32x4 fa[G::kLoads], fb[G::kLoads], fc[G::kCLoads];
   auto fetch = [&](int cnt) {
@@ -652,18 +670,23 @@ template <typename T, int MT, int CT, bool STATE> __global__ __launch_bounds__(2
   auto length = [&](int bi) { return bi >= B ? 0 : p.lengths ? min(max(p.lengths[bi], 0), p.T) : p.T; };
   int n = length(w.bgroup), n_next = length(w.bgroup + step), turn = 0;
   if (begin < n) {
-    place(w.bgroup, n);
+    place(n);
     fetch(n - begin);
   }
+  int64_t next0, next1;
+  const float* s0 = w.template first_at<STATE>(p, r, &next0);
+  float* s1 = w.template last_at<STATE>(p, r, &next1);
   for (int bi = w.bgroup; bi < B; bi += step, n = n_next, n_next = length(bi + step)) {
     const int stop = min(n, end);
     f32x4 S[MT];
-    const bool s0 = w.template first<STATE>(p, r, bi, S), s1 = STATE || (blockIdx.z == (unsigned)p.segments - 1 && r.s1);
-    char* const out = reinterpret_cast<char*>(r.out) + ((int64_t)bi * p.T * (p.H / r.fold) * N + w.h / r.fold * N + w.slice * 16) * cols_bytes;
+    w.load(r, s0, S);
     co_at = out + (int64_t)(reverse ? n - begin - G::kCRows : begin) * to;
     auto next_sequence = [&]() {
+      qa += next_a;
+      qb += next_b;
+      qc += next_c;
       if (begin < n_next) {
-        place(bi + step, n_next);
+        place(n_next);
         fetch(n_next - begin);
       }
     };
@@ -786,7 +809,10 @@ template <typename T, int MT, int CT, bool STATE> __global__ __launch_bounds__(2
         if (w.slice * wide + at < N * cols_bytes) *reinterpret_cast<u32x4*>(out + (int64_t)tok * to + at) = u32x4{0, 0, 0, 0};
       }
     }
-    w.template last<STATE>(p, r, bi, S);
+    w.store(r, s1, S);
+    out += next_out;
+    if (s0) s0 += next0;
+    if (s1) s1 += next1;
   }
 }
 
