@@ -104,6 +104,11 @@ template <> struct Mat<F32> {
     for (int e = 0; e < 4; ++e) v[e] = e < n ? v[e] : 0.f;
     return v;
   }
+  __device__ __forceinline__ static Op behind(Op v, int n) {   // zeros in place of the first n
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = e < n ? 0.f : v[e];
+    return v;
+  }
 };
 template <> struct Mat<BF16> {
   typedef s16x4 Raw;
@@ -134,6 +139,11 @@ template <> struct Mat<BF16> {
   __device__ __forceinline__ static Op upto(Op v, int n) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) v[e] = e < n ? v[e] : (short)0;
+    return v;
+  }
+  __device__ __forceinline__ static Op behind(Op v, int n) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = e < n ? (short)0 : v[e];
     return v;
   }
 };
@@ -179,6 +189,11 @@ template <> struct Mat<F16> {
   __device__ __forceinline__ static Op upto(Op v, int n) {
     v.hi = Mat<BF16>::upto(v.hi, n);
     v.lo = Mat<BF16>::upto(v.lo, n);
+    return v;
+  }
+  __device__ __forceinline__ static Op behind(Op v, int n) {
+    v.hi = Mat<BF16>::behind(v.hi, n);
+    v.lo = Mat<BF16>::behind(v.lo, n);
     return v;
   }
 };
@@ -1058,6 +1073,262 @@ template <typename T, int MT> __global__ __launch_bounds__(256, 2) void la_short
   }
 }
 
+// The three gradients of such sequences in one pass: a wave brings q, k, v and do once instead of nine rows' worth for three roles, and takes one
+// slice of dq, dk and dv from them, tokens in their own order (23 us as three roles of la_short_kernel, 16.5 so, for 16384 sequences of 10 tokens x 16 channels).  p.r[] are the roles of
+// the general form.
+template <typename T, int MT> __global__ __launch_bounds__(256, 2) void la_short_grad_kernel(LaArgs p) {
+  typedef Mat<T> X;
+  typedef Stage<T, MT, 1> G;
+  typedef typename X::Raw Raw;
+  typedef typename X::Op Op;
+  constexpr int kBytes = ElemTraits<T>::kBytes;
+  constexpr f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+  extern __shared__ __align__(16) char lds[];
+  const Role &rq = p.r[0], &rk = p.r[1], &rv = p.r[2];
+  const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+  const int DK = rv.M, DV = rv.N, slices = (max(DK, DV) + 15) >> 4, per = waves / p.group;
+  const int bgroup = blockIdx.x / p.columns, member = wave % p.group;
+  int f = (blockIdx.x - bgroup * p.columns) * per + wave / p.group;
+  const bool active = f < p.H / p.group * slices;
+  if (!active) f = 0;
+  const int slice = f % slices, h = f / slices * p.group + member, fold = rv.fold, step = p.bgroups, B = p.B;
+  const Decay decay(p.log_decay[h]);
+  constexpr int kRows16 = 16 * G::kRow;
+  char* const area = lds + wave * 4 * kRows16;   // q, k, v, do
+  f32x4* const sums = reinterpret_cast<f32x4*>(lds + waves * 4 * kRows16);
+
+  // operand x of head h of sequence bgroup; its token stride in bytes; the way to the next sequence
+  const Operand* const ops[4] = {&rk.c, &rq.c, &rq.b, &rq.a};
+  const char* at[4];
+  int64_t next[4];
+  int ts[4];
+#pragma unroll
+  for (int x = 0; x < 4; ++x) {
+    at[x] = reinterpret_cast<const char*>(ops[x]->p) + (bgroup * ops[x]->sb + (h / ops[x]->shared) * ops[x]->sh) * kBytes;
+    next[x] = step * ops[x]->sb * kBytes;
+    ts[x] = ops[x]->st * kBytes;
+  }
+  const int piece = lane % G::kLanes * 16, row = lane / G::kLanes;
+  const bool live_k = piece < DK * kBytes && row < 16, live_v = piece < DV * kBytes && row < 16;
+  auto length = [&](int bi) { return bi >= B ? 0 : p.lengths ? min(max(p.lengths[bi], 0), p.T) : p.T; };
+  u32x4 in[4][G::kLoads];
+  auto fetch = [&](int n) {
+#pragma unroll
+    for (int i = 0; i < G::kLoads; ++i) {
+      const int tok = min(i * G::kRows + row, n - 1);
+      if (live_k)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) in[x][i] = *reinterpret_cast<const u32x4*>(at[x] + (unsigned)(tok * ts[x] + piece));
+      if (live_v)
+#pragma unroll
+        for (int x = 2; x < 4; ++x) in[x][i] = *reinterpret_cast<const u32x4*>(at[x] + (unsigned)(tok * ts[x] + piece));
+    }
+  };
+  auto rows = [&](int x, int t) { return *reinterpret_cast<const Raw*>(area + x * kRows16 + c * G::kRow + (16 * t + 4 * g) * kBytes); };
+  auto cols = [&](int x, int t) { return columns<T>(area + x * kRows16, G::kRow, 0, t, c, g); };
+  if (DK != 16 * MT || DV != 16 * MT)   // (channels behind DK and DV)
+    for (int i = lane * 16; i < 4 * kRows16; i += 1024) *reinterpret_cast<u32x4*>(area + i) = u32x4{0, 0, 0, 0};
+
+  // scale g^{i-j}: [j][i] for dq, [i][j] for dk and dv;  scale g^{i+1} by lane and by element;  g^{n-1-j} by lane, and g^n - 1
+  f32x4 below, above, into;
+  const float g1 = decay.pow(1), from = p.scale * decay.pow(c + 1);
+  float back = 0.f, keep = 0.f;
+  int known = -1;
+  {
+    const int d = c - 4 * g;
+    below[3] = p.scale * decay.pow(max(d - 3, 0));
+    above[0] = p.scale * decay.pow(max(-d, 0));
+    into[0] = p.scale * decay.pow(4 * g + 1);
+#pragma unroll
+    for (int e = 2; e >= 0; --e) below[e] = d - e > 0 ? below[e + 1] * g1 : p.scale;
+#pragma unroll
+    for (int e = 1; e < 4; ++e) {
+      above[e] = e - d > 0 ? above[e - 1] * g1 : p.scale;
+      into[e] = into[e - 1] * g1;
+    }
+  }
+  // states: S of M x N read through the strides, this wave's 16 columns of it
+  auto state = [&](const float* s, int M, int N, int sm, int sn, f32x4* S) {
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int m = 16 * t + 4 * g + e, n = slice * 16 + c;
+        S[t][e] = 0.f;
+        if (m < M && n < N) S[t][e] = s[m * sm + n * sn];
+      }
+  };
+  const int64_t states = (int64_t)DK * DV, first = ((int64_t)bgroup * p.H + h) * states, next_states = (int64_t)step * p.H * states;
+  const float *s0 = rq.s0 ? rq.s0 + first : nullptr, *d1 = rv.s0 ? rv.s0 + first : nullptr;
+  float* d0 = rv.s1 ? rv.s1 + first : nullptr;
+  const int tq = p.H * DK * kBytes, tk = p.H / fold * DK * kBytes, tv = p.H / fold * DV * kBytes;   // bytes of a token of dq, dk, dv
+  char* oq = reinterpret_cast<char*>(rq.out) + (int64_t)bgroup * p.T * tq + (h * DK + slice * 16) * kBytes;
+  char* ok = reinterpret_cast<char*>(rk.out) + (int64_t)bgroup * p.T * tk + (h / fold * DK + slice * 16) * kBytes;
+  char* ov = reinterpret_cast<char*>(rv.out) + (int64_t)bgroup * p.T * tv + (h / fold * DV + slice * 16) * kBytes;
+  const int piece_c = lane % kBytes * 16, row_c = lane / kBytes;
+  const bool out_k = row_c < p.T && slice * 16 * kBytes + piece_c < DK * kBytes && row_c < 16, out_v = row_c < p.T && slice * 16 * kBytes + piece_c < DV * kBytes && row_c < 16;
+
+  // acc[n][.] += sum over tokens of c[token][n] scores[token][.]; a masked token's infinity or NaN must not come through as 0 * inf.  later:
+  // the tokens behind the lane's own count (dk, dv), not those in front of it (dq)
+  auto sum = [&](Raw craw, f32x4 x, f32x4 acc, bool later) {
+    const Op co = X::op(craw);
+    const f32x4 cf = X::to_float(craw);
+    const typename X::Split ps = X::split(x);
+    float top = 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) top = __builtin_elementwise_maximum(top, __builtin_fabsf(cf[e]));
+    if (__builtin_expect(__any(!(top <= 3.4028234e38f)), 0)) {
+      const f32x4 before = acc;
+#pragma unroll 1
+      for (int i = 0; i < 16; ++i) {
+        const f32x4 y = X::score(later ? X::behind(co, i - 4 * g) : X::upto(co, i + 1 - 4 * g), ps, before);
+        if (c == i) acc = y;
+      }
+      return acc;
+    }
+    return X::score(co, ps, acc);
+  };
+
+  int n = length(bgroup), n_next = length(bgroup + step), turn = 0;
+  if (n > 0) fetch(n);
+  for (int bi = bgroup; bi < B; bi += step, n = n_next, n_next = length(bi + step), ++turn) {
+    if (n > 0) {
+      wave_fence();
+#pragma unroll
+      for (int i = 0; i < G::kLoads; ++i) {
+        char* const o = area + (i * G::kRows + row) * G::kRow + piece;
+        if (live_k) {
+          *reinterpret_cast<u32x4*>(o) = in[0][i];
+          *reinterpret_cast<u32x4*>(o + kRows16) = in[1][i];
+        }
+        if (live_v) {
+          *reinterpret_cast<u32x4*>(o + 2 * kRows16) = in[2][i];
+          *reinterpret_cast<u32x4*>(o + 3 * kRows16) = in[3][i];
+        }
+      }
+      wave_fence();
+    }
+#pragma unroll
+    for (int x = 0; x < 4; ++x) at[x] += next[x];
+    if (n_next > 0) fetch(n_next);
+    f32x4 dq = zero, dk = zero, dv = zero;
+    if (n != known) {
+      known = n;
+      back = decay.pow(max(n - 1 - c, 0));
+      keep = expm1f(decay.la * (float)n);
+    }
+    f32x4 S[MT];
+    if (n > 0) {
+      f32x4 x1 = zero, x2 = zero, x3 = zero;
+      if constexpr (MT == 1) {
+        const Raw q = rows(0, 0), k = rows(1, 0), v = rows(2, 0), d = rows(3, 0);
+        x1 = X::raw(v, d, x1);
+        x2 = X::raw(d, v, x2);
+        x3 = X::raw(q, k, x3);
+      } else {
+#pragma unroll
+        for (int t = 0; t < MT; t += 2) {
+          const Raw q0 = rows(0, t), q1 = rows(0, t + 1), k0 = rows(1, t), k1 = rows(1, t + 1), v0 = rows(2, t), v1 = rows(2, t + 1), e0 = rows(3, t), e1 = rows(3, t + 1);
+          x1 = X::raw2(v0, v1, e0, e1, x1);
+          x2 = X::raw2(e0, e1, v0, v1, x2);
+          x3 = X::raw2(q0, q1, k0, k1, x3);
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int i = 4 * g + e;
+        x1[e] = i <= c ? x1[e] * below[e] : 0.f;
+        x2[e] = i >= c && i < n ? x2[e] * above[e] : 0.f;
+        x3[e] = i >= c && i < n ? x3[e] * above[e] : 0.f;
+      }
+      auto inter = [&](int x, f32x4 acc) {   // sum_m S[m][n] rows_x[m]
+        if constexpr (MT == 1) return X::state(X::split(S[0]), X::op(rows(x, 0)), acc);
+        else {
+#pragma unroll
+          for (int t = 0; t < MT; t += 2) acc = X::state2(X::split(S[t]), X::split(S[t + 1]), X::op(rows(x, t)), X::op(rows(x, t + 1)), acc);
+          return acc;
+        }
+      };
+      if (s0) {
+        state(s0, DV, DK, 1, DV, S);
+        dq = inter(3, dq) * from;
+      }
+      if (d1) {
+        state(d1, DV, DK, 1, DV, S);
+        dk = inter(2, dk) * back;
+        state(d1, DK, DV, DV, 1, S);
+        dv = inter(1, dv) * back;
+      }
+      dq = sum(cols(1, slice), x1, dq, false);
+      dk = sum(cols(0, slice), x2, dk, true);
+      dv = sum(cols(3, slice), x3, dv, true);
+    } else if (d1) {
+      state(d1, DK, DV, DV, 1, S);
+    }
+    if (d0) {   // g^n dS + sum_i q_i (scale g^{i+1} do_i^T)
+      if (!d1)
+#pragma unroll
+        for (int t = 0; t < MT; ++t) S[t] = zero;
+      if (n > 0) {
+        f32x4 w = X::to_float(cols(3, slice));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = 4 * g + e < n ? w[e] * into[e] : 0.f;
+        const typename X::Split3 ws = X::split3(w);
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) S[t][e] = fmaf(S[t][e], keep, S[t][e]);
+          S[t] = X::add(X::op(cols(0, t)), ws, S[t]);
+        }
+      }
+      if (active && slice * 16 + c < DV)
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (16 * t + 4 * g + e < DK) d0[(16 * t + 4 * g + e) * DV + slice * 16 + c] = S[t][e];
+    }
+    bool writes = active;
+    if (fold > 1) {   // (see Wave::fold)
+      f32x4* const buf = sums + (turn & 1) * waves * 128;
+      buf[wave * 128 + lane] = dk;
+      buf[wave * 128 + 64 + lane] = dv;
+      __syncthreads();
+      writes = active && member == 0;
+      if (writes)
+        for (int k = 1; k < fold; ++k) {
+          dk += buf[(wave + k) * 128 + lane];
+          dv += buf[(wave + k) * 128 + 64 + lane];
+        }
+    }
+    if (c >= n) dq = dk = dv = zero;
+    wave_fence();
+    auto put = [&](int x, f32x4 v) {
+      char* const o = area + x * kRows16 + c * G::kCRow + 4 * g * kBytes;
+      if constexpr (kBytes == 4) *reinterpret_cast<f32x4*>(o) = v;
+      else *reinterpret_cast<s16x4*>(o) = X::to_out(v);
+    };
+    put(0, dq);
+    put(1, dk);
+    put(2, dv);
+    wave_fence();
+    auto get = [&](int x) { return *reinterpret_cast<const u32x4*>(area + x * kRows16 + row_c * G::kCRow + piece_c); };
+    if (out_k && active) *reinterpret_cast<u32x4*>(oq + (unsigned)(row_c * tq + piece_c)) = get(0);
+    if (out_k && writes) *reinterpret_cast<u32x4*>(ok + (unsigned)(row_c * tk + piece_c)) = get(1);
+    if (out_v && writes) *reinterpret_cast<u32x4*>(ov + (unsigned)(row_c * tv + piece_c)) = get(2);
+    if (DK != 16 * MT || DV != 16 * MT) {   // (the channels behind DK and DV held parts of these rows)
+      wave_fence();
+      for (int i = lane * 16; i < 3 * kRows16; i += 1024) *reinterpret_cast<u32x4*>(area + i) = u32x4{0, 0, 0, 0};
+    }
+    oq += (int64_t)step * p.T * tq;
+    ok += (int64_t)step * p.T * tk;
+    ov += (int64_t)step * p.T * tv;
+    if (s0) s0 += next_states;
+    if (d1) d1 += next_states;
+    if (d0) d0 += next_states;
+  }
+}
+
 // the state in front of every segment, from each segment's own (written one place further on) and the first state: in place.  A workgroup
 // takes 64 elements of one state; 16 groups of threads take consecutive segments each and meet through LDS
 constexpr int kMaxSegments = 256;
@@ -1316,6 +1587,13 @@ template <typename T, int MT, int CT, bool STATE> int go_plain(const LaArgs& a, 
   return go(la_plain_kernel<T, MT, CT, STATE>, resident, 0, CT, !STATE && a.group > 1, a, grid, threads, st);
 }
 template <typename T, int MT> int go_short(const LaArgs& a, dim3 grid, int threads, hipStream_t st) {
+  if constexpr (MT < 8) {   // (128 channels: three roles, their registers do not fit one wave)
+    if (grid.y == 3 && !a.r[1].out_f32) {   // the three gradients
+      static Resident resident;
+      grid.y = 1;
+      return go(la_short_grad_kernel<T, MT>, resident, 4 * 16 * Stage<T, MT, 1>::kRow, 2, a.group > 1, a, grid, threads, st);
+    }
+  }
   static Resident resident;
   return go(la_short_kernel<T, MT>, resident, Stage<T, MT, 1>::kArea, 1, a.group > 1, a, grid, threads, st);
 }

@@ -467,6 +467,30 @@ def test_attention_nonfinite_tokens_reach_no_earlier_one(which, value, dt):
             assert torch.equal(p[:, at + 1:], o[:, at + 1:])
 
 
+@pytest.mark.parametrize("dt", [F32, BF16, F16])
+@pytest.mark.parametrize("value", [math.inf, math.nan])
+@pytest.mark.parametrize("which", ["q", "k", "v", "do"])
+def test_attention_nonfinite_tokens_in_the_gradients(which, value, dt):
+    """dq_i takes from do_i and from k, v up to i; dk_j from v_j and from q, do at j and behind it; dv_j from k_j and from q, do there"""
+    for T, at, D in ((10, 6, 16), (16, 3, 20), (40, 21, 17), (150, 77, 64)):
+        q, k, v, do, state, dstate, decay = attention_inputs(1, T, 2, 2, D, D, dt, seed=3)
+        decay = torch.tensor([-0.05, -0.2], device=DEV)
+        good = ops.linear_attention_backward(do, q, k, v, decay, state=state, dstate=dstate)
+        bad = dict(q=q, k=k, v=v, do=do)
+        bad[which] = bad[which].clone()
+        bad[which][0, at, 1, 5] = value
+        got = ops.linear_attention_backward(bad["do"], bad["q"], bad["k"], bad["v"], decay, state=state, dstate=dstate)
+        clean = {"q": (range(T), range(at + 1, T), range(at + 1, T)), "do": ([i for i in range(T) if i != at], range(at + 1, T), range(at + 1, T)),
+                 "k": (range(at), range(T), [j for j in range(T) if j != at]), "v": (range(at), [j for j in range(T) if j != at], range(T))}[which]
+        for name, a, b, rows in zip(("dq", "dk", "dv"), got, good, clean):
+            rows = list(rows)
+            assert torch.equal(a[:, rows], b[:, rows]), (which, name, T)
+            assert torch.equal(a[:, :, 0], b[:, :, 0]), (which, name, T)
+        touched = {"q": (1, 2), "do": (0, 1, 2), "k": (0, 2), "v": (0, 1)}[which]
+        for i in touched:
+            assert not bool(torch.isfinite(got[i][0, at, 1]).all())
+
+
 def test_attention_does_not_read_behind_the_lengths():
     for dt in (F32, BF16, F16):
         q, k, v, do, state, dstate, decay = attention_inputs(3, 90, 2, 2, 32, 32, dt, seed=4)
