@@ -601,10 +601,10 @@ typedef struct {
   int64_t q_stride[3], k_stride[3], v_stride[3];   /* sequence, token, head */
   float scale;
 } tg_la_desc;
-int64_t tg_linear_attention_scratch_floats(const tg_la_desc* d);
+int64_t tg_linear_attention_scratch_floats(int dtype, const tg_la_desc* d);
 int tg_linear_attention(int dtype, const tg_la_desc* d, const void* q, const void* k, const void* v, const float* log_decay,
                         const int32_t* lengths, const float* state_in, void* o, float* state_out, float* scratch, void* stream);
-int64_t tg_linear_attention_bwd_scratch_floats(const tg_la_desc* d);
+int64_t tg_linear_attention_bwd_scratch_floats(int dtype, const tg_la_desc* d);
 int tg_linear_attention_bwd(int dtype, const tg_la_desc* d, const void* q, const void* k, const void* v, const void* dout,
                             const int64_t* dout_stride, const float* log_decay, const int32_t* lengths, const float* state_in,
                             const float* dstate_out, void* dq, void* dk, void* dv, float* dstate_in, float* scratch, void* stream);

@@ -124,9 +124,9 @@ _PROTOS = {
     "tg_rms_norm_bwd_scratch_floats": (_L, [_L, _I]),
     "tg_rms_norm_bwd": (_I, [_I, _P, _L, _P, _L, _P, _L, _P, _P, _P, _L, _P, _P, _P, _L, _I, _P]),
     "tg_dropout": (_I, [_I, _P, _P, _P, _L, _D, _P, _I, _P]),
-    "tg_linear_attention_scratch_floats": (_L, [_P]),
+    "tg_linear_attention_scratch_floats": (_L, [_I, _P]),
     "tg_linear_attention": (_I, [_I, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P]),
-    "tg_linear_attention_bwd_scratch_floats": (_L, [_P]),
+    "tg_linear_attention_bwd_scratch_floats": (_L, [_I, _P]),
     "tg_linear_attention_bwd": (_I, [_I, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P]),
     "tg_linear_attention_step": (_I, [_I, _P, _P, _P, _P, _P, _P, _P, _P]),
     "tg_stream_create_cumask": (_I, [_I, C.POINTER(C.c_void_p)]),

@@ -15,7 +15,7 @@
 // so ONE kernel serves all four: out_i = za g^{i+1-sh} a_i S + scale sum_{j<=i} g^{i-j} (a_i . b_j) c_j,
 // S' = g^n S + zs sum_j g^{n-1-j+sh} b_j c_j^T over tokens taken forwards (sh = 0, za = scale, zs = 1) or backwards (sh = 1, za = 1, zs = scale).
 //
-// Layout: a wave owns 16 columns of c (and of S and out) of one head and walks the tokens in chunks of 16 CT.  Everything is
+// Layout: a wave owns 16 columns of c (and of S and out) of one head, or twice as many, and walks the tokens in chunks of 16 CT.  Everything is
 // made of 16 x 16 tiles in the matrix instructions' own shape: lane (c = lane % 16, g = lane / 16) holds 4 consecutive values 4g .. 4g+3
 // of row / column c.  An accumulator tile X[k][c] has the shape of an operand with c along its free dimension and k along the summed one,
 // so the scores (b a^T, tile [j][i]) and the state (tiles [m][n]) go from accumulators to operands without leaving the registers.
@@ -264,16 +264,16 @@ __device__ __forceinline__ void wave_fence() {   // the wave's own LDS writes an
   __builtin_amdgcn_wave_barrier();
 }
 
-// What a wave works on: 16 columns (a slice) of one head, and the sequences bgroup, bgroup + bgroups, .. of it.  A wave without work does another's
+// What a wave works on: NS x 16 columns (a slice) of one head, and the sequences bgroup, bgroup + bgroups, .. of it.  A wave without work does another's
 // and writes nothing (it meets the barriers of the summed roles).
-template <typename T, int MT> struct Wave {
+template <typename T, int MT, int NS = 1> struct Wave {
   int lane, c, g, wave, waves, member, bgroup, slice, h;
   bool active;
   Decay decay;
   __device__ __forceinline__ explicit Wave(const LaArgs& p) : decay(0.f) {
     const Role& r = p.r[blockIdx.y];
     lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
-    const int slices = (r.N + 15) >> 4, per = waves / p.group;       // (stored head, slice) pairs of a workgroup
+    const int slices = (r.N + 16 * NS - 1) / (16 * NS), per = waves / p.group;   // (stored head, slice) pairs of a workgroup
     bgroup = blockIdx.x / p.columns;
     int f = (blockIdx.x - bgroup * p.columns) * per + wave / p.group;
     member = wave % p.group;
@@ -283,8 +283,8 @@ template <typename T, int MT> struct Wave {
     h = f / slices * p.group + member;
     decay = Decay(p.log_decay[h]);
   }
-  __device__ __forceinline__ bool whole(const Role& r) const { return r.M == 16 * MT && (r.N & 15) == 0; }   // no part tiles
-  __device__ __forceinline__ bool has_col(const Role& r) const { return slice * 16 + c < r.N; }
+  __device__ __forceinline__ bool whole(const Role& r) const { return r.M == 16 * MT && r.N % (16 * NS) == 0; }   // no part tiles
+  __device__ __forceinline__ int col(int s) const { return (slice * NS + s) * 16 + c; }
   // sequence bgroup's states of this wave's head, and how far it is to the next sequence's: in front of the first token (null: zeros), and
   // behind the last one (null: not wanted)
   template <bool STATE> __device__ __forceinline__ const float* first_at(const LaArgs& p, const Role& r, int64_t* next) const {
@@ -300,52 +300,62 @@ template <typename T, int MT> struct Wave {
     if (STATE) return r.seg + (pair * p.segments + blockIdx.z + 1) * states;
     return (int)blockIdx.z == p.segments - 1 && r.s1 ? r.s1 + pair * states : nullptr;
   }
-  __device__ __forceinline__ void load(const Role& r, const float* s0, f32x4* S) const {
+  __device__ __forceinline__ void load(const Role& r, const float* s0, f32x4 (&S)[NS][MT]) const {
 #pragma unroll
-    for (int t = 0; t < MT; ++t) S[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-    if (!s0) return;
-    const int at = 4 * g * r.sm + (slice * 16 + c) * r.sn;
-    if (whole(r)) {
+    for (int s = 0; s < NS; ++s) {
 #pragma unroll
-      for (int t = 0; t < MT; ++t)
+      for (int t = 0; t < MT; ++t) S[s][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (!s0) continue;
+      const int at = 4 * g * r.sm + col(s) * r.sn;
+      if (whole(r)) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) S[t][e] = s0[at + (16 * t + e) * r.sm];
-    } else if (has_col(r)) {
+        for (int t = 0; t < MT; ++t)
 #pragma unroll
-      for (int t = 0; t < MT; ++t)
+          for (int e = 0; e < 4; ++e) S[s][t][e] = s0[at + (16 * t + e) * r.sm];
+      } else if (col(s) < r.N) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (16 * t + 4 * g + e < r.M) S[t][e] = s0[at + (16 * t + e) * r.sm];
+        for (int t = 0; t < MT; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (16 * t + 4 * g + e < r.M) S[s][t][e] = s0[at + (16 * t + e) * r.sm];
+      }
     }
   }
-  __device__ __forceinline__ void store(const Role& r, float* s1, const f32x4* S) const {
-    if (!s1 || !active || !has_col(r)) return;
-    const int at = 4 * g * r.sm + (slice * 16 + c) * r.sn;
-    if (whole(r)) {
+  __device__ __forceinline__ void store(const Role& r, float* s1, const f32x4 (&S)[NS][MT]) const {
+    if (!s1 || !active) return;
 #pragma unroll
-      for (int t = 0; t < MT; ++t)
+    for (int s = 0; s < NS; ++s) {
+      const int at = 4 * g * r.sm + col(s) * r.sn;
+      if (whole(r)) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s1[at + (16 * t + e) * r.sm] = S[t][e];
-    } else {
+        for (int t = 0; t < MT; ++t)
 #pragma unroll
-      for (int t = 0; t < MT; ++t)
+          for (int e = 0; e < 4; ++e) s1[at + (16 * t + e) * r.sm] = S[s][t][e];
+      } else if (col(s) < r.N) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (16 * t + 4 * g + e < r.M) s1[at + (16 * t + e) * r.sm] = S[t][e];
+        for (int t = 0; t < MT; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (16 * t + 4 * g + e < r.M) s1[at + (16 * t + e) * r.sm] = S[s][t][e];
+      }
     }
   }
   // the heads of one stored head add up, in order, in the first one's wave; whether this wave writes.  (Uniform over the launch's role.  Two
   // buffers: who writes one again has passed the next barrier, and so have its readers.)
-  template <int CT> __device__ __forceinline__ bool fold(f32x4* acc, f32x4* sums, int heads, int turn) const {
+  template <int CT> __device__ __forceinline__ bool fold(f32x4 (&acc)[NS][CT], f32x4* sums, int heads, int turn) const {
     if (heads == 1) return active;
-    f32x4* const buf = sums + (turn & 1) * waves * CT * 64;
+    f32x4* const buf = sums + (turn & 1) * waves * NS * CT * 64;
 #pragma unroll
-    for (int t = 0; t < CT; ++t) buf[(wave * CT + t) * 64 + lane] = acc[t];
+    for (int s = 0; s < NS; ++s)
+#pragma unroll
+      for (int t = 0; t < CT; ++t) buf[((wave * NS + s) * CT + t) * 64 + lane] = acc[s][t];
     __syncthreads();
     if (!writer(heads)) return false;
     for (int k = 1; k < heads; ++k)
 #pragma unroll
-      for (int t = 0; t < CT; ++t) acc[t] += buf[((wave + k) * CT + t) * 64 + lane];
+      for (int s = 0; s < NS; ++s)
+#pragma unroll
+        for (int t = 0; t < CT; ++t) acc[s][t] += buf[(((wave + k) * NS + s) * CT + t) * 64 + lane];
     return true;
   }
   __device__ __forceinline__ bool writer(int heads) const { return active && (heads == 1 || member == 0); }
@@ -477,11 +487,11 @@ template <typename T, int MT, int CT, bool STATE> __global__ __launch_bounds__(2
   for (int bi = w.bgroup; bi < p.B; bi += p.bgroups, s0 += s0 ? next0 : 0, s1 += s1 ? next1 : 0) {
     const int n = p.lengths ? min(max(p.lengths[bi], 0), p.T) : p.T;
     const char *qa = pa + bi * r.a.sb * kBytes, *qb = pb + bi * r.b.sb * kBytes, *qc = pc + bi * r.c.sb * kBytes;
-    f32x4 S[MT];
-    w.load(r, s0, S);
+    f32x4 Ss[1][MT], (&S)[MT] = Ss[0];
+    w.load(r, s0, Ss);
     for (int t0 = begin; t0 < end; t0 += C, ++turn) {
       const int cnt = min(C, n - t0);
-      f32x4 acc[CT];
+      f32x4 accs[1][CT], (&acc)[CT] = accs[0];
 #pragma unroll
       for (int t = 0; t < CT; ++t) acc[t] = zero;
       if (cnt > 0) {
@@ -543,7 +553,7 @@ template <typename T, int MT, int CT, bool STATE> __global__ __launch_bounds__(2
         }
       }
       if constexpr (!STATE) {
-        const bool writes = w.template fold<CT>(acc, sums, r.fold, turn);
+        const bool writes = w.template fold<CT>(accs, sums, r.fold, turn);
         // (tokens behind the sequence's length get zeros)
         char* const base = reinterpret_cast<char*>(r.out) + ((int64_t)bi * p.T * row_out + w.h / r.fold * r.N + n0) * out_bytes;
 #pragma unroll
@@ -569,7 +579,7 @@ template <typename T, int MT, int CT, bool STATE> __global__ __launch_bounds__(2
         }
       }
     }
-    w.store(r, s1, S);
+    w.store(r, s1, Ss);
   }
 }
 
@@ -578,29 +588,29 @@ template <typename T, int MT, int CT, bool STATE> __global__ __launch_bounds__(2
 // 16 rows at a time, 8 bytes per lane - cost one L1 access per LANE: 54 per load instruction, and the L1s became the bound: 370 us
 // instead of 311 for 65536 sequences of 120 tokens, the more waves the worse.)  The next chunk's rows are on their way, in registers,
 // while this one is worked on.
-template <typename T, int MT, int CT> struct Stage {
+template <typename T, int MT, int CT, int NS = 1> struct Stage {
   static constexpr int kBytes = ElemTraits<T>::kBytes;
   static constexpr int C = 16 * CT;
   static constexpr int kLanes = kBytes * MT;                      // lanes (16-byte pieces) of a row of a or b
   static constexpr int kRow = 16 * kLanes + 16;                   // bytes between rows: 16 rows x 16 bytes hit every bank once
-  static constexpr int kCRow = 16 * kBytes + 16;                  // the same for c: 16 columns
-  static constexpr int kLoads = (C * kLanes + 63) / 64, kCLoads = (C * kBytes + 63) / 64;
-  static constexpr int kRows = C < 64 / kLanes ? C : 64 / kLanes, kCRows = C < 64 / kBytes ? C : 64 / kBytes;   // rows of one load
+  static constexpr int kCLanes = kBytes * NS, kCRow = 16 * kCLanes + 16;   // the same for c: NS x 16 columns
+  static constexpr int kLoads = (C * kLanes + 63) / 64, kCLoads = (C * kCLanes + 63) / 64;
+  static constexpr int kRows = C < 64 / kLanes ? C : 64 / kLanes, kCRows = C < 64 / kCLanes ? C : 64 / kCLanes;   // rows of one load
   static constexpr int kArea = C * (2 * kRow + kCRow);            // LDS of a wave
 };
 
 // The staged form.  Addresses are a uniform pointer to the chunk's lowest token, which moves on by a constant, and every lane's own offset:
 // the loop holds no multiplication and no scalar load (with both, 187 scalar instructions and 7 loads stood beside 325 vector ones a chunk).
-template <typename T, int MT, int CT, bool STATE> __global__ __launch_bounds__(256, 2) void la_kernel(LaArgs p) {
+template <typename T, int MT, int CT, int NS, bool STATE> __global__ __launch_bounds__(256, 2) void la_kernel(LaArgs p) {
   typedef Mat<T> X;
-  typedef Stage<T, MT, CT> G;
+  typedef Stage<T, MT, CT, NS> G;
   typedef typename X::Raw Raw;
   typedef typename X::Op Op;
   constexpr int kBytes = ElemTraits<T>::kBytes;
   constexpr int C = 16 * CT;
   constexpr f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-  extern __shared__ __align__(16) char lds[];           // [waves][kArea], then [2][waves][CT][64] sums of 4 floats if a role folds
-  const Wave<T, MT> w(p);
+  extern __shared__ __align__(16) char lds[];           // [waves][kArea], then [2][waves][NS][CT][64] sums of 4 floats if a role folds
+  const Wave<T, MT, NS> w(p);
   const Role& r = p.r[blockIdx.y];
   const int lane = w.lane, c = w.c, g = w.g, reverse = r.reverse, N = r.N, B = p.B, step = p.bgroups;
   const int begin = blockIdx.z * p.seg, end = min(begin + p.seg, p.T);
@@ -613,8 +623,8 @@ template <typename T, int MT, int CT, bool STATE> __global__ __launch_bounds__(2
   Weights<CT> k(w.decay, c, g, p.scale, r.za, r.zs, r.sh);
 
   // this lane's piece of a row, its row of a load, and its place in one of a whole chunk's loads
-  const int piece = lane % G::kLanes * 16, piece_c = lane % kBytes * 16, row_a = lane / G::kLanes, row_c = lane / kBytes;
-  const bool live_a = piece < r.M * kBytes && row_a < C, live_c = w.slice * 16 * kBytes + piece_c < N * kBytes && row_c < C;
+  const int piece = lane % G::kLanes * 16, piece_c = lane % G::kCLanes * 16, row_a = lane / G::kLanes, row_c = lane / G::kCLanes;
+  const bool live_a = piece < r.M * kBytes && row_a < C, live_c = w.slice * 16 * G::kCLanes + piece_c < N * kBytes && row_c < C;
   const int up_a = reverse ? G::kRows - 1 - row_a : row_a, up_c = reverse ? G::kCRows - 1 - row_c : row_c;
   const unsigned va = (unsigned)(up_a * ta + piece), vb = (unsigned)(up_a * tb + piece), vc = (unsigned)(up_c * tc + piece_c), vo = (unsigned)(up_c * to + piece_c);
   // uniform: the lowest token of the next load of a, b, c, and of the next store of out; from load to load; back from a chunk's first load to its
@@ -625,8 +635,8 @@ template <typename T, int MT, int CT, bool STATE> __global__ __launch_bounds__(2
   // a sequence's rows, and how far it is to the wave's next one
   const char *qa = reinterpret_cast<const char*>(r.a.p) + (w.bgroup * r.a.sb + (w.h / r.a.shared) * r.a.sh) * kBytes;
   const char *qb = reinterpret_cast<const char*>(r.b.p) + (w.bgroup * r.b.sb + (w.h / r.b.shared) * r.b.sh) * kBytes;
-  const char *qc = reinterpret_cast<const char*>(r.c.p) + (w.bgroup * r.c.sb + (w.h / r.c.shared) * r.c.sh + w.slice * 16) * kBytes;
-  char* out = reinterpret_cast<char*>(r.out) + (int64_t)w.bgroup * p.T * to + (w.h / r.fold * N + w.slice * 16) * cols_bytes;
+  const char *qc = reinterpret_cast<const char*>(r.c.p) + (w.bgroup * r.c.sb + (w.h / r.c.shared) * r.c.sh + w.slice * 16 * NS) * kBytes;
+  char* out = reinterpret_cast<char*>(r.out) + (int64_t)w.bgroup * p.T * to + (w.h / r.fold * N + w.slice * 16 * NS) * cols_bytes;
   const int64_t next_a = step * r.a.sb * kBytes, next_b = step * r.b.sb * kBytes, next_c = step * r.c.sb * kBytes, next_out = (int64_t)step * p.T * to;
   auto place = [&](int n) {   // at a sequence's first chunk
     const int tok = reverse ? n - begin - G::kRows : begin, tok_c = reverse ? n - begin - G::kCRows : begin;
@@ -693,7 +703,7 @@ template <typename T, int MT, int CT, bool STATE> __global__ __launch_bounds__(2
   float* s1 = w.template last_at<STATE>(p, r, &next1);
   for (int bi = w.bgroup; bi < B; bi += step, n = n_next, n_next = length(bi + step)) {
     const int stop = min(n, end);
-    f32x4 S[MT];
+    f32x4 S[NS][MT];
     w.load(r, s0, S);
     co_at = out + (int64_t)(reverse ? n - begin - G::kCRows : begin) * to;
     auto next_sequence = [&]() {
@@ -711,13 +721,15 @@ template <typename T, int MT, int CT, bool STATE> __global__ __launch_bounds__(2
       stage();
       if (t0 + C < stop) fetch(stop - t0 - C);
       else next_sequence();
-      f32x4 acc[CT], cf[CT];
-      Raw craw[CT];
+      f32x4 acc[NS][CT];
+      Raw craw[NS][CT];
 #pragma unroll
-      for (int t = 0; t < CT; ++t) {
-        craw[t] = columns<T>(area_c, G::kCRow, 16 * t, 0, c, g);
-        acc[t] = zero;
-      }
+      for (int s = 0; s < NS; ++s)
+#pragma unroll
+        for (int t = 0; t < CT; ++t) {
+          craw[s][t] = columns<T>(area_c, G::kCRow, 16 * t, s, c, g);
+          acc[s][t] = zero;
+        }
       if constexpr (!STATE) {
         // scores x[jt][it][j][i] = b_j . a_i
         f32x4 x[CT][CT];
@@ -748,45 +760,63 @@ template <typename T, int MT, int CT, bool STATE> __global__ __launch_bounds__(2
         }
         if (s0 || t0 > begin) {   // acc[it][n][i] = za g^{i+1-sh} sum_m S[m][n] a_i[m]; nothing is read from a state of zeros
           if constexpr (MT == 1) {
-            const typename X::Split s = X::split(S[0]);
 #pragma unroll
-            for (int it = 0; it < CT; ++it) acc[it] = X::state(s, X::op(A(it, 0)), zero);
+            for (int s = 0; s < NS; ++s)
+#pragma unroll
+              for (int it = 0; it < CT; ++it) acc[s][it] = X::state(X::split(S[s][0]), X::op(A(it, 0)), zero);
           } else {
 #pragma unroll
             for (int t = 0; t < MT; t += 2) {
-              const typename X::Split s = X::split(S[t]), u = X::split(S[t + 1]);
+              Op a0[CT], a1[CT];
 #pragma unroll
-              for (int it = 0; it < CT; ++it) acc[it] = X::state2(s, u, X::op(A(it, t)), X::op(A(it, t + 1)), acc[it]);
+              for (int it = 0; it < CT; ++it) {
+                a0[it] = X::op(A(it, t));
+                a1[it] = X::op(A(it, t + 1));
+              }
+#pragma unroll
+              for (int s = 0; s < NS; ++s) {
+                const typename X::Split u = X::split(S[s][t]), v = X::split(S[s][t + 1]);
+#pragma unroll
+                for (int it = 0; it < CT; ++it) acc[s][it] = X::state2(u, v, a0[it], a1[it], acc[s][it]);
+              }
             }
           }
 #pragma unroll
-          for (int t = 0; t < CT; ++t) acc[t] *= k.from[t];
+          for (int s = 0; s < NS; ++s)
+#pragma unroll
+            for (int t = 0; t < CT; ++t) acc[s][t] *= k.from[t];
         }
         typename X::Split ps[CT][CT];
-        Op co[CT];
 #pragma unroll
-        for (int it = 0; it < CT; ++it) {
+        for (int it = 0; it < CT; ++it)
 #pragma unroll
           for (int jt = 0; jt <= it; ++jt) ps[jt][it] = X::split(k.masked(x[jt][it], it, jt, c, g));
-          cf[it] = X::to_float(craw[it]);
-          co[it] = X::op(craw[it]);
-        }
-        weighted_sum<T, CT>(acc, ps, co, cf, c, g);
-      } else {
 #pragma unroll
-        for (int t = 0; t < CT; ++t) cf[t] = X::to_float(craw[t]);
+        for (int s = 0; s < NS; ++s) {
+          Op co[CT];
+          f32x4 cf[CT];
+#pragma unroll
+          for (int t = 0; t < CT; ++t) {
+            cf[t] = X::to_float(craw[s][t]);
+            co[t] = X::op(craw[s][t]);
+          }
+          weighted_sum<T, CT>(acc[s], ps, co, cf, c, g);
+        }
       }
       if (s1 || t0 + C < stop) {   // (nothing is added to a state that nobody reads)
         k.length(w.decay, cnt, g, r.zs, r.sh);
-        typename X::Split3 ws[CT];
+        typename X::Split3 ws[NS][CT];
 #pragma unroll
-        for (int t = 0; t < CT; ++t) ws[t] = X::split3(cf[t] * k.into(cnt, t));
+        for (int s = 0; s < NS; ++s)
+#pragma unroll
+          for (int t = 0; t < CT; ++t) ws[s][t] = X::split3(X::to_float(craw[s][t]) * k.into(cnt, t));
 #pragma unroll
         for (int t = 0; t < MT; ++t) {
           Op b[CT];
 #pragma unroll
           for (int jt = 0; jt < CT; ++jt) b[jt] = X::op(columns<T>(area_b, G::kRow, 16 * jt, t, c, g));
-          S[t] = X::template grown<CT>(k.kept(S[t], cnt), b, ws);
+#pragma unroll
+          for (int s = 0; s < NS; ++s) S[s][t] = X::template grown<CT>(k.kept(S[s][t], cnt), b, ws[s]);
         }
       }
       if constexpr (!STATE) {
@@ -794,11 +824,13 @@ template <typename T, int MT, int CT, bool STATE> __global__ __launch_bounds__(2
         if (writes && cols_bytes == kBytes) {   // through c's place in the LDS: whole rows again, 16 bytes per lane
           wave_fence();
 #pragma unroll
-          for (int t = 0; t < CT; ++t) {
-            char* const o = area_c + (16 * t + c) * G::kCRow + 4 * g * kBytes;
-            if constexpr (kBytes == 4) *reinterpret_cast<f32x4*>(o) = acc[t];
-            else *reinterpret_cast<s16x4*>(o) = X::to_out(acc[t]);
-          }
+          for (int s = 0; s < NS; ++s)
+#pragma unroll
+            for (int t = 0; t < CT; ++t) {
+              char* const o = area_c + (16 * t + c) * G::kCRow + (16 * s + 4 * g) * kBytes;
+              if constexpr (kBytes == 4) *reinterpret_cast<f32x4*>(o) = acc[s][t];
+              else *reinterpret_cast<s16x4*>(o) = X::to_out(acc[s][t]);
+            }
           wave_fence();
           if (live_c)
 #pragma unroll
@@ -809,16 +841,19 @@ template <typename T, int MT, int CT, bool STATE> __global__ __launch_bounds__(2
             }
         } else if (writes) {
 #pragma unroll
-          for (int t = 0; t < CT; ++t) {
-            const int row = 16 * t + c;
-            if (row < cnt && w.slice * 16 + 4 * g < N) *reinterpret_cast<f32x4*>(co_at + (int64_t)(reverse ? G::kCRows - 1 - row : row) * to + 16 * g) = acc[t];
-          }
+          for (int s = 0; s < NS; ++s)
+#pragma unroll
+            for (int t = 0; t < CT; ++t) {
+              const int row = 16 * t + c;
+              if (row < cnt && (w.slice * NS + s) * 16 + 4 * g < N)
+                *reinterpret_cast<f32x4*>(co_at + (int64_t)(reverse ? G::kCRows - 1 - row : row) * to + 64 * s + 16 * g) = acc[s][t];
+            }
         }
         co_at += G::kCLoads * d_out;
       }
     }
     if (!STATE && w.writer(r.fold)) {   // tokens behind the sequence's length get zeros
-      const int wide = 16 * cols_bytes;   // bytes of the slice in a row: pieces of 16
+      const int wide = 16 * NS * cols_bytes;   // bytes of the slice in a row: pieces of 16
       for (int i = lane; i < max(end - max(n, begin), 0) * (wide / 16); i += 64) {
         const int at = i % (wide / 16) * 16, tok = max(n, begin) + i / (wide / 16);
         if (w.slice * wide + at < N * cols_bytes) *reinterpret_cast<u32x4*>(out + (int64_t)tok * to + at) = u32x4{0, 0, 0, 0};
@@ -1330,7 +1365,7 @@ template <typename T, int MT> __global__ __launch_bounds__(256, 2) void la_short
 }
 
 // the state in front of every segment, from each segment's own (written one place further on) and the first state: in place.  A workgroup
-// takes 64 elements of one state; 16 groups of threads take consecutive segments each and meet through LDS
+// takes 64 elements of one state; its waves take consecutive segments each and meet through LDS
 constexpr int kMaxSegments = 256;
 __global__ __launch_bounds__(1024) void la_scan_kernel(LaArgs p) {
   __shared__ float total[16][64], fades[16];
@@ -1341,7 +1376,7 @@ __global__ __launch_bounds__(1024) void la_scan_kernel(LaArgs p) {
   const Decay decay(p.log_decay[h]);
   const bool live = at < states;
   float* const seg = r.seg + pair * p.segments * states + at;
-  const int joins = p.segments - 1, K = (joins + 15) / 16, s0 = min(z * K, joins), s1 = min(s0 + K, joins);   // this group's segments
+  const int joins = p.segments - 1, G = blockDim.x >> 6, K = (joins + G - 1) / G, s0 = min(z * K, joins), s1 = min(s0 + K, joins);   // this group's segments
   // the decay over segment s: whole, the one that holds the sequence's end, or behind it
   const int last = n / p.seg;
   const float over = decay.pow(p.seg), part = decay.pow(n - last * p.seg);
@@ -1541,7 +1576,9 @@ constexpr int kFold = 4;   // shared heads that are summed inside a workgroup; m
 
 inline int tiles(int m) { return m <= 16 ? 1 : m <= 32 ? 2 : m <= 64 ? 4 : 8; }
 
-// Segments: as many as two waves per SIMD need, each of at least kMinSegment tokens
+// Segments: as many as two waves per SIMD need, each of at least kMinSegment tokens.  The additional pass over b and c and the two launches cost
+// more than two segments bring at any length (64 sequences, 4 fp32 heads of 64: 300 tokens 48 us whole and 64 in two, 2000 tokens 284 and 304), and
+// three bring something for long sequences only (40 sequences: 300 tokens 45 us whole and 56 in three, 2000 tokens 278 and 210)
 constexpr int64_t kWaves = 2048;
 constexpr int kMinSegment = 32;
 constexpr int kCUs = 256;
@@ -1551,7 +1588,7 @@ void segmentation(int T, int64_t waves, int* seg, int* segments) {
   int64_t want = waves > 0 ? kWaves / waves : 1, most = T / kMinSegment;
   if (want > most) want = most;
   if (want > kMaxSegments) want = kMaxSegments;
-  if (want < 2) { *seg = (T + 31) / 32 * 32; *segments = 1; return; }
+  if (want < (T < 1024 ? 4 : 3)) { *seg = (T + 31) / 32 * 32; *segments = 1; return; }
   int64_t s = (T + want - 1) / want;
   s = (s + 31) / 32 * 32;
   *seg = (int)s;
@@ -1578,9 +1615,9 @@ int go(void (*kernel)(LaArgs), Resident& resident, int area, int ct, bool folds,
   kernel<<<grid, threads, lds, st>>>(a);
   return tg_launch_status();
 }
-template <typename T, int MT, int CT, bool STATE> int go_long(const LaArgs& a, dim3 grid, int threads, hipStream_t st) {
+template <typename T, int MT, int CT, int NS, bool STATE> int go_long(const LaArgs& a, dim3 grid, int threads, hipStream_t st) {
   static Resident resident;
-  return go(la_kernel<T, MT, CT, STATE>, resident, Stage<T, MT, CT>::kArea, CT, !STATE && a.group > 1, a, grid, threads, st);
+  return go(la_kernel<T, MT, CT, NS, STATE>, resident, Stage<T, MT, CT, NS>::kArea, CT * NS, !STATE && a.group > 1, a, grid, threads, st);
 }
 template <typename T, int MT, int CT, bool STATE> int go_plain(const LaArgs& a, dim3 grid, int threads, hipStream_t st) {
   static Resident resident;
@@ -1597,27 +1634,38 @@ template <typename T, int MT> int go_short(const LaArgs& a, dim3 grid, int threa
   static Resident resident;
   return go(la_short_kernel<T, MT>, resident, Stage<T, MT, 1>::kArea, 1, a.group > 1, a, grid, threads, st);
 }
-template <typename T, int MT> int go_mt(const LaArgs& a, bool staged, bool state, dim3 grid, int threads, hipStream_t st) {
+// Slices of 32 columns share a chunk's scores, its rows and the columns of b between two of 16 (16384 tokens of 64 channels: the gradients'
+// launch 61 us instead of 72).  For heads wider than 16 channels beside operands of 17 .. 64 in 16 bits; fp32 and 128 channels do not fit the
+// registers so
+inline int slice_tiles(int dtype, int M, int N) { return dtype != TG_F32 && N > 16 && (tiles(M) == 2 || tiles(M) == 4) ? 2 : 1; }
+
+template <typename T, int MT> int go_mt(const LaArgs& a, bool staged, bool state, int ns, dim3 grid, int threads, hipStream_t st) {
   // chunks of 32 tokens halve the work on the state per token; sequences of one chunk of 16 would waste half of them, and two tiles of 128
   // fp32 channels, or of 128 channels that every lane loads itself, do not fit the registers
-  constexpr int CT = MT == 8 && sizeof(typename Mat<T>::Raw) == 16 ? 1 : 2, CU = MT == 8 ? 1 : 2;
+  constexpr bool f32 = sizeof(typename Mat<T>::Raw) == 16;
+  constexpr int CT = MT == 8 && f32 ? 1 : 2, CU = MT == 8 ? 1 : 2;
   if (staged) {
-    if (state) return go_long<T, MT, CT, true>(a, grid, threads, st);
-    return a.T <= 16 ? go_short<T, MT>(a, grid, threads, st) : go_long<T, MT, CT, false>(a, grid, threads, st);
+    if (!state && a.T <= 16) return go_short<T, MT>(a, grid, threads, st);
+    if constexpr (!f32 && (MT == 2 || MT == 4))
+      if (ns == 2) return state ? go_long<T, MT, CT, 2, true>(a, grid, threads, st) : go_long<T, MT, CT, 2, false>(a, grid, threads, st);
+    return state ? go_long<T, MT, CT, 1, true>(a, grid, threads, st) : go_long<T, MT, CT, 1, false>(a, grid, threads, st);
   }
   if (state) return go_plain<T, MT, CU, true>(a, grid, threads, st);
   return a.T <= 16 ? go_plain<T, MT, 1, false>(a, grid, threads, st) : go_plain<T, MT, CU, false>(a, grid, threads, st);
 }
 // `roles` roles with the same number of m tiles in one launch
-template <typename T> int launch(LaArgs a, int roles, bool state, hipStream_t st) {
-  int mt = 1, slices = 1;
+template <typename T> int launch(LaArgs a, int dtype, int roles, bool state, hipStream_t st) {
+  int mt = 1, most = 1, ns = 2;
   bool staged = true;
   for (int i = 0; i < roles; ++i) {
     const Role& r = a.r[i];
     if (tiles(r.M) > mt) mt = tiles(r.M);
-    if ((r.N + 15) / 16 > slices) slices = (r.N + 15) / 16;
+    if (r.N > most) most = r.N;
+    if (slice_tiles(dtype, r.M, r.N) < ns) ns = slice_tiles(dtype, r.M, r.N);
+    staged = staged && r.pieces;
   }
-  for (int i = 0; i < roles; ++i) staged = staged && a.r[i].pieces;
+  if (!staged || (!state && a.T <= 16)) ns = 1;
+  const int slices = (most + 16 * ns - 1) / (16 * ns);
   // workgroups of up to kFold waves, as few idle ones among them as possible
   const int64_t units = (int64_t)(a.H / a.group) * slices;
   if (units > 0x7fffff00) return TG_E_UNSUPPORTED;
@@ -1627,13 +1675,14 @@ template <typename T> int launch(LaArgs a, int roles, bool state, hipStream_t st
   a.columns = (int)((units + per - 1) / per);
   const dim3 grid(1, roles, state ? a.segments - 1 : a.segments);
   const int threads = 64 * per * a.group;
-  if (mt == 1) return go_mt<T, 1>(a, staged, state, grid, threads, st);
-  if (mt == 2) return go_mt<T, 2>(a, staged, state, grid, threads, st);
-  if (mt == 4) return go_mt<T, 4>(a, staged, state, grid, threads, st);
-  return go_mt<T, 8>(a, staged, state, grid, threads, st);
+  if (mt == 1) return go_mt<T, 1>(a, staged, state, ns, grid, threads, st);
+  if (mt == 2) return go_mt<T, 2>(a, staged, state, ns, grid, threads, st);
+  if (mt == 4) return go_mt<T, 4>(a, staged, state, ns, grid, threads, st);
+  return go_mt<T, 8>(a, staged, state, ns, grid, threads, st);
 }
 int launch_dt(int dtype, const LaArgs& a, int roles, bool state, hipStream_t st) {
-  TG_DISPATCH_DTYPE(dtype, return launch<BF16>(a, roles, state, st), return launch<F16>(a, roles, state, st), return launch<F32>(a, roles, state, st));
+  TG_DISPATCH_DTYPE(dtype, return launch<BF16>(a, dtype, roles, state, st), return launch<F16>(a, dtype, roles, state, st),
+                    return launch<F32>(a, dtype, roles, state, st));
 }
 
 struct Strided { Operand o; bool wide, pieces; };   // aligned to 4 elements, to 16 bytes: the address and all strides
@@ -1654,11 +1703,16 @@ int check(int dtype, const tg_la_desc* d) {
   return TG_OK;
 }
 
-inline int64_t slices_of(int n) { return (n + 15) / 16; }
+inline int64_t slices_of(int dtype, int M, int N) {
+  const int n = 16 * slice_tiles(dtype, M, N);
+  return (N + n - 1) / n;
+}
 // segments of the forward pass (one role) and of the backward pass (three)
-void forward_segments(const tg_la_desc* d, int* seg, int* segments) { segmentation(d->T, (int64_t)d->B * d->H * slices_of(d->DV), seg, segments); }
-void backward_segments(const tg_la_desc* d, int* seg, int* segments) {
-  segmentation(d->T, (int64_t)d->B * d->H * (2 * slices_of(d->DK) + slices_of(d->DV)), seg, segments);
+void forward_segments(int dtype, const tg_la_desc* d, int* seg, int* segments) {
+  segmentation(d->T, (int64_t)d->B * d->H * slices_of(dtype, d->DK, d->DV), seg, segments);
+}
+void backward_segments(int dtype, const tg_la_desc* d, int* seg, int* segments) {
+  segmentation(d->T, (int64_t)d->B * d->H * (2 * slices_of(dtype, d->DV, d->DK) + slices_of(dtype, d->DK, d->DV)), seg, segments);
 }
 inline int64_t states(const tg_la_desc* d) { return (int64_t)d->B * d->H * d->DK * d->DV; }
 inline int64_t fold_floats(const tg_la_desc* d) { return d->H / d->HK > kFold ? (int64_t)d->B * d->T * d->H * (d->DK + d->DV) : 0; }
@@ -1667,7 +1721,8 @@ inline int64_t fold_floats(const tg_la_desc* d) { return d->H / d->HK > kFold ? 
 int join_segments(int dtype, const LaArgs& a, int roles, hipStream_t st) {
   const int rc = launch_dt(dtype, a, roles, true, st);
   if (rc != TG_OK) return rc;
-  la_scan_kernel<<<dim3((a.r[0].M * a.r[0].N + 63) / 64, (unsigned)(a.B * a.H), roles), 1024, 0, st>>>(a);
+  const int joins = a.segments - 1, waves = joins < 16 ? joins : 16;
+  la_scan_kernel<<<dim3((a.r[0].M * a.r[0].N + 63) / 64, (unsigned)(a.B * a.H), roles), 64 * waves, 0, st>>>(a);
   return tg_launch_status();
 }
 
@@ -1688,10 +1743,10 @@ template <typename T> int launch_step(const StepArgs& a, bool wide, hipStream_t 
 
 }  // namespace
 
-extern "C" int64_t tg_linear_attention_scratch_floats(const tg_la_desc* d) {
-  if (check(TG_F32, d) != TG_OK) return 0;
+extern "C" int64_t tg_linear_attention_scratch_floats(int dtype, const tg_la_desc* d) {
+  if (check(dtype, d) != TG_OK) return 0;
   int seg, segments;
-  forward_segments(d, &seg, &segments);
+  forward_segments(dtype, d, &seg, &segments);
   return segments > 1 ? segments * states(d) : 0;
 }
 
@@ -1701,7 +1756,7 @@ extern "C" int tg_linear_attention(int dtype, const tg_la_desc* d, const void* q
   if (rc != TG_OK) return rc;
   if (d->B == 0) return TG_OK;
   LaArgs a{};
-  forward_segments(d, &a.seg, &a.segments);
+  forward_segments(dtype, d, &a.seg, &a.segments);
   if (!log_decay || !state_out || (d->T > 0 && (!q || !k || !v || !o)) || (a.segments > 1 && !scratch)) return TG_E_BADARG;
   if (!elem_aligned(dtype, q) || !elem_aligned(dtype, k) || !elem_aligned(dtype, v) || !elem_aligned(dtype, o) || !word_aligned(log_decay) ||
       !word_aligned(lengths) || !word_aligned(state_in) || !word_aligned(state_out) || !word_aligned(scratch))
@@ -1722,10 +1777,10 @@ extern "C" int tg_linear_attention(int dtype, const tg_la_desc* d, const void* q
   return launch_dt(dtype, a, 1, false, st);
 }
 
-extern "C" int64_t tg_linear_attention_bwd_scratch_floats(const tg_la_desc* d) {
-  if (check(TG_F32, d) != TG_OK) return 0;
+extern "C" int64_t tg_linear_attention_bwd_scratch_floats(int dtype, const tg_la_desc* d) {
+  if (check(dtype, d) != TG_OK) return 0;
   int seg, segments;
-  backward_segments(d, &seg, &segments);
+  backward_segments(dtype, d, &seg, &segments);
   return fold_floats(d) + (segments > 1 ? 2 * segments * states(d) : 0);
 }
 
@@ -1736,9 +1791,9 @@ extern "C" int tg_linear_attention_bwd(int dtype, const tg_la_desc* d, const voi
   if (rc != TG_OK) return rc;
   if (d->B == 0) return TG_OK;
   LaArgs a{};
-  backward_segments(d, &a.seg, &a.segments);
+  backward_segments(dtype, d, &a.seg, &a.segments);
   const int G = d->H / d->HK;
-  if (!log_decay || !dout_stride || (d->T > 0 && (!q || !k || !v || !dout || !dq || !dk || !dv)) || (tg_linear_attention_bwd_scratch_floats(d) && !scratch))
+  if (!log_decay || !dout_stride || (d->T > 0 && (!q || !k || !v || !dout || !dq || !dk || !dv)) || (tg_linear_attention_bwd_scratch_floats(dtype, d) && !scratch))
     return TG_E_BADARG;
   if (dout_stride[0] < 0 || dout_stride[1] < 0 || dout_stride[2] < 0) return TG_E_BADARG;
   if (dout_stride[1] > 0x7fffffff) return TG_E_UNSUPPORTED;

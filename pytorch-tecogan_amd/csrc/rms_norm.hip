@@ -17,8 +17,8 @@
 namespace {
 
 // One 16-byte piece of a row - W consecutive elements - as floats.  EVEN: every piece is whole and aligned.  Otherwise C or an address
-// does not fill 16 bytes: the loads and stores are unaligned ones (the hardware takes them: a 1001-channel fp16 row costs 1.15 of an
-// aligned one's time instead of the 2.9 of single elements), and a row's last piece goes element by element.  n: elements of the row left.
+// does not fill 16 bytes: the loads and stores are unaligned ones, which the hardware takes (fp16 rows of 1001 channels: forward 6.6 us
+// instead of the 13.4 of single elements, gradient 10.6 instead of 25.4), and a row's last piece goes element by element.  n: elements left.
 template <typename T, bool EVEN> struct Piece {
   static constexpr int W = 16 / ElemTraits<T>::kBytes;
   __device__ __forceinline__ static void load(const void* base, int64_t i, int n, float* v) {

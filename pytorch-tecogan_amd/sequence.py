@@ -312,7 +312,7 @@ def _attention_fwd(q, k, v, log_decay, scale, state, lengths):
     lengths = _lengths(q, lengths)
     o = torch.empty((B, T, H, DV), dtype=q.dtype, device=dev)
     last = torch.empty((B, H, DK, DV), dtype=torch.float32, device=dev)
-    n = _floats_of("tg_linear_attention_scratch_floats", d)
+    n = _floats_of("tg_linear_attention_scratch_floats", dt, d)
     scratch = torch.empty(n, dtype=torch.float32, device=dev) if n else None
     _call(dev, "tg_linear_attention", dt, d, q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), _ptr(lengths), _ptr(state), o.data_ptr(),
           last.data_ptr(), _ptr(scratch))
@@ -363,7 +363,7 @@ def linear_attention_backward(do, q, k, v, log_decay, scale=None, state=None, le
     lengths = _lengths(q, lengths)
     dq, dk, dv = _rowmajor(q), _rowmajor(k), _rowmajor(v)
     first = None if state is None else torch.empty(shape, dtype=torch.float32, device=dev)
-    n = _floats_of("tg_linear_attention_bwd_scratch_floats", d)
+    n = _floats_of("tg_linear_attention_bwd_scratch_floats", dt, d)
     scratch = torch.empty(n, dtype=torch.float32, device=dev) if n else None
     _call(dev, "tg_linear_attention_bwd", dt, d, q.data_ptr(), k.data_ptr(), v.data_ptr(), do.data_ptr(), _STRIDES.pack(*do.stride()[:3]),
           log_decay.data_ptr(), _ptr(lengths), _ptr(state), _ptr(dstate), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _ptr(first), _ptr(scratch))

@@ -66,10 +66,10 @@ def test_linear_attention_arguments():
     for d, want in ((desc(B=-1), BADARG), (desc(T=-1), BADARG), (desc(H=0), BADARG), (desc(HK=0), BADARG), (desc(DK=0), BADARG), (desc(DV=0), BADARG),
                     (desc(H=3), UNSUPPORTED), (desc(DK=129), UNSUPPORTED), (desc(DV=129), UNSUPPORTED)):
         assert lib.tg_linear_attention(L.TG_F32, ref(d), P, P, P, P, None, None, P, P, None, None) == want
-        assert lib.tg_linear_attention_scratch_floats(ref(d)) == 0
+        assert lib.tg_linear_attention_scratch_floats(L.TG_BF16, ref(d)) == 0
         assert lib.tg_linear_attention_step(L.TG_F32, ref(d), P, P, P, P, P, P, None) == want
         assert lib.tg_linear_attention_bwd(L.TG_F32, ref(d), P, P, P, P, (C.c_int64 * 3)(80, 16, 8), P, None, None, None, P, P, P, None, P, None) == want
-        assert lib.tg_linear_attention_bwd_scratch_floats(ref(d)) == 0
+        assert lib.tg_linear_attention_bwd_scratch_floats(L.TG_BF16, ref(d)) == 0
     d = desc()
     good = [L.TG_BF16, ref(d), P, P, P, P, None, None, P, P, None, None]
     for at, value, want in ((0, 9, BADARG), (1, None, BADARG), (2, None, BADARG), (3, None, BADARG), (4, None, BADARG), (5, None, BADARG), (8, None, BADARG),
@@ -93,8 +93,8 @@ def test_linear_attention_arguments():
         assert lib.tg_linear_attention_bwd(*bad) == want, (at, value)
     # one long sequence is cut into segments: their states need scratch
     long = desc(B=1, T=4096, H=1, HK=1)
-    need = lib.tg_linear_attention_scratch_floats(ref(long))
-    assert need >= 2 * 16 * 8 and lib.tg_linear_attention_bwd_scratch_floats(ref(long)) >= 4 * 16 * 8
+    need = lib.tg_linear_attention_scratch_floats(L.TG_BF16, ref(long))
+    assert need >= 2 * 16 * 8 and lib.tg_linear_attention_bwd_scratch_floats(L.TG_BF16, ref(long)) >= 4 * 16 * 8
     assert lib.tg_linear_attention(L.TG_BF16, ref(long), P, P, P, P, None, None, P, P, None, None) == BADARG
     wild = desc()
     wild.k_stride[1] = 1 << 31
