@@ -1585,7 +1585,7 @@ constexpr int kCUs = 256;
 
 // (tokens in a segment, segments) for `waves` waves per segment
 void segmentation(int T, int64_t waves, int* seg, int* segments) {
-  int64_t want = waves > 0 ? kWaves / waves : 1, most = T / kMinSegment;
+  int64_t want = waves > 0 ? kWaves / waves : 1, most = (T + kMinSegment - 1) / kMinSegment;
   if (want > most) want = most;
   if (want > kMaxSegments) want = kMaxSegments;
   if (want < (T < 1024 ? 4 : 3)) { *seg = (T + 31) / 32 * 32; *segments = 1; return; }
