@@ -569,8 +569,8 @@ int tg_resample_u8(const void* frames_u8, void* tmp_u8, float* out_nchw, const i
  * row-major with the channel dimension contiguous, TG_F32 / TG_BF16 / TG_F16, any size and alignment of the element type (16-byte
  * aligned pointers and strides take the wide loads); strides are in ELEMENTS.  No float atomics: the same call gives the same bits.
  *
- * tg_rms_norm: s = x + res (res may be null: s = x), y = s * rstd * weight, rstd = 1 / sqrt(mean_c s^2 + eps), per row of C channels;
- *   weight [C] fp32 or null (ones); x, res rows at x_stride, res_stride; y, s [rows][C] contiguous; s (null: not stored; written only with
+ * tg_rms_norm: s = x + res (res may be null: s = x), y = s * rstd * weight, rstd = 1 / sqrt(mean_c s^2 + eps), per row of C <= 2^30
+ *   channels; weight [C] fp32 or null (ones); x, res rows at x_stride, res_stride; y, s [rows][C] contiguous; s (null: not stored; written only with
  *   res) is rounded to the element type, y is computed from the unrounded sum; rstd [rows] or null.
  * tg_rms_norm_e4m3: q [rows][C] = e4m3(y / scale[row]), scale[row] = max(max_c |y|, 2^-100) / 448.  A NaN in a row makes its scale NaN.
  * tg_rms_norm_bwd: dx = rstd (g - xhat mean_c(g xhat)) (+ ds), g = dy weight, xhat = (x + res) rstd; dweight [C] (null: not wanted) =
@@ -590,7 +590,8 @@ int tg_rms_norm_bwd(int dtype, const void* dy, int64_t dy_stride, const void* x,
 int tg_dropout(int dtype, const void* x, const void* res, void* y, int64_t n, double p, const int64_t* rng, int layer, void* stream);
 
 /* S_t = exp(log_decay[h]) S_{t-1} + k_t v_t^T, o_t = scale q_t S_t per sequence and head; q [B][T][H][DK], k [B][T][HK][DK], v [B][T][HK][DV]
- * at the given strides of (sequence, token, head), H % HK == 0: head h reads stored head h / (H / HK); 1 <= DK, DV <= 128, H <= 65536.
+ * at the given strides of (sequence, token, head), H % HK == 0: head h reads stored head h / (H / HK); 1 <= DK, DV <= 128, H <= 65536,
+ * B and T <= 2^30.
  * Outputs o, dq [B][T][H][..], dk, dv [B][T][HK][..] are contiguous; states [B][H][DK][DV] fp32; lengths [B] int32 or null: tokens at and
  * behind lengths[b] (clamped to 0 .. T) are not read, their rows of the outputs are zero and the last state is the one at the length.
  * state_in null: zeros.  tg_linear_attention_bwd: dstate_out null: zeros; dstate_in may be null.  scratch: *_scratch_floats floats (0: may

@@ -1597,15 +1597,18 @@ void segmentation(int T, int64_t waves, int* seg, int* segments) {
 
 // One launch.  Sequences are dealt out so that the grid fills the machine ONCE (a wave makes its decay's powers once, and no second round of
 // workgroups finds the machine half empty: 4096 waves where 3072 fit ran 338 us, 3072 ran 274)
-struct Resident { std::atomic<int> n[2][kFold + 1]; };   // a kernel's workgroups on a CU, by folds and waves; 0: not known yet
+constexpr int kDevices = 16;
+struct Resident { std::atomic<int> n[kDevices][2][kFold + 1]; };   // a kernel's workgroups on a CU, by device, folds and waves; 0: not known yet
 int go(void (*kernel)(LaArgs), Resident& resident, int area, int ct, bool folds, LaArgs a, dim3 grid, int threads, hipStream_t st) {
   const int waves = threads / 64, lds = (folds ? 2 * waves * ct * 64 * 16 : 0) + waves * area;
-  int per_cu = resident.n[folds][waves].load(std::memory_order_relaxed);
+  int dev;
+  TG_CHECK_HIP(hipGetDevice(&dev));   // (a kernel's attributes are each device's own)
+  int per_cu = dev < kDevices ? resident.n[dev][folds][waves].load(std::memory_order_relaxed) : 0;
   if (per_cu == 0) {
     TG_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
     TG_CHECK_HIP(hipOccupancyMaxActiveBlocksPerMultiprocessor(&per_cu, reinterpret_cast<const void*>(kernel), threads, (size_t)lds));
     if (per_cu < 1) return TG_E_UNSUPPORTED;
-    resident.n[folds][waves].store(per_cu, std::memory_order_relaxed);
+    if (dev < kDevices) resident.n[dev][folds][waves].store(per_cu, std::memory_order_relaxed);
   }
   const int64_t columns = a.columns, others = columns * grid.y * grid.z, room = (int64_t)per_cu * kCUs;
   const int64_t each = (a.B * others + room - 1) / room;             // sequences of a workgroup
@@ -1694,9 +1697,10 @@ Strided operand(int dtype, const void* p, const int64_t* stride, int shared) {
   return {Operand{p, stride[0], stride[2], (int)stride[1], shared}, aligned(4), aligned(16 / elem_bytes(dtype)) && stride[1] * elem_bytes(dtype) <= (1 << 25)};
 }
 
+constexpr int kMost = 1 << 30;   // sequences and tokens: the kernels' steps beyond the last one stay within 32 bits
 int check(int dtype, const tg_la_desc* d) {
   if (!d || !known(dtype) || d->B < 0 || d->T < 0 || d->H <= 0 || d->HK <= 0 || d->DK <= 0 || d->DV <= 0) return TG_E_BADARG;
-  if (d->H % d->HK || d->DK > kMaxHead || d->DV > kMaxHead || d->T > 0x7fffff00 || d->H > 65536) return TG_E_UNSUPPORTED;
+  if (d->H % d->HK || d->DK > kMaxHead || d->DV > kMaxHead || d->B > kMost || d->T > kMost || d->H > 65536) return TG_E_UNSUPPORTED;
   for (const int64_t* s : {d->q_stride, d->k_stride, d->v_stride})
     if (s[0] < 0 || s[1] < 0 || s[2] < 0) return TG_E_BADARG;
     else if (s[1] > 0x7fffffff) return TG_E_UNSUPPORTED;

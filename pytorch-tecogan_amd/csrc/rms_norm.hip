@@ -439,6 +439,7 @@ __global__ __launch_bounds__(1024) void rms_dw_fold_kernel(const float* partial,
 
 constexpr int kMaxGrid = 1 << 20;      // (forward) workgroups; rows beyond are walked
 constexpr int kBwdGrid = 512;         // (backward) workgroups = partial rows of dw
+constexpr int kMaxChannels = 1 << 30;  // channel indices, and a workgroup's step beyond the last one, are 32-bit
 
 struct Shape { int L, NV; };           // lanes of a row and 16-byte pieces of a lane; 0: the long form
 inline Shape pick(int pieces) {
@@ -499,6 +500,7 @@ inline bool wide(int dtype, int C, int64_t stride, const void* p) {   // 16-byte
 template <bool Q8>
 int rms_fwd(int dtype, const FwdArgs& a, hipStream_t st) {
   if (!known(dtype) || a.rows < 0 || a.C <= 0 || a.xs < 0 || a.rs < 0 || !(a.eps >= 0.f)) return TG_E_BADARG;
+  if (a.C > kMaxChannels) return TG_E_UNSUPPORTED;
   if (a.rows == 0) return TG_OK;
   if (!a.x || !a.y || (Q8 && !a.scale)) return TG_E_BADARG;
   if (!elem_aligned(a.x, dtype) || !elem_aligned(a.res, dtype) || !elem_aligned(a.s, dtype) || (!Q8 && !elem_aligned(a.y, dtype)) ||
@@ -533,6 +535,7 @@ extern "C" int tg_rms_norm_bwd(int dtype, const void* dy, int64_t dy_stride, con
                                float* dweight, float* scratch, int64_t rows, int C, void* stream) {
   if (!known(dtype) || rows < 0 || C <= 0 || dy_stride < 0 || x_stride < 0 || res_stride < 0 || ds_stride < 0 || (dweight && rows && !scratch))
     return TG_E_BADARG;
+  if (C > kMaxChannels) return TG_E_UNSUPPORTED;
   const BwdArgs a{dy, x, res, ds, rstd, weight, dx, dweight ? scratch : nullptr, dy_stride, x_stride, res_stride, ds_stride, rows, C};
   hipStream_t st = (hipStream_t)stream;
   if (rows == 0) {   // the gradient of no rows

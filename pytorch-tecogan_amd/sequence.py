@@ -18,6 +18,7 @@ __all__ = ["rms_norm", "rms_norm_backward", "rms_norm_e4m3", "dropout", "dropout
            "linear_attention_backward", "linear_attention_step"]
 
 MAX_HEAD = 128   # largest Dk / Dv of linear_attention
+MOST = 1 << 30   # channels of a normalised row, sequences and tokens
 
 
 def _fail(text):
@@ -76,9 +77,13 @@ def _f32(x, t, what, shape):
     return t if t.is_contiguous() else t.contiguous()
 
 
+def _wants_grad(*tensors):
+    return torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in tensors)
+
+
 def _grad(*tensors):
     """whether autograd has to record this call"""
-    if not torch.is_grad_enabled() or not any(t is not None and t.requires_grad for t in tensors):
+    if not _wants_grad(*tensors):
         return False
     if torch.cuda.is_current_stream_capturing():
         _fail("autograd is not captured into graphs: use torch.no_grad(), or the explicit backward functions on detached tensors")
@@ -105,8 +110,8 @@ def _rowmajor(x):
 
 def _norm_args(x, weight, residual, eps):
     dt = _floats(x, "x")
-    if x.dim() < 1 or x.shape[-1] < 1:
-        _fail("rms_norm normalises the last dimension: it must have at least one channel")
+    if x.dim() < 1 or not 1 <= x.shape[-1] <= MOST:
+        _fail("rms_norm normalises the last dimension: it must have 1 .. 2^30 channels")
     if not eps >= 0:
         _fail("eps must not be negative")
     channels = x.shape[-1]
@@ -193,7 +198,7 @@ def rms_norm_backward(dy, x, rstd, weight=None, residual=None, ds=None, dweight=
 def rms_norm_e4m3(x, weight=None, residual=None, eps=1e-6):
     """rms_norm with an 8-bit output: (q, scale), or (q, scale, s) with a residual; q float8_e4m3fn like x, scale float32 per row =
     max(max|y|, 2^-100) / 448, y ~ q * scale.  A serving form: it has no gradient."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, residual)):
+    if _wants_grad(x, weight, residual):
         _fail("rms_norm_e4m3 has no gradient: call it under torch.no_grad()")
     dt, channels, weight = _norm_args(x, weight, residual, eps)
     xr, xs = _rows(x, channels)
@@ -284,6 +289,8 @@ def _desc(q, k, v, log_decay, scale, step, recorded=True):
         _fail(f"{H} query heads do not divide over {HK} key / value heads")
     if not (1 <= DK <= MAX_HEAD and 1 <= DV <= MAX_HEAD):
         _fail(f"head sizes must be 1 .. {MAX_HEAD}: got {DK} and {DV}")
+    if B > MOST or T > MOST:
+        _fail("at most 2^30 sequences and tokens")
     log_decay = _f32(q, log_decay, "log_decay", (H,))
     if recorded and log_decay.requires_grad and torch.is_grad_enabled():
         _fail("log_decay is a constant of the heads: it has no gradient")
@@ -374,7 +381,7 @@ def linear_attention_step(q, k, v, log_decay, state, scale=None):
     """The next token of every sequence: q (B, H, Dk), k (B, Hk, Dk), v (B, Hk, Dv) -> o (B, H, Dv); `state`, float32 (B, H, Dk, Dv) and
     contiguous, is updated in place.  The single-token form of linear_attention (as generator.recurrent_step is of generator.recurrent); it has no
     gradient."""
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, state)):
+    if _wants_grad(q, k, v, state):
         _fail("linear_attention_step has no gradient: call it under torch.no_grad(), or linear_attention with one token")
     dt, d, (B, _, H, DK, DV), q, k, v, log_decay = _desc(q, k, v, log_decay, scale, True)
     _f32(q, state, "state", (B, H, DK, DV))

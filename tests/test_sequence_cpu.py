@@ -27,7 +27,8 @@ def test_rms_norm_arguments():
     f = L.load().tg_rms_norm
     good = [L.TG_BF16, P, 64, None, 0, P, P, None, None, 4, 64, 1e-6, None]
     for at, value, want in ((0, 7, BADARG), (1, None, BADARG), (6, None, BADARG), (9, -1, BADARG), (10, 0, BADARG), (2, -64, BADARG), (11, -1.0, BADARG),
-                            (11, float("nan"), BADARG), (1, P + 1, ALIGN), (3, P + 1, ALIGN), (6, P + 1, ALIGN), (5, P + 2, ALIGN), (8, P + 2, ALIGN)):
+                            (11, float("nan"), BADARG), (1, P + 1, ALIGN), (3, P + 1, ALIGN), (6, P + 1, ALIGN), (5, P + 2, ALIGN), (8, P + 2, ALIGN),
+                            (10, (1 << 30) + 1, UNSUPPORTED)):
         bad = list(good)
         bad[at] = value
         assert f(*bad) == want, (at, value)
@@ -41,7 +42,7 @@ def test_rms_norm_arguments():
     f = L.load().tg_rms_norm_bwd
     good = [L.TG_F16, P, 64, P, 64, None, 0, P, P, None, 0, P, P, P, 4, 64, None]
     for at, value, want in ((1, None, BADARG), (3, None, BADARG), (7, None, BADARG), (11, None, BADARG), (13, None, BADARG), (14, -1, BADARG), (15, 0, BADARG),
-                            (1, P + 1, ALIGN), (9, P + 1, ALIGN), (12, P + 2, ALIGN), (13, P + 2, ALIGN)):
+                            (1, P + 1, ALIGN), (9, P + 1, ALIGN), (12, P + 2, ALIGN), (13, P + 2, ALIGN), (15, (1 << 30) + 1, UNSUPPORTED)):
         bad = list(good)
         bad[at] = value
         assert f(*bad) == want, (at, value)
@@ -64,7 +65,7 @@ def test_linear_attention_arguments():
     lib = L.load()
     ref = C.byref
     for d, want in ((desc(B=-1), BADARG), (desc(T=-1), BADARG), (desc(H=0), BADARG), (desc(HK=0), BADARG), (desc(DK=0), BADARG), (desc(DV=0), BADARG),
-                    (desc(H=3), UNSUPPORTED), (desc(DK=129), UNSUPPORTED), (desc(DV=129), UNSUPPORTED)):
+                    (desc(H=3), UNSUPPORTED), (desc(DK=129), UNSUPPORTED), (desc(DV=129), UNSUPPORTED), (desc(B=(1 << 30) + 1), UNSUPPORTED), (desc(T=(1 << 30) + 1), UNSUPPORTED)):
         assert lib.tg_linear_attention(L.TG_F32, ref(d), P, P, P, P, None, None, P, P, None, None) == want
         assert lib.tg_linear_attention_scratch_floats(L.TG_BF16, ref(d)) == 0
         assert lib.tg_linear_attention_step(L.TG_F32, ref(d), P, P, P, P, P, P, None) == want

@@ -8,6 +8,7 @@ states into two bf16 halves beside 16-bit inputs: 2^-16 of the magnitudes for ea
 own two halves)."""
 import math
 import os
+import subprocess
 import sys
 
 import numpy as np
@@ -304,14 +305,12 @@ def test_dropout_past_32_bit_indices():
     x = torch.ones(n, device=DEV, dtype=BF16)
     y = ops.dropout(x, 0.5, ops.dropout_rng(3, DEV))
     del x
-    low = np.uint64(0xffffffff)
     # words of block 2^30: counter (2^30, 0, ..): 32-bit element arithmetic would have wrapped to block 0
     tail = y[-4:].float().cpu() != 0
     first = y[:4].float().cpu() != 0
     c = philox_block(1 << 30, 3)
     assert torch.equal(tail, torch.tensor([w >= 1 << 31 for w in c])), (tail, c)
     assert torch.equal(first, torch.tensor([int(w) >= 1 << 31 for w in philox_words(4, 3, 0, 0)]))
-    assert low
 
 
 def philox_block(block, seed, step=0, layer=0):
@@ -738,6 +737,39 @@ def test_autograd_is_refused_inside_a_capture():
     assert y.shape == x.shape
 
 
+FIRST_CALL = """
+import torch
+import pytorch_tecogan_amd
+from pytorch_tecogan_amd import ops
+torch.manual_seed(5)
+x, w = torch.randn(70, 200, device="cuda"), torch.randn(200, device="cuda")
+q, k, v, do = (torch.randn(2, 300, 2, 64, device="cuda").bfloat16() for _ in range(4))
+decay, state = torch.tensor([-0.1, -0.5], device="cuda"), torch.randn(2, 2, 64, 64, device="cuda")
+rng = torch.tensor([1, 2], device="cuda")
+def run():
+    one = state.clone()
+    return (ops.rms_norm(x, w), ops.rms_norm_e4m3(x, w)[1], ops.dropout(x, 0.3, rng), *ops.linear_attention(q, k, v, decay, state=state),
+            *ops.linear_attention_backward(do, q, k, v, decay, state=state), ops.linear_attention_step(q[:, 0], k[:, 0], v[:, 0], decay, one), one)
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    got = run()
+for i in range(3):
+    x.normal_(), q.normal_()
+    torch.cuda.synchronize()
+    graph.replay()
+    torch.cuda.synchronize()
+    for a, b in zip(got, run()):
+        assert torch.equal(a, b), i
+print("replays equal")
+"""
+
+
+def test_the_first_call_of_a_process_inside_a_capture():
+    """kernels are loaded and their attributes set by the captured call itself"""
+    r = subprocess.run([sys.executable, "-c", FIRST_CALL], cwd=ROOT, env={**os.environ, "PYTHONPATH": ROOT}, capture_output=True, text=True, timeout=100)
+    assert r.returncode == 0 and "replays equal" in r.stdout, r.stderr[-2000:]
+
+
 def test_refusals():
     x, w = randn(4, 64), randn(64)
     rng, decay = ops.dropout_rng(1, DEV), torch.zeros(2, device=DEV)
@@ -765,6 +797,16 @@ def test_refusals():
         lambda: ops.linear_attention_step(q[:, 0], k[:, 0], v[:, 0], decay, state.transpose(2, 3)),
         lambda: ops.linear_attention_step(q[:, 0], k[:, 0], v[:, 0], decay, randn(2, 2, 8, 16).transpose(2, 3)),
         lambda: ops.linear_attention_step(q[:, 0].clone().requires_grad_(), k[:, 0], v[:, 0], decay, state),
+        # no tensors
+        lambda: ops.rms_norm([1.0]), lambda: ops.rms_norm(x, 2.0), lambda: ops.rms_norm(x, w, residual=1.0), lambda: ops.rms_norm_e4m3(x, 2.0),
+        lambda: ops.dropout(None, 0.1, rng), lambda: ops.dropout(x, 0.1, rng, residual=0.0), lambda: ops.linear_attention(None, k, v, decay),
+        lambda: ops.linear_attention(q, [1.0], v, decay), lambda: ops.linear_attention(q, k, v, -0.1), lambda: ops.linear_attention(q, k, v, decay, state=0.0),
+        lambda: ops.linear_attention(q, k, v, decay, lengths=[1, 2]), lambda: ops.linear_attention_step(q[:, 0], None, v[:, 0], decay, state),
+        lambda: ops.linear_attention_step(q[:, 0], k[:, 0], v[:, 0], decay, None),
+        # 2^30 + 1 sequences (strides of zero: nothing is allocated before the refusal)
+        lambda: ops.linear_attention_step(*(t[:1, 0].expand((1 << 30) + 1, -1, -1) for t in (q, k, v)), decay, state),
+        lambda: ops.linear_attention(*(t[:1, :1].expand(-1, (1 << 30) + 1, -1, -1) for t in (q, k, v)), decay),
+        lambda: ops.rms_norm(x[:1, :1].expand(1, (1 << 30) + 1)),
     ]
     for i, call in enumerate(bad):
         with pytest.raises(L.TecoganHipError):
