@@ -399,41 +399,39 @@ template <typename T> __global__ __launch_bounds__(256) void rms_dw_long_kernel(
   a.partial[(int64_t)blockIdx.y * a.C + c] = t;
 }
 
-// dw[c] = sum over the n partial rows: 64 columns a workgroup, thread (slice, 4 columns) adds every 64th row with eight loads in flight, and the
-// slices meet in order (one thread per column and 16 slices waited for each of its 64 loads: 16.6 us for 1024 rows of 64; 2.9 us for 512 so)
+// dw[c] = sum over the n partial rows: 16 columns a workgroup, thread (slice, 4 columns) adds every 256th row with four loads in flight, the slices of
+// a wave meet in a tree and the waves in order (64 columns a workgroup and 64 slices, single elements for an odd C: 8.5 us for 512 rows of
+// 1001; 3.7 so.  One thread per column and 16 slices waited for each of its loads: 16.6 us for 1024 rows of 64)
 __global__ __launch_bounds__(1024) void rms_dw_fold_kernel(const float* partial, float* dw, int n, int C) {
-  __shared__ float t[64][64 + 4], u[16][64];
-  const int q = (threadIdx.x & 15) * 4, z = threadIdx.x >> 4, c = blockIdx.x * 64 + q;
-  f32x4 v = {0.f, 0.f, 0.f, 0.f};
-  const bool whole = C % 4 == 0 && (reinterpret_cast<uintptr_t>(partial) & 15) == 0;
-  for (int i = z; i < n; i += 64 * 8) {
-    f32x4 w[8];
+  __shared__ float t[16][16];
+  const int q = (threadIdx.x & 3) * 4, c = blockIdx.x * 16 + q;
+  float v[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int i = threadIdx.x >> 2; i < n && c < C; i += 256 * 4) {
+    float w[4][4];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      w[k] = f32x4{0.f, 0.f, 0.f, 0.f};
-      const float* p = partial + (int64_t)(i + 64 * k) * C + c;
-      if (i + 64 * k < n && c < C) {
-        if (whole) w[k] = *reinterpret_cast<const f32x4*>(p);
-        else
+    for (int k = 0; k < 4; ++k) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (c + e < C) w[k][e] = p[e];
-      }
+      for (int e = 0; e < 4; ++e) w[k][e] = 0.f;
+      if (i + 256 * k < n) load_f32<4, false>(partial + (int64_t)(i + 256 * k) * C, c, C - c, w[k]);
     }
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v += w[k];
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] += w[k][e];
   }
 #pragma unroll
-  for (int e = 0; e < 4; ++e) t[z][q + e] = v[e];
-  __syncthreads();
-  const int x = threadIdx.x & 63, y = threadIdx.x >> 6;
-  u[y][x] = (t[4 * y][x] + t[4 * y + 1][x]) + (t[4 * y + 2][x] + t[4 * y + 3][x]);
-  __syncthreads();
-  if (y == 0 && blockIdx.x * 64 + x < C) {
-    float s = 0.f;
+  for (int o = 4; o < 64; o <<= 1)
 #pragma unroll
-    for (int k = 0; k < 16; ++k) s += u[k][x];
-    dw[blockIdx.x * 64 + x] = s;
+    for (int e = 0; e < 4; ++e) v[e] += __shfl_xor(v[e], o, 64);
+  if ((threadIdx.x & 63) < 4)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) t[threadIdx.x >> 6][q + e] = v[e];
+  __syncthreads();
+  if (threadIdx.x < 16 && blockIdx.x * 16 + threadIdx.x < C) {
+    float sum = 0.f;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) sum += t[k][threadIdx.x];
+    dw[blockIdx.x * 16 + threadIdx.x] = sum;
   }
 }
 
@@ -485,7 +483,7 @@ template <typename T, bool EVEN> int launch_bwd(const BwdArgs& a, float* dw, hip
   };
   const int rc = go();
   if (rc != TG_OK || !dw) return rc;
-  rms_dw_fold_kernel<<<(a.C + 63) / 64, 1024, 0, st>>>(a.partial, dw, grid, a.C);
+  rms_dw_fold_kernel<<<(a.C + 15) / 16, 1024, 0, st>>>(a.partial, dw, grid, a.C);
   return tg_launch_status();
 }
 
@@ -539,7 +537,7 @@ extern "C" int tg_rms_norm_bwd(int dtype, const void* dy, int64_t dy_stride, con
   const BwdArgs a{dy, x, res, ds, rstd, weight, dx, dweight ? scratch : nullptr, dy_stride, x_stride, res_stride, ds_stride, rows, C};
   hipStream_t st = (hipStream_t)stream;
   if (rows == 0) {   // the gradient of no rows
-    if (dweight) rms_dw_fold_kernel<<<(C + 63) / 64, 1024, 0, st>>>(nullptr, dweight, 0, C);
+    if (dweight) rms_dw_fold_kernel<<<(C + 15) / 16, 1024, 0, st>>>(nullptr, dweight, 0, C);
     return tg_launch_status();
   }
   if (!dy || !x || !rstd || !dx) return TG_E_BADARG;
