@@ -625,13 +625,18 @@ template <typename T, int MT, int CT, int NS, bool STATE> __global__ __launch_bo
   // this lane's piece of a row, its row of a load, and its place in one of a whole chunk's loads
   const int piece = lane % G::kLanes * 16, piece_c = lane % G::kCLanes * 16, row_a = lane / G::kLanes, row_c = lane / G::kCLanes;
   const bool live_a = piece < r.M * kBytes && row_a < C, live_c = w.slice * 16 * G::kCLanes + piece_c < N * kBytes && row_c < C;
-  const int up_a = reverse ? G::kRows - 1 - row_a : row_a, up_c = reverse ? G::kCRows - 1 - row_c : row_c;
-  const unsigned va = (unsigned)(up_a * ta + piece), vb = (unsigned)(up_a * tb + piece), vc = (unsigned)(up_c * tc + piece_c), vo = (unsigned)(up_c * to + piece_c);
-  // uniform: the lowest token of the next load of a, b, c, and of the next store of out; from load to load; back from a chunk's first load to its
-  // lowest token
+  // (lanes without a piece of their own bring another's again: a load for all lanes can stay in flight into the loop's registers, one for some is
+  // merged with the old values by copies that wait for it)
+  const int piece_r = live_a ? piece : 0, row_r = min(row_a, C - 1), piece_rc = live_c ? piece_c : 0, row_rc = min(row_c, C - 1);
+  const int up_a = reverse ? C - 1 - row_r : row_r, up_c = reverse ? C - 1 - row_rc : row_rc;   // from a chunk's lowest token
+  const unsigned va = (unsigned)(up_a * ta + piece_r), vb = (unsigned)(up_a * tb + piece_r), vc = (unsigned)(up_c * tc + piece_rc);
+  const unsigned vo = (unsigned)((reverse ? G::kCRows - 1 - row_c : row_c) * to + piece_c);
+  const int sign = reverse ? -1 : 1;
+  const unsigned la = (unsigned)(sign * G::kRows * ta), lb = (unsigned)(sign * G::kRows * tb), lc = (unsigned)(sign * G::kCRows * tc);   // from load to load
+  // uniform: the lowest token of the chunk in the registers, of a, b and c, from chunk to chunk; of the next store of out
   const char *ca = nullptr, *cb = nullptr, *cc = nullptr;
   char* co_at = nullptr;
-  const int64_t sign = reverse ? -1 : 1, da = sign * G::kRows * ta, db = sign * G::kRows * tb, dc = sign * G::kCRows * tc, d_out = sign * G::kCRows * to;
+  const int64_t da = (int64_t)sign * C * ta, db = (int64_t)sign * C * tb, dc = (int64_t)sign * C * tc, d_out = (int64_t)sign * G::kCRows * to;
   // a sequence's rows, and how far it is to the wave's next one
   const char *qa = reinterpret_cast<const char*>(r.a.p) + (w.bgroup * r.a.sb + (w.h / r.a.shared) * r.a.sh) * kBytes;
   const char *qb = reinterpret_cast<const char*>(r.b.p) + (w.bgroup * r.b.sb + (w.h / r.b.shared) * r.b.sh) * kBytes;
@@ -639,39 +644,43 @@ template <typename T, int MT, int CT, int NS, bool STATE> __global__ __launch_bo
   char* out = reinterpret_cast<char*>(r.out) + (int64_t)w.bgroup * p.T * to + (w.h / r.fold * N + w.slice * 16 * NS) * cols_bytes;
   const int64_t next_a = step * r.a.sb * kBytes, next_b = step * r.b.sb * kBytes, next_c = step * r.c.sb * kBytes, next_out = (int64_t)step * p.T * to;
   auto place = [&](int n) {   // at a sequence's first chunk
-    const int tok = reverse ? n - begin - G::kRows : begin, tok_c = reverse ? n - begin - G::kCRows : begin;
-    ca = qa + (int64_t)tok * ta;
-    cb = qb + (int64_t)tok * tb;
-    cc = qc + (int64_t)tok_c * tc;
+    const int64_t tok = reverse ? n - begin - C : begin;
+    ca = qa + tok * ta;
+    cb = qb + tok * tb;
+    cc = qc + tok * tc;
   };
   u32x4 fa[G::kLoads], fb[G::kLoads], fc[G::kCLoads];
-  auto fetch = [&](int cnt) {
+  auto fetch = [&](int cnt) {   // the chunk at ca, cb, cc; its tokens
+    unsigned oa[G::kLoads], ob[G::kLoads], oc[G::kCLoads];
     if (cnt >= C) {
-      if (live_a)
 #pragma unroll
-        for (int i = 0; i < G::kLoads; ++i) {
-          if (!STATE) fa[i] = *reinterpret_cast<const u32x4*>(ca + i * da + va);
-          fb[i] = *reinterpret_cast<const u32x4*>(cb + i * db + vb);
-        }
-      if (live_c)
+      for (int i = 0; i < G::kLoads; ++i) {
+        oa[i] = va + i * la;
+        ob[i] = vb + i * lb;
+      }
 #pragma unroll
-        for (int i = 0; i < G::kCLoads; ++i) fc[i] = *reinterpret_cast<const u32x4*>(cc + i * dc + vc);
-    } else {   // cnt tokens (behind the last one its row again: those scores lie above every valid token's diagonal and their weights in the state are 0)
-      auto at = [&](int row, int rows) { return (int64_t)(reverse ? rows - 1 - min(row, cnt - 1) : min(row, cnt - 1)); };
-      if (live_a)
+      for (int i = 0; i < G::kCLoads; ++i) oc[i] = vc + i * lc;
+    } else {   // (behind the last one its row again: those scores lie above every valid token's diagonal and their weights in the state are 0)
+      auto at = [&](int row) {
+        const int r = min(row, cnt - 1);
+        return (unsigned)(reverse ? C - 1 - r : r);
+      };
 #pragma unroll
-        for (int i = 0; i < G::kLoads; ++i) {
-          const int64_t row = at(i * G::kRows + row_a, G::kRows);
-          if (!STATE) fa[i] = *reinterpret_cast<const u32x4*>(ca + row * ta + piece);
-          fb[i] = *reinterpret_cast<const u32x4*>(cb + row * tb + piece);
-        }
-      if (live_c)
+      for (int i = 0; i < G::kLoads; ++i) {
+        const unsigned row = at(i * G::kRows + row_r);
+        oa[i] = row * ta + piece_r;
+        ob[i] = row * tb + piece_r;
+      }
 #pragma unroll
-        for (int i = 0; i < G::kCLoads; ++i) fc[i] = *reinterpret_cast<const u32x4*>(cc + at(i * G::kCRows + row_c, G::kCRows) * tc + piece_c);
+      for (int i = 0; i < G::kCLoads; ++i) oc[i] = at(i * G::kCRows + row_rc) * tc + piece_rc;
     }
-    ca += G::kLoads * da;
-    cb += G::kLoads * db;
-    cc += G::kCLoads * dc;
+#pragma unroll
+    for (int i = 0; i < G::kLoads; ++i) {
+      if (!STATE) fa[i] = *reinterpret_cast<const u32x4*>(ca + oa[i]);
+      fb[i] = *reinterpret_cast<const u32x4*>(cb + ob[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < G::kCLoads; ++i) fc[i] = *reinterpret_cast<const u32x4*>(cc + oc[i]);
   };
   // into the wave's LDS, which the wave alone reads (its LDS operations run in order).  Channels behind M and N were cleared once
   auto stage = [&]() {
@@ -694,10 +703,7 @@ template <typename T, int MT, int CT, int NS, bool STATE> __global__ __launch_bo
 
   auto length = [&](int bi) { return bi >= B ? 0 : p.lengths ? min(max(p.lengths[bi], 0), p.T) : p.T; };
   int n = length(w.bgroup), n_next = length(w.bgroup + step), turn = 0;
-  if (begin < n) {
-    place(n);
-    fetch(n - begin);
-  }
+  bool ready = false;   // the sequence's first chunk is on its way
   int64_t next0, next1;
   const float* s0 = w.template first_at<STATE>(p, r, &next0);
   float* s1 = w.template last_at<STATE>(p, r, &next1);
@@ -706,21 +712,32 @@ template <typename T, int MT, int CT, int NS, bool STATE> __global__ __launch_bo
     f32x4 S[NS][MT];
     w.load(r, s0, S);
     co_at = out + (int64_t)(reverse ? n - begin - G::kCRows : begin) * to;
-    auto next_sequence = [&]() {
-      qa += next_a;
-      qb += next_b;
-      qc += next_c;
-      if (begin < n_next) {
-        place(n_next);
-        fetch(n_next - begin);
-      }
-    };
-    if (begin >= n) next_sequence();
-    for (int t0 = begin; t0 < stop; t0 += C, ++turn) {
+    if (!ready && begin < n) {
+      place(n);
+      ca -= da;
+      cb -= db;
+      cc -= dc;
+    }
+    // a sequence whose first chunk is not there begins with a turn that only brings it: the loads stand in one place, where they stay in flight
+    int t0 = ready ? begin : begin - C;
+    ready = false;
+    qa += next_a;
+    qb += next_b;
+    qc += next_c;
+    for (; begin < n && t0 < stop; t0 += C) {
       const int cnt = min(C, stop - t0);
-      stage();
-      if (t0 + C < stop) fetch(stop - t0 - C);
-      else next_sequence();
+      if (t0 >= begin) stage();
+      if (t0 + C < stop) {
+        ca += da;
+        cb += db;
+        cc += dc;
+        fetch(stop - t0 - C);
+      } else {
+        ready = begin < n_next;
+        if (ready) place(n_next);
+        fetch(ready ? n_next - begin : cnt);   // (nothing to come: the same rows again)
+      }
+      if (t0 < begin) continue;
       f32x4 acc[NS][CT];
       Raw craw[NS][CT];
 #pragma unroll
@@ -820,7 +837,7 @@ template <typename T, int MT, int CT, int NS, bool STATE> __global__ __launch_bo
         }
       }
       if constexpr (!STATE) {
-        const bool writes = w.template fold<CT>(acc, sums, r.fold, turn);
+        const bool writes = w.template fold<CT>(acc, sums, r.fold, turn++);
         if (writes && cols_bytes == kBytes) {   // through c's place in the LDS: whole rows again, 16 bytes per lane
           wave_fence();
 #pragma unroll
