@@ -927,6 +927,9 @@ template <typename T, int MT> __global__ __launch_bounds__(256, 2) void la_short
 
   const int piece = lane % G::kLanes * 16, piece_c = lane % kBytes * 16, row_a = lane / G::kLanes, row_c = lane / kBytes;
   const bool live_a = piece < M * kBytes && row_a < 16, live_c = slice * 16 * kBytes + piece_c < N * kBytes && row_c < 16;
+  const int piece_r = live_a ? piece : 0, piece_rc = live_c ? piece_c : 0;   // (lanes without a piece bring another's again: see la_kernel)
+  constexpr bool kTogether = 16 * MT * kBytes < 128;   // (see la_kernel; 65536 sequences of 10 tokens, 4 heads of 16 channels: 149 us, 175 without.
+                                                       // The gradients in one pass have fewer waves and lose by it: 164 us, 160 without)
   // lengths, and what goes by them: the lanes' places in a sequence, the weights in the state, the rows of out
   auto length = [&](int bi) { return p.lengths ? min(max(p.lengths[bi], 0), Tn) : Tn; };
   unsigned oa[G::kLoads], ob[G::kLoads], oc;
@@ -938,23 +941,19 @@ template <typename T, int MT> __global__ __launch_bounds__(256, 2) void la_short
 #pragma unroll
     for (int i = 0; i < G::kLoads; ++i) {
       const int tok = token(i * G::kRows + row_a);
-      oa[i] = (unsigned)(tok * ta + piece);
-      ob[i] = (unsigned)(tok * tb + piece);
+      oa[i] = (unsigned)(tok * ta + piece_r);
+      ob[i] = (unsigned)(tok * tb + piece_r);
     }
-    oc = (unsigned)(token(row_c) * tc + piece_c);
+    oc = (unsigned)(token(row_c) * tc + piece_rc);
   };
   u32x4 fa[G::kLoads], fb[G::kLoads], fc;
   auto fetch = [&]() {
 #pragma unroll
-    for (int i = 0; i < G::kLoads; ++i) fa[i] = fb[i] = u32x4{0, 0, 0, 0};
-    fc = u32x4{0, 0, 0, 0};
-    if (live_a)
-#pragma unroll
-      for (int i = 0; i < G::kLoads; ++i) {
-        fa[i] = *reinterpret_cast<const u32x4*>(qa + oa[i]);
-        fb[i] = *reinterpret_cast<const u32x4*>(qb + ob[i]);
-      }
-    if (live_c) fc = *reinterpret_cast<const u32x4*>(qc + oc);
+    for (int i = 0; i < G::kLoads; ++i) {
+      fa[i] = *reinterpret_cast<const u32x4*>(qa + oa[i]);
+      fb[i] = *reinterpret_cast<const u32x4*>(qb + ob[i]);
+    }
+    fc = *reinterpret_cast<const u32x4*>(qc + oc);
   };
   auto columns = [&](const char* area, int row, int t) {
     if constexpr (kBytes == 2) {
@@ -988,6 +987,8 @@ template <typename T, int MT> __global__ __launch_bounds__(256, 2) void la_short
     }
   };
 
+  if (M != 16 * MT || N % 16 != 0)   // channels behind M and N
+    for (int i = lane * 16; i < G::kArea; i += 1024) *reinterpret_cast<u32x4*>(area_a + i) = u32x4{0, 0, 0, 0};
   int n = active && bgroup < B ? length(bgroup) : 0, placed = n, weighted = -1, turn = 0;
   places(n);
   if (n > 0) fetch();
@@ -1007,16 +1008,17 @@ template <typename T, int MT> __global__ __launch_bounds__(256, 2) void la_short
     if (n > 0) {   // into the wave's LDS
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       __builtin_amdgcn_wave_barrier();
-      if (row_a < 16)
+      if (live_a)
 #pragma unroll
         for (int i = 0; i < G::kLoads; ++i) {
           *reinterpret_cast<u32x4*>(area_a + (i * G::kRows + row_a) * G::kRow + piece) = fa[i];
           *reinterpret_cast<u32x4*>(area_b + (i * G::kRows + row_a) * G::kRow + piece) = fb[i];
         }
-      if (row_c < 16) *reinterpret_cast<u32x4*>(area_c + row_c * G::kCRow + piece_c) = fc;
+      if (live_c) *reinterpret_cast<u32x4*>(area_c + row_c * G::kCRow + piece_c) = fc;
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       __builtin_amdgcn_wave_barrier();
     }
+    if constexpr (kTogether) __builtin_amdgcn_s_barrier();
     int n_next = 0;
     if (active && bi + step < B) {
       qa += next_a;
@@ -1166,18 +1168,15 @@ template <typename T, int MT> __global__ __launch_bounds__(256, 2) void la_short
   }
   const int piece = lane % G::kLanes * 16, row = lane / G::kLanes;
   const bool live_k = piece < DK * kBytes && row < 16, live_v = piece < DV * kBytes && row < 16;
+  const int piece_k = live_k ? piece : 0, piece_v = live_v ? piece : 0;   // (lanes without a piece bring another's again: see la_kernel)
   auto length = [&](int bi) { return bi >= B ? 0 : p.lengths ? min(max(p.lengths[bi], 0), p.T) : p.T; };
   u32x4 in[4][G::kLoads];
   auto fetch = [&](int n) {
 #pragma unroll
     for (int i = 0; i < G::kLoads; ++i) {
       const int tok = min(i * G::kRows + row, n - 1);
-      if (live_k)
 #pragma unroll
-        for (int x = 0; x < 2; ++x) in[x][i] = *reinterpret_cast<const u32x4*>(at[x] + (unsigned)(tok * ts[x] + piece));
-      if (live_v)
-#pragma unroll
-        for (int x = 2; x < 4; ++x) in[x][i] = *reinterpret_cast<const u32x4*>(at[x] + (unsigned)(tok * ts[x] + piece));
+      for (int x = 0; x < 4; ++x) in[x][i] = *reinterpret_cast<const u32x4*>(at[x] + (unsigned)(tok * ts[x] + (x < 2 ? piece_k : piece_v)));
     }
   };
   auto rows = [&](int x, int t) { return *reinterpret_cast<const Raw*>(area + x * kRows16 + c * G::kRow + (16 * t + 4 * g) * kBytes); };
