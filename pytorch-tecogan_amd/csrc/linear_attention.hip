@@ -241,6 +241,7 @@ struct LaArgs {
   int group;               // waves of a workgroup that belong to one (stored head, slice)
   int columns, bgroups;    // blockIdx.x = bgroup * columns + column: workgroups over (stored head, slice), and over the sequences
   int seg, segments;       // tokens in a segment (a multiple of 32)
+  bool wide;               // (for the launch) slices of 32 columns where they can be
   float scale;
   Role r[3];
 };
@@ -1657,10 +1658,13 @@ template <typename T, int MT> int go_short(const LaArgs& a, dim3 grid, int threa
   static Resident resident;
   return go(la_short_kernel<T, MT>, resident, Stage<T, MT, 1>::kArea, 1, a.group > 1, a, grid, threads, st);
 }
-// Slices of 32 columns share a chunk's scores, its rows and the columns of b between two of 16 (16384 tokens of 64 channels: the gradients'
-// launch 61 us instead of 72).  For heads wider than 16 channels beside operands of 17 .. 64 in 16 bits; fp32 and 128 channels do not fit the
-// registers so
-inline int slice_tiles(int dtype, int M, int N) { return dtype != TG_F32 && N > 16 && (tiles(M) == 2 || tiles(M) == 4) ? 2 : 1; }
+// Slices of 32 columns share a chunk's scores, its rows and the columns of b between two of 16: worth it where half the waves still fill the
+// machine (128 sequences of 2000 tokens, 4 bf16 heads of 64: 151 us, 194 in slices of 16; gradients 408 us, 642), not where sequences are cut
+// into segments for want of waves (20 such sequences: 70 us, 53 in slices of 16; gradients 89 us, 81).  For heads wider than 16 channels beside
+// operands of 17 .. 64 in 16 bits; fp32 and 128 channels do not fit the registers so
+constexpr int64_t kWideWaves = 512;
+inline bool can_be_wide(int dtype, int M, int N) { return dtype != TG_F32 && N > 16 && (tiles(M) == 2 || tiles(M) == 4); }
+inline int slice_tiles(int dtype, int M, int N, bool wide) { return wide && can_be_wide(dtype, M, N) ? 2 : 1; }
 
 template <typename T, int MT> int go_mt(const LaArgs& a, bool staged, bool state, int ns, dim3 grid, int threads, hipStream_t st) {
   // chunks of 32 tokens halve the work on the state per token; sequences of one chunk of 16 would waste half of them, and two tiles of 128
@@ -1684,7 +1688,7 @@ template <typename T> int launch(LaArgs a, int dtype, int roles, bool state, hip
     const Role& r = a.r[i];
     if (tiles(r.M) > mt) mt = tiles(r.M);
     if (r.N > most) most = r.N;
-    if (slice_tiles(dtype, r.M, r.N) < ns) ns = slice_tiles(dtype, r.M, r.N);
+    if (slice_tiles(dtype, r.M, r.N, a.wide) < ns) ns = slice_tiles(dtype, r.M, r.N, a.wide);
     staged = staged && r.pieces;
   }
   if (!staged || (!state && a.T <= 16)) ns = 1;
@@ -1727,16 +1731,18 @@ int check(int dtype, const tg_la_desc* d) {
   return TG_OK;
 }
 
-inline int64_t slices_of(int dtype, int M, int N) {
-  const int n = 16 * slice_tiles(dtype, M, N);
+inline int64_t slices_of(int dtype, int M, int N, bool wide) {
+  const int n = 16 * slice_tiles(dtype, M, N, wide);
   return (N + n - 1) / n;
 }
-// segments of the forward pass (one role) and of the backward pass (three)
-void forward_segments(int dtype, const tg_la_desc* d, int* seg, int* segments) {
-  segmentation(d->T, (int64_t)d->B * d->H * slices_of(dtype, d->DK, d->DV), seg, segments);
-}
-void backward_segments(int dtype, const tg_la_desc* d, int* seg, int* segments) {
-  segmentation(d->T, (int64_t)d->B * d->H * (2 * slices_of(dtype, d->DV, d->DK) + slices_of(dtype, d->DK, d->DV)), seg, segments);
+// slices and segments of the forward pass (one role) and of the backward pass (three)
+void plan(int dtype, const tg_la_desc* d, bool backward, LaArgs* a) {
+  auto waves = [&](bool wide) {
+    const int64_t one = slices_of(dtype, d->DK, d->DV, wide);
+    return (int64_t)d->B * d->H * (backward ? one + 2 * slices_of(dtype, d->DV, d->DK, wide) : one);
+  };
+  a->wide = waves(true) >= kWideWaves;
+  segmentation(d->T, waves(a->wide), &a->seg, &a->segments);
 }
 inline int64_t states(const tg_la_desc* d) { return (int64_t)d->B * d->H * d->DK * d->DV; }
 inline int64_t fold_floats(const tg_la_desc* d) { return d->H / d->HK > kFold ? (int64_t)d->B * d->T * d->H * (d->DK + d->DV) : 0; }
@@ -1769,9 +1775,9 @@ template <typename T> int launch_step(const StepArgs& a, bool wide, hipStream_t 
 
 extern "C" int64_t tg_linear_attention_scratch_floats(int dtype, const tg_la_desc* d) {
   if (check(dtype, d) != TG_OK) return 0;
-  int seg, segments;
-  forward_segments(dtype, d, &seg, &segments);
-  return segments > 1 ? segments * states(d) : 0;
+  LaArgs a;
+  plan(dtype, d, false, &a);
+  return a.segments > 1 ? a.segments * states(d) : 0;
 }
 
 extern "C" int tg_linear_attention(int dtype, const tg_la_desc* d, const void* q, const void* k, const void* v, const float* log_decay,
@@ -1780,7 +1786,7 @@ extern "C" int tg_linear_attention(int dtype, const tg_la_desc* d, const void* q
   if (rc != TG_OK) return rc;
   if (d->B == 0) return TG_OK;
   LaArgs a{};
-  forward_segments(dtype, d, &a.seg, &a.segments);
+  plan(dtype, d, false, &a);
   if (!log_decay || !state_out || (d->T > 0 && (!q || !k || !v || !o)) || (a.segments > 1 && !scratch)) return TG_E_BADARG;
   if (!elem_aligned(dtype, q) || !elem_aligned(dtype, k) || !elem_aligned(dtype, v) || !elem_aligned(dtype, o) || !word_aligned(log_decay) ||
       !word_aligned(lengths) || !word_aligned(state_in) || !word_aligned(state_out) || !word_aligned(scratch))
@@ -1803,9 +1809,9 @@ extern "C" int tg_linear_attention(int dtype, const tg_la_desc* d, const void* q
 
 extern "C" int64_t tg_linear_attention_bwd_scratch_floats(int dtype, const tg_la_desc* d) {
   if (check(dtype, d) != TG_OK) return 0;
-  int seg, segments;
-  backward_segments(dtype, d, &seg, &segments);
-  return fold_floats(d) + (segments > 1 ? 2 * segments * states(d) : 0);
+  LaArgs a;
+  plan(dtype, d, true, &a);
+  return fold_floats(d) + (a.segments > 1 ? 2 * a.segments * states(d) : 0);
 }
 
 extern "C" int tg_linear_attention_bwd(int dtype, const tg_la_desc* d, const void* q, const void* k, const void* v, const void* dout,
@@ -1815,7 +1821,7 @@ extern "C" int tg_linear_attention_bwd(int dtype, const tg_la_desc* d, const voi
   if (rc != TG_OK) return rc;
   if (d->B == 0) return TG_OK;
   LaArgs a{};
-  backward_segments(dtype, d, &a.seg, &a.segments);
+  plan(dtype, d, true, &a);
   const int G = d->H / d->HK;
   if (!log_decay || !dout_stride || (d->T > 0 && (!q || !k || !v || !dout || !dq || !dk || !dv)) || (tg_linear_attention_bwd_scratch_floats(dtype, d) && !scratch))
     return TG_E_BADARG;

@@ -427,6 +427,16 @@ def test_attention_many_short_sequences():
     attention_case(300, 3, 4, 2, 16, 24, F32, lengths=[i % 4 for i in range(300)])
 
 
+@pytest.mark.parametrize("dt", [F32, BF16, F16])
+@pytest.mark.parametrize("DK,DV", [(64, 64), (32, 64), (40, 24), (48, 16)])
+def test_attention_many_wide_heads(DK, DV, dt):
+    """enough sequences for slices of 32 columns, whole and in segments"""
+    B = 600
+    attention_case(B, 70, 2, 1, DK, DV, dt, lengths=[(17 * i) % 71 for i in range(B)])
+    attention_case(150, 40, 4, 4, DK, DV, dt)
+    attention_case(66, 1100, 4, 4, DK, DV, dt, lengths=[1100 - (37 * i) % 1101 for i in range(66)])
+
+
 def test_attention_scale_and_extreme_decays():
     attention_case(2, 40, 3, 3, 24, 24, BF16, scale=1.0)
     q, k, v, do, state, dstate, _ = attention_inputs(2, 40, 3, 3, 24, 24, F32)
