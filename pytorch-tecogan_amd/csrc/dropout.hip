@@ -3,6 +3,8 @@
 // (i / 4 low, i / 4 high, layer, step) under the 64-bit key `seed`, kept if word >= threshold = round(p 2^32).  Forward and backward are the
 // same launch on other tensors.  (seed, step) are read from device memory, so a captured graph draws a new mask on every replay whose step
 // has moved.  The mask depends on the element's index alone, not on the element type or on how a launch is cut.
+// Bound by memory: 655360 x 64 bf16 elements with a residual, and the gradient, 84 us together, 420 MB at 5.0 TB/s (what a large copy reaches); eight
+// elements a lane are two 16-byte pieces at most and two generator blocks.
 #include "common.h"
 
 namespace {
