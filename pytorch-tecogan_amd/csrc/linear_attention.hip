@@ -1600,19 +1600,22 @@ constexpr int kFold = 4;   // shared heads that are summed inside a workgroup; m
 
 inline int tiles(int m) { return m <= 16 ? 1 : m <= 32 ? 2 : m <= 64 ? 4 : 8; }
 
-// Segments: as many as two waves per SIMD need, each of at least kMinSegment tokens.  The additional pass over b and c and the two launches cost
-// more than two segments bring at any length (64 sequences, 4 fp32 heads of 64: 300 tokens 48 us whole and 64 in two, 2000 tokens 284 and 304), and
-// three bring something for long sequences only (40 sequences: 300 tokens 45 us whole and 56 in three, 2000 tokens 278 and 210)
+// Segments: as many as two waves per SIMD need, each of at least kMinSegment tokens.  They cost an additional pass over b and c and two launches, about
+// what the whole sequence takes in 400 tokens of 16 bits or in 200 of fp32, and twice that where the machine is half full already: forward of two sequences,
+// 4 heads of 64, whole and in segments, bf16 300 tokens 17 us and 20, 700 tokens 30 and 19; fp32 200 tokens 25 and 19; of 20 sequences, bf16 700 tokens
+// 31 and 37, 1000 tokens 44 and 41; fp32 300 tokens 34 and 38, 520 tokens 53 and 46.  Two segments never bring anything (64 sequences of 2000 tokens,
+// fp32: 189 us whole and 215)
 constexpr int64_t kWaves = 2048;
 constexpr int kMinSegment = 32;
 constexpr int kCUs = 256;
 
 // (tokens in a segment, segments) for `waves` waves per segment
-void segmentation(int T, int64_t waves, int* seg, int* segments) {
+void segmentation(int dtype, int T, int64_t waves, int* seg, int* segments) {
   int64_t want = waves > 0 ? kWaves / waves : 1, most = (T + kMinSegment - 1) / kMinSegment;
   if (want > most) want = most;
   if (want > kMaxSegments) want = kMaxSegments;
-  if (want < (T < 1024 ? 4 : 3)) { *seg = (T + 31) / 32 * 32; *segments = 1; return; }
+  const int whole = (dtype == TG_F32 ? 256 : 512) * (want < 8 ? 2 : 1);
+  if (want < 3 || T < whole) { *seg = (T + 31) / 32 * 32; *segments = 1; return; }
   int64_t s = (T + want - 1) / want;
   s = (s + 31) / 32 * 32;
   *seg = (int)s;
@@ -1745,7 +1748,7 @@ void plan(int dtype, const tg_la_desc* d, bool backward, LaArgs* a) {
     return (int64_t)d->B * d->H * (backward ? one + 2 * slices_of(dtype, d->DV, d->DK, wide) : one);
   };
   a->wide = waves(true) >= kWideWaves;
-  segmentation(d->T, waves(a->wide), &a->seg, &a->segments);
+  segmentation(dtype, d->T, waves(a->wide), &a->seg, &a->segments);
 }
 inline int64_t states(const tg_la_desc* d) { return (int64_t)d->B * d->H * d->DK * d->DV; }
 inline int64_t fold_floats(const tg_la_desc* d) { return d->H / d->HK > kFold ? (int64_t)d->B * d->T * d->H * (d->DK + d->DV) : 0; }

@@ -422,6 +422,26 @@ def test_attention_long(B, T, H, D, dt):
     attention_case(B, T, H, H, D, D, dt)
 
 
+@pytest.mark.parametrize("dt", [F32, BF16, F16])
+@pytest.mark.parametrize("DK,DV", [(16, 16), (24, 40), (17, 31), (64, 128)])
+def test_attention_segments_of_ragged_batches(DK, DV, dt):
+    """lengths that end in the first segment, in a later one, at its border, at none"""
+    attention_case(4, 777, 4, 2, DK, DV, dt, lengths=[777, 300, 64, 0])
+    attention_case(1, 1029, 1, 1, DK, DV, dt, with_state=False)
+
+
+@pytest.mark.parametrize("dt", [F32, BF16, F16])
+def test_attention_nonfinite_tokens_across_segments(dt):
+    """the segments in front of an infinity give the same bits as without it; what follows is not finite"""
+    q, k, v, _, state, _, decay = attention_inputs(2, 640, 2, 2, 32, 32, dt)
+    o, last = ops.linear_attention(q, k, v, decay, state=state)
+    k[0, 333, 0, 5] = math.inf
+    o1, last1 = ops.linear_attention(q, k, v, decay, state=state)
+    assert torch.equal(o1[0, :333], o[0, :333]) and torch.equal(o1[1], o[1]) and torch.equal(o1[0, :, 1], o[0, :, 1])
+    assert torch.equal(last1[1], last[1]) and torch.equal(last1[0, 1], last[0, 1])
+    assert not o1[0, 333:, 0].isfinite().all(-1).any() and not last1[0, 0, 5].isfinite().any()
+
+
 def test_attention_many_short_sequences():
     attention_case(700, 10, 4, 4, 16, 16, BF16)
     attention_case(300, 3, 4, 2, 16, 24, F32, lengths=[i % 4 for i in range(300)])
