@@ -603,7 +603,7 @@ template <typename T, int MT, int CT, int NS = 1> struct Stage {
 // The staged form.  Addresses are a uniform pointer to the chunk's lowest token, which moves on by a constant, and every lane's own offset:
 // the loop holds no multiplication and no scalar load (with both, 187 scalar instructions and 7 loads stood beside 325 vector ones a chunk).
 // Measured: 65536 sequences of 120 tokens x 16 fp16 channels 224 - 233 us, 1.0 GB at 4.4 TB/s, bound by memory; two of 16384 tokens, 4 bf16 heads of
-// 64 channels: 23 us, the gradients 63 us, bound by issuing some 500 vector instructions a chunk at two waves per SIMD, whose registers are full.
+// 64 channels: 23 us, the gradients 63 us, bound by issuing some 500 vector instructions a chunk at two waves per SIMD, with no registers for a third.
 template <typename T, int MT, int CT, int NS, bool STATE> __global__ __launch_bounds__(256, 2) void la_kernel(LaArgs p) {
   typedef Mat<T> X;
   typedef Stage<T, MT, CT, NS> G;
@@ -1623,7 +1623,7 @@ void segmentation(int dtype, int T, int64_t waves, int* seg, int* segments) {
 }
 
 // One launch.  Sequences are dealt out so that the grid fills the machine ONCE (a wave makes its decay's powers once, and no second round of
-// workgroups finds the machine half empty: 4096 waves where 3072 fit ran 338 us, 3072 ran 274)
+// workgroups finds the machine half empty: a third more waves than fit ran 338 us, as many as fit 274)
 constexpr int kDevices = 16;
 struct Resident { std::atomic<int> n[kDevices][2][kFold + 1]; };   // a kernel's workgroups on a CU, by device, folds and waves; 0: not known yet
 int go(void (*kernel)(LaArgs), Resident& resident, int area, int ct, bool folds, LaArgs a, dim3 grid, int threads, hipStream_t st) {
