@@ -23,12 +23,11 @@
 // Long sequences: T is cut into segments of `seg` tokens so that a few heads fill the machine.  la_kernel with STATE sums each segment's own state,
 // la_scan_kernel joins them into the state in front of every segment, and the segments then run side by side.
 //
-// Rounding: raw inputs are multiplied as they are (exact products, fp32 sums).  Scores and state are fp32; as operands beside 16-bit
-// inputs they are split into TWO bf16 halves (hi + lo: 16 bits of mantissa) instead of one rounding to 8 bits - the products cost twice
-// the matrix instructions of a kernel that waits for memory, and the result is off by its own last rounding alone.  fp16 inputs are
-// split the same way beside them (exactly: 11 bits), because a score or a state may pass fp16's range.  What is ADDED to the state is
-// split into three (24 bits): the state leaves in fp32 and is as exact as one summed in fp32.  fp32 inputs run on the fp32 matrix
-// instructions.
+// Rounding: raw inputs are multiplied as they are (exact products, fp32 sums).  Scores, states and what is added to a state are fp32; as
+// operands beside 16-bit inputs they are split into THREE bf16 parts (hi + mid + lo: all 24 bits), so the products are those of fp32 and a result is off by
+// fp32 sums and its own last rounding.  (Two parts, 16 bits, were up to 14 % faster where instruction issue is the bound, and lost what neighbouring tokens
+// differ by: keys that differ by 2^-8 with opposite values, fp16 9e-4 off where 2.1e-4 is the type's own.)  fp16 inputs are split into two bf16 parts beside
+// them (exactly: 11 bits), because a score or a state may pass fp16's range.  fp32 inputs run on the fp32 matrix instructions.
 #include "common.h"
 
 namespace {
@@ -37,7 +36,7 @@ typedef __attribute__((ext_vector_type(8))) short s16x8;
 typedef __attribute__((ext_vector_type(4))) _Float16 f16x4;
 
 // ---- products of 16 x 16 tiles, summed dimension 16 (mma) or 32 (mma2: two tiles of each operand).  Raw: an input as loaded; Op: an input
-// beside a computed operand; Split / Split3: a computed operand
+// beside a computed operand; Split: a computed operand
 __device__ __forceinline__ f32x4 mma_bf16(s16x4 a, s16x4 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ s16x8 join(s16x4 a, s16x4 b) { return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); }
 __device__ __forceinline__ f32x4 mma2_bf16(s16x4 a0, s16x4 a1, s16x4 b0, s16x4 b1, f32x4 c) {
@@ -75,7 +74,6 @@ template <> struct Mat<F32> {
   typedef f32x4 Raw;
   typedef f32x4 Op;
   typedef f32x4 Split;
-  typedef f32x4 Split3;
   __device__ __forceinline__ static f32x4 mma(f32x4 a, f32x4 b, f32x4 c) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], b[e], c, 0, 0, 0);
@@ -86,16 +84,13 @@ template <> struct Mat<F32> {
   __device__ __forceinline__ static Op op(Raw v) { return v; }
   __device__ __forceinline__ static Op op_of(f32x4 v) { return v; }
   __device__ __forceinline__ static Split split(f32x4 v) { return v; }
-  __device__ __forceinline__ static Split3 split3(f32x4 v) { return v; }
   __device__ __forceinline__ static f32x4 raw(Raw a, Raw b, f32x4 c) { return mma(a, b, c); }
   __device__ __forceinline__ static f32x4 raw2(Raw a0, Raw a1, Raw b0, Raw b1, f32x4 c) { return mma(a1, b1, mma(a0, b0, c)); }
   __device__ __forceinline__ static f32x4 state(Split s, Op a, f32x4 c) { return mma(s, a, c); }
   __device__ __forceinline__ static f32x4 state2(Split s0, Split s1, Op a0, Op a1, f32x4 c) { return mma(s1, a1, mma(s0, a0, c)); }
-  __device__ __forceinline__ static f32x4 score(Op v, Split p, f32x4 c) { return mma(v, p, c); }
-  __device__ __forceinline__ static f32x4 score2(Op v0, Op v1, Split p0, Split p1, f32x4 c) { return mma(v1, p1, mma(v0, p0, c)); }
-  __device__ __forceinline__ static f32x4 add(Op b, Split3 w, f32x4 c) { return mma(b, w, c); }
-  __device__ __forceinline__ static f32x4 add2(Op b0, Op b1, Split3 w0, Split3 w1, f32x4 c) { return mma(b1, w1, mma(b0, w0, c)); }
-  template <int CT> __device__ __forceinline__ static f32x4 grown(f32x4 s, const Op* b, const Split3* w) {
+  __device__ __forceinline__ static f32x4 add(Op b, Split w, f32x4 c) { return mma(b, w, c); }
+  __device__ __forceinline__ static f32x4 add2(Op b0, Op b1, Split w0, Split w1, f32x4 c) { return mma(b1, w1, mma(b0, w0, c)); }
+  template <int CT> __device__ __forceinline__ static f32x4 grown(f32x4 s, const Op* b, const Split* w) {
     if constexpr (CT == 1) return add(b[0], w[0], s);
     else return add2(b[0], b[1], w[0], w[1], s);
   }
@@ -113,26 +108,24 @@ template <> struct Mat<F32> {
 template <> struct Mat<BF16> {
   typedef s16x4 Raw;
   typedef s16x4 Op;
-  typedef Halves Split;
-  typedef Thirds Split3;
+  typedef Thirds Split;
   __device__ __forceinline__ static Raw one(int d) { return Raw{(short)(d == 0 ? 0x3f80 : 0), (short)(d == 1 ? 0x3f80 : 0), (short)(d == 2 ? 0x3f80 : 0), (short)(d == 3 ? 0x3f80 : 0)}; }
   __device__ __forceinline__ static s16x4 to_out(f32x4 v) { return to_bf16(v); }
   __device__ __forceinline__ static f32x4 to_float(Raw v) { return from_bf16(v); }
   __device__ __forceinline__ static Op op(Raw v) { return v; }
   __device__ __forceinline__ static Op op_of(f32x4 v) { return to_bf16(v); }   // (of values that are bf16)
-  __device__ __forceinline__ static Split split(f32x4 v) { return halves(v); }
-  __device__ __forceinline__ static Split3 split3(f32x4 v) { return thirds(v); }
+  __device__ __forceinline__ static Split split(f32x4 v) { return thirds(v); }
   __device__ __forceinline__ static f32x4 raw(Raw a, Raw b, f32x4 c) { return mma_bf16(a, b, c); }
   __device__ __forceinline__ static f32x4 raw2(Raw a0, Raw a1, Raw b0, Raw b1, f32x4 c) { return mma2_bf16(a0, a1, b0, b1, c); }
-  __device__ __forceinline__ static f32x4 state(Split s, Op a, f32x4 c) { return mma_bf16(s.hi, a, mma_bf16(s.lo, a, c)); }
-  __device__ __forceinline__ static f32x4 state2(Split s0, Split s1, Op a0, Op a1, f32x4 c) { return mma2_bf16(s0.hi, s1.hi, a0, a1, mma2_bf16(s0.lo, s1.lo, a0, a1, c)); }
-  __device__ __forceinline__ static f32x4 score(Op v, Split p, f32x4 c) { return mma_bf16(v, p.hi, mma_bf16(v, p.lo, c)); }
-  __device__ __forceinline__ static f32x4 score2(Op v0, Op v1, Split p0, Split p1, f32x4 c) { return mma2_bf16(v0, v1, p0.hi, p1.hi, mma2_bf16(v0, v1, p0.lo, p1.lo, c)); }
-  __device__ __forceinline__ static f32x4 add(Op b, Split3 w, f32x4 c) { return mma_bf16(b, w.hi, mma_bf16(b, w.mid, mma_bf16(b, w.lo, c))); }
-  __device__ __forceinline__ static f32x4 add2(Op b0, Op b1, Split3 w0, Split3 w1, f32x4 c) {
+  __device__ __forceinline__ static f32x4 state(Split s, Op a, f32x4 c) { return mma_bf16(s.hi, a, mma_bf16(s.mid, a, mma_bf16(s.lo, a, c))); }
+  __device__ __forceinline__ static f32x4 state2(Split s0, Split s1, Op a0, Op a1, f32x4 c) {
+    return mma2_bf16(s0.hi, s1.hi, a0, a1, mma2_bf16(s0.mid, s1.mid, a0, a1, mma2_bf16(s0.lo, s1.lo, a0, a1, c)));
+  }
+  __device__ __forceinline__ static f32x4 add(Op b, Split w, f32x4 c) { return mma_bf16(b, w.hi, mma_bf16(b, w.mid, mma_bf16(b, w.lo, c))); }
+  __device__ __forceinline__ static f32x4 add2(Op b0, Op b1, Split w0, Split w1, f32x4 c) {
     return mma2_bf16(b0, b1, w0.hi, w1.hi, mma2_bf16(b0, b1, w0.mid, w1.mid, mma2_bf16(b0, b1, w0.lo, w1.lo, c)));
   }
-  template <int CT> __device__ __forceinline__ static f32x4 grown(f32x4 s, const Op* b, const Split3* w) {
+  template <int CT> __device__ __forceinline__ static f32x4 grown(f32x4 s, const Op* b, const Split* w) {
     if constexpr (CT == 1) return add(b[0], w[0], s);
     else return add2(b[0], b[1], w[0], w[1], s);
   }
@@ -150,39 +143,41 @@ template <> struct Mat<BF16> {
 template <> struct Mat<F16> {
   typedef s16x4 Raw;
   typedef Halves Op;
-  typedef Halves Split;
-  typedef Thirds Split3;
+  typedef Thirds Split;
   __device__ __forceinline__ static Raw one(int d) { return Raw{(short)(d == 0 ? 0x3c00 : 0), (short)(d == 1 ? 0x3c00 : 0), (short)(d == 2 ? 0x3c00 : 0), (short)(d == 3 ? 0x3c00 : 0)}; }
   __device__ __forceinline__ static s16x4 to_out(f32x4 v) { return __builtin_bit_cast(s16x4, __builtin_convertvector(v, f16x4)); }
   __device__ __forceinline__ static f32x4 to_float(Raw v) { return __builtin_convertvector(__builtin_bit_cast(f16x4, v), f32x4); }
   __device__ __forceinline__ static Op op(Raw v) { return halves(to_float(v)); }
   __device__ __forceinline__ static Op op_of(f32x4 v) { return halves(v); }
-  __device__ __forceinline__ static Split split(f32x4 v) { return halves(v); }
-  __device__ __forceinline__ static Split3 split3(f32x4 v) { return thirds(v); }
+  __device__ __forceinline__ static Split split(f32x4 v) { return thirds(v); }
   __device__ __forceinline__ static f32x4 raw(Raw a, Raw b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(f16x4, a), __builtin_bit_cast(f16x4, b), c, 0, 0, 0);
   }
   __device__ __forceinline__ static f32x4 raw2(Raw a0, Raw a1, Raw b0, Raw b1, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, join(a0, a1)), __builtin_bit_cast(f16x8, join(b0, b1)), c, 0, 0, 0);
   }
-  // (lo * lo: below 16 bits of the product, and 24 of the state's increment, respectively)
-  __device__ __forceinline__ static f32x4 state(Split s, Op a, f32x4 c) { return mma_bf16(s.hi, a.hi, mma_bf16(s.hi, a.lo, mma_bf16(s.lo, a.hi, c))); }
-  __device__ __forceinline__ static f32x4 state2(Split s0, Split s1, Op a0, Op a1, f32x4 c) {
-    return mma2_bf16(s0.hi, s1.hi, a0.hi, a1.hi, mma2_bf16(s0.hi, s1.hi, a0.lo, a1.lo, mma2_bf16(s0.lo, s1.lo, a0.hi, a1.hi, c)));
+  // (lo * lo: 2^-9 of the input by 2^-18 of the operand, below 24 bits of the product)
+  __device__ __forceinline__ static f32x4 state(Split s, Op a, f32x4 c) {
+    return mma_bf16(s.hi, a.hi, mma_bf16(s.mid, a.hi, mma_bf16(s.hi, a.lo, mma_bf16(s.lo, a.hi, mma_bf16(s.mid, a.lo, c)))));
   }
-  __device__ __forceinline__ static f32x4 score(Op v, Split p, f32x4 c) { return state(v, p, c); }
-  __device__ __forceinline__ static f32x4 score2(Op v0, Op v1, Split p0, Split p1, f32x4 c) { return state2(v0, v1, p0, p1, c); }
-  __device__ __forceinline__ static f32x4 add(Op b, Split3 w, f32x4 c) {
+  __device__ __forceinline__ static f32x4 state2(Split s0, Split s1, Op a0, Op a1, f32x4 c) {
+    c = mma2_bf16(s0.mid, s1.mid, a0.lo, a1.lo, c);
+    c = mma2_bf16(s0.lo, s1.lo, a0.hi, a1.hi, c);
+    c = mma2_bf16(s0.hi, s1.hi, a0.lo, a1.lo, c);
+    c = mma2_bf16(s0.mid, s1.mid, a0.hi, a1.hi, c);
+    return mma2_bf16(s0.hi, s1.hi, a0.hi, a1.hi, c);
+  }
+  __device__ __forceinline__ static f32x4 add(Op b, Split w, f32x4 c) {
     return mma_bf16(b.hi, w.hi, mma_bf16(b.hi, w.mid, mma_bf16(b.lo, w.hi, mma_bf16(b.hi, w.lo, mma_bf16(b.lo, w.mid, c)))));
   }
-  __device__ __forceinline__ static f32x4 add2(Op b0, Op b1, Split3 w0, Split3 w1, f32x4 c) {
+  __device__ __forceinline__ static f32x4 add2(Op b0, Op b1, Split w0, Split w1, f32x4 c) {
     c = mma2_bf16(b0.lo, b1.lo, w0.mid, w1.mid, c);
     c = mma2_bf16(b0.hi, b1.hi, w0.lo, w1.lo, c);
     c = mma2_bf16(b0.lo, b1.lo, w0.hi, w1.hi, c);
     c = mma2_bf16(b0.hi, b1.hi, w0.mid, w1.mid, c);
     return mma2_bf16(b0.hi, b1.hi, w0.hi, w1.hi, c);
   }
-  template <int CT> __device__ __forceinline__ static f32x4 grown(f32x4 s, const Op* b, const Split3* w) {
+  template <int CT> __device__ __forceinline__ static f32x4 grown(f32x4 s, const Op* b, const Split* w) {
     if constexpr (CT == 1) return add(b[0], w[0], s);
     else return add2(b[0], b[1], w[0], w[1], s);
   }
@@ -428,8 +423,8 @@ __device__ __forceinline__ void weighted_sum(f32x4* acc, const typename Mat<T>::
 #pragma unroll
     for (int e = 0; e < 4; ++e) top = __builtin_elementwise_maximum(top, __builtin_fabsf(cf[t][e]));   // (a NaN stays)
   auto inner = [&](int it, typename X::Op last, f32x4 y) {
-    if constexpr (CT == 1) return X::score(last, ps[0][0], y);
-    else return it == 0 ? X::score(last, ps[0][0], y) : X::score2(co[0], last, ps[0][1], ps[1][1], y);
+    if constexpr (CT == 1) return X::add(last, ps[0][0], y);
+    else return it == 0 ? X::add(last, ps[0][0], y) : X::add2(co[0], last, ps[0][1], ps[1][1], y);
   };
   if (__builtin_expect(__any(!(top <= 3.4028234e38f)), 0)) {
 #pragma unroll
@@ -542,9 +537,9 @@ template <typename T, int MT, int CT, bool STATE> __global__ __launch_bounds__(2
           weighted_sum<T, CT>(acc, ps, co, cf, c, g);
         }
         k.length(w.decay, cnt, g, r.zs, r.sh);
-        typename X::Split3 ws[CT];
+        typename X::Split ws[CT];
 #pragma unroll
-        for (int t = 0; t < CT; ++t) ws[t] = X::split3(cf[t] * k.into(cnt, t));
+        for (int t = 0; t < CT; ++t) ws[t] = X::split(cf[t] * k.into(cnt, t));
 #pragma unroll
         for (int t = 0; t < MT; ++t) {
           Op b[CT];
@@ -829,11 +824,11 @@ template <typename T, int MT, int CT, int NS, bool STATE> __global__ __launch_bo
       }
       if (s1 || t0 + C < stop) {   // (nothing is added to a state that nobody reads)
         k.length(w.decay, cnt, g, r.zs, r.sh);
-        typename X::Split3 ws[NS][CT];
+        typename X::Split ws[NS][CT];
 #pragma unroll
         for (int s = 0; s < NS; ++s)
 #pragma unroll
-          for (int t = 0; t < CT; ++t) ws[s][t] = X::split3(X::to_float(craw[s][t]) * k.into(cnt, t));
+          for (int t = 0; t < CT; ++t) ws[s][t] = X::split(X::to_float(craw[s][t]) * k.into(cnt, t));
 #pragma unroll
         for (int t = 0; t < MT; ++t) {
           Op b[CT];
@@ -1068,18 +1063,18 @@ template <typename T, int MT> __global__ __launch_bounds__(256, 2) void la_short
         const f32x4 before = acc;
 #pragma unroll 1
         for (int i = 0; i < 16; ++i) {
-          const f32x4 y = X::score(X::upto(co, i + 1 - 4 * g), ps, before);
+          const f32x4 y = X::add(X::upto(co, i + 1 - 4 * g), ps, before);
           if (c == i) acc = y;
         }
       } else {
-        acc = X::score(co, ps, acc);
+        acc = X::add(co, ps, acc);
       }
       if (s1) {
         if (n != weighted) {
           weighted = n;
           weights(n);
         }
-        const typename X::Split3 ws = X::split3(cf * into);
+        const typename X::Split ws = X::split(cf * into);
 #pragma unroll
         for (int t = 0; t < MT; ++t) {
           f32x4 v = zero;
@@ -1137,8 +1132,9 @@ template <typename T, int MT> __global__ __launch_bounds__(256, 2) void la_short
 
 // The three gradients of such sequences in one pass: a wave brings q, k, v and do once instead of nine rows' worth for three roles, and takes one
 // slice of dq, dk and dv from them, tokens in their own order (23 us as three roles of la_short_kernel, 15.6 so, for 16384 sequences of 10 tokens x
-// 16 channels).  p.r[] are the roles of the general form.
-template <typename T, int MT> __global__ __launch_bounds__(256, 2) void la_short_grad_kernel(LaArgs p) {
+// 16 channels).  p.r[] are the roles of the general form.  Heads of up to 16 channels are held to the registers of four waves per SIMD, which they fit
+// (16384 sequences, 4 heads, bf16: forward and this 138 us, 173 with the 171 registers and two waves that the compiler takes by itself).
+template <typename T, int MT> __global__ __launch_bounds__(256, MT == 1 ? 4 : 2) void la_short_grad_kernel(LaArgs p) {
   typedef Mat<T> X;
   typedef Stage<T, MT, 1> G;
   typedef typename X::Raw Raw;
@@ -1240,12 +1236,12 @@ template <typename T, int MT> __global__ __launch_bounds__(256, 2) void la_short
       const f32x4 before = acc;
 #pragma unroll 1
       for (int i = 0; i < 16; ++i) {
-        const f32x4 y = X::score(later ? X::behind(co, i - 4 * g) : X::upto(co, i + 1 - 4 * g), ps, before);
+        const f32x4 y = X::add(later ? X::behind(co, i - 4 * g) : X::upto(co, i + 1 - 4 * g), ps, before);
         if (c == i) acc = y;
       }
       return acc;
     }
-    return X::score(co, ps, acc);
+    return X::add(co, ps, acc);
   };
 
   int n = length(bgroup), n_next = length(bgroup + step), turn = 0;
@@ -1332,7 +1328,7 @@ template <typename T, int MT> __global__ __launch_bounds__(256, 2) void la_short
         f32x4 w = X::to_float(cols(3, slice));
 #pragma unroll
         for (int e = 0; e < 4; ++e) w[e] = 4 * g + e < n ? w[e] * into[e] : 0.f;
-        const typename X::Split3 ws = X::split3(w);
+        const typename X::Split ws = X::split(w);
 #pragma unroll
         for (int t = 0; t < MT; ++t) {
 #pragma unroll

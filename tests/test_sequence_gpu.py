@@ -664,6 +664,72 @@ def test_attention_in_pieces():
     close(d, want["dstate"], F32, mag["dstate"], units, "dstate")
 
 
+# ------------------------------------------------------------------------- scores, states and decays at fp32's own precision
+# what each result sums, sum_j (a_i . b_j) c_j and a_i S: the names of a, b, c and of the state
+ROLES = {"o": ("q", "k", "v", "state"), "dq": ("do", "v", "k", "state"), "dk": ("v", "do", "q", "dstate"), "dv": ("k", "q", "do", "dstate")}
+EXACT_SHAPES = [(2, 16, 16), (9, 16, 24), (16, 32, 16), (16, 64, 64), (12, 128, 128), (14, 17, 9), (33, 16, 16), (40, 32, 32), (70, 64, 64), (50, 40, 24),
+                (48, 128, 128), (61, 19, 33), (30, 65, 97), (1040, 64, 64), (1100, 21, 16)]
+
+
+def exact_run(name, x, scale):
+    """result `name` of the operands x, memory that does not fade"""
+    decay = torch.zeros(x["q"].shape[2], device=DEV)
+    x = {n: None if t is None else t.to(DEV) for n, t in x.items()}
+    if name == "o":
+        got = ops.linear_attention(x["q"], x["k"], x["v"], decay, scale=scale, state=x["state"])[0]
+    else:
+        got = ops.linear_attention_backward(x["do"], x["q"], x["k"], x["v"], decay, scale=scale, state=x["state"], dstate=x["dstate"])[("dq", "dk", "dv").index(name)]
+    want, mag = attention_oracle(x["q"], x["k"], x["v"], decay, scale, x["state"], None, x["do"], x["dstate"])
+    # the premise: whole numbers of units of `scale` that fp32 adds in any order
+    assert float(mag[name].max()) < 2.0 ** 24 * scale and float(want[name].abs().max()) < 60000
+    want = want[name].to(got.dtype).double()
+    off = got.double().cpu() != want
+    assert not off.any(), (name, int(off.sum()), float((got.double().cpu() - want).abs().max()))
+
+
+@pytest.mark.parametrize("dt", [F32, BF16, F16])
+@pytest.mark.parametrize("T,DK,DV", EXACT_SHAPES)
+def test_attention_scores_that_cancel(T, DK, DV, dt):
+    """Neighbouring tokens b, b' that differ in the last places, with c' = -c: the scores are whole numbers below 2^20, their sums exact in fp32 in any
+    order, and the results (small whole numbers, times a power of two) carry no rounding but their own.  Scores held to 16 bits are off by up
+    to 8, more than most results."""
+    for name, (a, b, c, _) in ROLES.items():
+        g = torch.Generator().manual_seed(T)
+        pick = lambda lo, hi, *s: torch.randint(lo, hi + 1, s, generator=g).to(F32)   # noqa: E731
+        x = {n: torch.zeros(1, T, 2, DK if n in ("q", "k") else DV) for n in ("q", "k", "v", "do")}
+        wide = x[a].shape[-1]
+        for m, w in ((wide - 1, 2.0 ** 4), (wide // 2, 2.0 ** 2), (0, 1.0)):   # a b = 2^14 r + 2^7 r' + r''
+            x[a][..., m] = w
+        x[a] *= 2 * pick(0, 1, 1, T, 2, 1) - 1
+        for at in sorted({0, T // 4 * 2, (T - 2) // 2 * 2}):
+            for m, w in ((wide - 1, 2.0 ** 10), (wide // 2, 2.0 ** 5), (0, 1.0)):
+                x[b][0, at, :, m] = x[b][0, at + 1, :, m] = w * pick(1, 31, 2)
+            x[b][0, at + 1, :, 0] += pick(1, 3, 2)
+            x[c][0, at] = pick(1, 2, *x[c].shape[2:])
+            x[c][0, at + 1] = -x[c][0, at]
+        y = {n: t.to(dt) for n, t in x.items()}
+        assert all(torch.equal(y[n].float(), x[n]) for n in x)
+        exact_run(name, dict(y, state=None, dstate=None), 2.0 ** -6)
+
+
+@pytest.mark.parametrize("dt", [F32, BF16, F16])
+@pytest.mark.parametrize("T,DK,DV", EXACT_SHAPES)
+def test_attention_states_that_cancel(T, DK, DV, dt):
+    """differences of neighbouring rows of a state of whole numbers below 2^22: small whole numbers, exact in fp32"""
+    for name, (a, _, _, s) in ROLES.items():
+        g = torch.Generator().manual_seed(T + 1)
+        pick = lambda lo, hi, *s: torch.randint(lo, hi + 1, s, generator=g).to(F32)   # noqa: E731
+        x = {n: torch.zeros(1, T, 2, DK if n in ("q", "k") else DV, dtype=dt) for n in ("q", "k", "v", "do")}
+        x[a][..., 0], x[a][..., x[a].shape[-1] - 1] = 1, -1
+        x[a] *= (2 * pick(0, 1, 1, T, 2, 1) - 1).to(dt)
+        state = pick(1 << 20, 1 << 22, 1, 2, DK, DV)
+        if x[a].shape[-1] == DK and a in ("q", "k"):
+            state[:, :, -1] = state[:, :, 0] + pick(-3, 3, 1, 2, DV)
+        else:
+            state[..., -1] = state[..., 0] + pick(-3, 3, 1, 2, DK)
+        exact_run(name, dict(x, state=state if s == "state" else torch.zeros_like(state), dstate=state if s == "dstate" else torch.zeros_like(state)), 1.0)
+
+
 # ------------------------------------------------------------------------------------- streams, graphs, refusals, together
 def all_operators(x, w, rng, q, k, v, decay, state, out):
     """every operator once into the dict `out` (explicit forms, as a captured step calls them)"""
