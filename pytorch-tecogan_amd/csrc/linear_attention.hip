@@ -79,10 +79,8 @@ template <> struct Mat<F32> {
     for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], b[e], c, 0, 0, 0);
     return c;
   }
-  __device__ __forceinline__ static Raw one(int d) { return Raw{d == 0 ? 1.f : 0.f, d == 1 ? 1.f : 0.f, d == 2 ? 1.f : 0.f, d == 3 ? 1.f : 0.f}; }
   __device__ __forceinline__ static f32x4 to_float(Raw v) { return v; }
   __device__ __forceinline__ static Op op(Raw v) { return v; }
-  __device__ __forceinline__ static Op op_of(f32x4 v) { return v; }
   __device__ __forceinline__ static Split split(f32x4 v) { return v; }
   __device__ __forceinline__ static f32x4 raw(Raw a, Raw b, f32x4 c) { return mma(a, b, c); }
   __device__ __forceinline__ static f32x4 raw2(Raw a0, Raw a1, Raw b0, Raw b1, f32x4 c) { return mma(a1, b1, mma(a0, b0, c)); }
@@ -109,11 +107,9 @@ template <> struct Mat<BF16> {
   typedef s16x4 Raw;
   typedef s16x4 Op;
   typedef Thirds Split;
-  __device__ __forceinline__ static Raw one(int d) { return Raw{(short)(d == 0 ? 0x3f80 : 0), (short)(d == 1 ? 0x3f80 : 0), (short)(d == 2 ? 0x3f80 : 0), (short)(d == 3 ? 0x3f80 : 0)}; }
   __device__ __forceinline__ static s16x4 to_out(f32x4 v) { return to_bf16(v); }
   __device__ __forceinline__ static f32x4 to_float(Raw v) { return from_bf16(v); }
   __device__ __forceinline__ static Op op(Raw v) { return v; }
-  __device__ __forceinline__ static Op op_of(f32x4 v) { return to_bf16(v); }   // (of values that are bf16)
   __device__ __forceinline__ static Split split(f32x4 v) { return thirds(v); }
   __device__ __forceinline__ static f32x4 raw(Raw a, Raw b, f32x4 c) { return mma_bf16(a, b, c); }
   __device__ __forceinline__ static f32x4 raw2(Raw a0, Raw a1, Raw b0, Raw b1, f32x4 c) { return mma2_bf16(a0, a1, b0, b1, c); }
@@ -144,11 +140,9 @@ template <> struct Mat<F16> {
   typedef s16x4 Raw;
   typedef Halves Op;
   typedef Thirds Split;
-  __device__ __forceinline__ static Raw one(int d) { return Raw{(short)(d == 0 ? 0x3c00 : 0), (short)(d == 1 ? 0x3c00 : 0), (short)(d == 2 ? 0x3c00 : 0), (short)(d == 3 ? 0x3c00 : 0)}; }
   __device__ __forceinline__ static s16x4 to_out(f32x4 v) { return __builtin_bit_cast(s16x4, __builtin_convertvector(v, f16x4)); }
   __device__ __forceinline__ static f32x4 to_float(Raw v) { return __builtin_convertvector(__builtin_bit_cast(f16x4, v), f32x4); }
   __device__ __forceinline__ static Op op(Raw v) { return halves(to_float(v)); }
-  __device__ __forceinline__ static Op op_of(f32x4 v) { return halves(v); }
   __device__ __forceinline__ static Split split(f32x4 v) { return thirds(v); }
   __device__ __forceinline__ static f32x4 raw(Raw a, Raw b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(f16x4, a), __builtin_bit_cast(f16x4, b), c, 0, 0, 0);
@@ -455,26 +449,33 @@ template <typename T> __device__ __forceinline__ typename Mat<T>::Raw columns(co
   }
 }
 
-// Operands that are not aligned to 16 bytes, or whose channels do not fill them: every lane loads its tiles' elements itself.
+// Operands that are not aligned to 16 bytes, or whose channels do not fill them: every lane loads its tiles' elements itself.  Columns (of b and
+// c) come from the wave's own part of the LDS, never out of a product with the identity, which would spread one channel's infinity over a tile.
+template <typename T, int MT, int CT> struct Turn {
+  static constexpr int kRow = 16 * MT * ElemTraits<T>::kBytes + 16, kCRow = 16 * ElemTraits<T>::kBytes + 16;   // bytes between rows (see Stage)
+  static constexpr int kArea = 16 * CT * (kRow + kCRow);
+};
 template <typename T, int MT, int CT, bool STATE> __global__ __launch_bounds__(256, 2) void la_plain_kernel(LaArgs p) {
   typedef Mat<T> X;
+  typedef Turn<T, MT, CT> G;
   typedef typename X::Raw Raw;
   typedef typename X::Op Op;
   constexpr int kBytes = ElemTraits<T>::kBytes;
   constexpr int C = 16 * CT;
   constexpr f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-  extern __shared__ __align__(16) char lds[];           // [2][waves][CT][64] sums of 4 floats if a role folds
+  extern __shared__ __align__(16) char lds[];           // [waves][kArea], then [2][waves][CT][64] sums of 4 floats if a role folds
   const Wave<T, MT> w(p);
   const Role& r = p.r[blockIdx.y];
-  const int lane = w.lane, c = w.c, g = w.g;
+  const int c = w.c, g = w.g;
   const int begin = blockIdx.z * p.seg, end = min(begin + p.seg, p.T);
   const char* pa = reinterpret_cast<const char*>(r.a.p) + (w.h / r.a.shared) * r.a.sh * kBytes;
   const char* pb = reinterpret_cast<const char*>(r.b.p) + (w.h / r.b.shared) * r.b.sh * kBytes;
   const char* pc = reinterpret_cast<const char*>(r.c.p) + ((w.h / r.c.shared) * r.c.sh + w.slice * 16) * kBytes;
   const int n0 = w.slice * 16 + 4 * g;                  // this lane's 4 columns of c's rows and of out
   const int row_out = p.H / r.fold * r.N, out_bytes = r.out_f32 ? 4 : kBytes;
-  const Raw unit = X::one(c - 4 * g);
-  f32x4* const sums = reinterpret_cast<f32x4*>(lds);
+  char* const area_b = lds + w.wave * G::kArea;
+  char* const area_c = area_b + C * G::kRow;
+  f32x4* const sums = reinterpret_cast<f32x4*>(lds + w.waves * G::kArea);
   Weights<CT> k(w.decay, c, g, p.scale, r.za, r.zs, r.sh);
   int64_t next0, next1;
   const float* s0 = w.template first_at<STATE>(p, r, &next0);
@@ -492,7 +493,7 @@ template <typename T, int MT, int CT, bool STATE> __global__ __launch_bounds__(2
       for (int t = 0; t < CT; ++t) acc[t] = zero;
       if (cnt > 0) {
         // (behind the last token its row again: those scores lie above every valid token's diagonal and their weights in the state are 0)
-        Raw av[CT][MT], bv[CT][MT];
+        Raw av[CT][MT], bv[CT][MT], craw[CT];
         f32x4 cf[CT];
 #pragma unroll
         for (int it = 0; it < CT; ++it) {
@@ -504,8 +505,21 @@ template <typename T, int MT, int CT, bool STATE> __global__ __launch_bounds__(2
             if (!STATE) av[it][t] = load4<T>(qa + (tok * r.a.st + m) * kBytes, r.M - m, r.wide);
             bv[it][t] = load4<T>(qb + (tok * r.b.st + m) * kBytes, r.M - m, r.wide);
           }
-          // by columns: a product with the identity turns a tile (exactly)
-          cf[it] = X::raw(load4<T>(qc + (tok * r.c.st + 4 * g) * kBytes, r.N - n0, r.wide), unit, zero);
+          craw[it] = load4<T>(qc + (tok * r.c.st + 4 * g) * kBytes, r.N - n0, r.wide);
+        }
+        wave_fence();
+#pragma unroll
+        for (int it = 0; it < CT; ++it) {
+          char* const row = area_b + (16 * it + c) * G::kRow + 4 * g * kBytes;
+#pragma unroll
+          for (int t = 0; t < MT; ++t) *reinterpret_cast<Raw*>(row + 16 * t * kBytes) = bv[it][t];
+          *reinterpret_cast<Raw*>(area_c + (16 * it + c) * G::kCRow + 4 * g * kBytes) = craw[it];
+        }
+        wave_fence();
+#pragma unroll
+        for (int it = 0; it < CT; ++it) {
+          craw[it] = columns<T>(area_c, G::kCRow, 16 * it, 0, c, g);
+          cf[it] = X::to_float(craw[it]);
         }
         if constexpr (!STATE) {
           typename X::Split ps[CT][CT];
@@ -533,7 +547,7 @@ template <typename T, int MT, int CT, bool STATE> __global__ __launch_bounds__(2
           }
           Op co[CT];
 #pragma unroll
-          for (int t = 0; t < CT; ++t) co[t] = X::op_of(cf[t]);
+          for (int t = 0; t < CT; ++t) co[t] = X::op(craw[t]);
           weighted_sum<T, CT>(acc, ps, co, cf, c, g);
         }
         k.length(w.decay, cnt, g, r.zs, r.sh);
@@ -544,7 +558,7 @@ template <typename T, int MT, int CT, bool STATE> __global__ __launch_bounds__(2
         for (int t = 0; t < MT; ++t) {
           Op b[CT];
 #pragma unroll
-          for (int jt = 0; jt < CT; ++jt) b[jt] = X::op_of(X::raw(bv[jt][t], unit, zero));
+          for (int jt = 0; jt < CT; ++jt) b[jt] = X::op(columns<T>(area_b, G::kRow, 16 * jt, t, c, g));
           S[t] = X::template grown<CT>(k.kept(S[t], cnt), b, ws);
         }
       }
@@ -1647,7 +1661,7 @@ template <typename T, int MT, int CT, int NS, bool STATE> int go_long(const LaAr
 }
 template <typename T, int MT, int CT, bool STATE> int go_plain(const LaArgs& a, dim3 grid, int threads, hipStream_t st) {
   static Resident resident;
-  return go(la_plain_kernel<T, MT, CT, STATE>, resident, 0, CT, !STATE && a.group > 1, a, grid, threads, st);
+  return go(la_plain_kernel<T, MT, CT, STATE>, resident, Turn<T, MT, CT>::kArea, CT, !STATE && a.group > 1, a, grid, threads, st);
 }
 template <typename T, int MT> int go_short(const LaArgs& a, dim3 grid, int threads, hipStream_t st) {
   if constexpr (MT < 8) {   // (128 channels: three roles, their registers do not fit one wave)

@@ -730,6 +730,41 @@ def test_attention_states_that_cancel(T, DK, DV, dt):
         exact_run(name, dict(x, state=state if s == "state" else torch.zeros_like(state), dstate=state if s == "dstate" else torch.zeros_like(state)), 1.0)
 
 
+@pytest.mark.parametrize("dt", [F32, BF16, F16])
+@pytest.mark.parametrize("value", [math.inf, math.nan])
+@pytest.mark.parametrize("T,D,off", [(10, 16, 0), (10, 17, 0), (40, 17, 0), (40, 32, 1), (150, 64, 0), (150, 63, 0), (40, 127, 0), (1100, 33, 0)])
+def test_attention_nonfinite_channels_reach_no_other_channel(T, D, off, value, dt):
+    """One channel of one token is not finite: an infinite v makes one column of o, of the state; an infinite k one row of the state and one
+    channel of dq; q and do likewise in dk, dv and the state's gradient.  All others keep their bits - whatever the alignment and the head size."""
+    x = dict(zip(("q", "k", "v", "do", "state", "dstate", "decay"), attention_inputs(1, T, 2, 2, D, D, dt, seed=3)))
+    x["decay"] = torch.tensor([-0.05, -0.2], device=DEV)
+    if off:   # (addresses off 16 bytes)
+        for n in ("q", "k", "v", "do"):
+            flat = torch.empty(x[n].numel() + off, dtype=dt, device=DEV)
+            x[n] = flat[off:].view(x[n].shape).copy_(x[n])
+    names = ("o", "state", "dq", "dk", "dv", "dstate")
+
+    def run(x):
+        o = ops.linear_attention(x["q"], x["k"], x["v"], x["decay"], state=x["state"])
+        return dict(zip(names, (*o, *ops.linear_attention_backward(x["do"], x["q"], x["k"], x["v"], x["decay"], state=x["state"], dstate=x["dstate"]))))
+
+    good = run(x)
+    at, m = T // 2, 5
+    # the results that have the non-finite channel as a channel of their own, and the dimension of it
+    alone = {"q": (("dk", 3), ("dstate", 2)), "k": (("state", 2), ("dq", 3)), "v": (("o", 3), ("state", 3)), "do": (("dv", 3), ("dstate", 3))}
+    for which in ("q", "k", "v", "do"):
+        y = dict(x)
+        y[which] = x[which].clone() if not off else torch.empty(x[which].numel() + off, dtype=dt, device=DEV)[off:].view(x[which].shape).copy_(x[which])
+        y[which][0, at, 1, m] = value
+        bad = run(y)
+        others = [i for i in range(D) if i != m]
+        for name, dim in alone[which]:
+            keep = lambda t: t.index_select(dim, torch.tensor(others, device=DEV))   # noqa: E731
+            assert torch.equal(keep(bad[name]), keep(good[name])), (which, name)
+            one = bad[name].select(dim, m)
+            assert not torch.isfinite(one[0, 1] if name in ("state", "dstate") else one[0, at, 1]).any(), (which, name)
+
+
 # ------------------------------------------------------------------------------------- streams, graphs, refusals, together
 def all_operators(x, w, rng, q, k, v, decay, state, out):
     """every operator once into the dict `out` (explicit forms, as a captured step calls them)"""
