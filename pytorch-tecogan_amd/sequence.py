@@ -379,8 +379,8 @@ def linear_attention_backward(do, q, k, v, log_decay, scale=None, state=None, le
 
 def linear_attention_step(q, k, v, log_decay, state, scale=None):
     """The next token of every sequence: q (B, H, Dk), k (B, Hk, Dk), v (B, Hk, Dv) -> o (B, H, Dv); `state`, float32 (B, H, Dk, Dv) and
-    contiguous, is updated in place.  The single-token form of linear_attention (as generator.recurrent_step is of generator.recurrent); it has no
-    gradient."""
+    contiguous, is updated in place (and counts as modified for autograd).  The single-token form of linear_attention (as generator.recurrent_step is
+    of generator.recurrent); it has no gradient."""
     if _wants_grad(q, k, v, state):
         _fail("linear_attention_step has no gradient: call it under torch.no_grad(), or linear_attention with one token")
     dt, d, (B, _, H, DK, DV), q, k, v, log_decay = _desc(q, k, v, log_decay, scale, True)
@@ -389,4 +389,5 @@ def linear_attention_step(q, k, v, log_decay, state, scale=None):
         _fail("state is updated in place: it must be contiguous")
     o = torch.empty((B, H, DV), dtype=q.dtype, device=q.device)
     _call(q.device, "tg_linear_attention_step", dt, d, q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), o.data_ptr(), state.data_ptr())
+    torch.autograd.graph.increment_version(state)   # (written through its address: a backward pass that saved the old values is to notice)
     return o

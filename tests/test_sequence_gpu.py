@@ -765,6 +765,27 @@ def test_attention_nonfinite_channels_reach_no_other_channel(T, D, off, value, d
             assert not torch.isfinite(one[0, 1] if name in ("state", "dstate") else one[0, at, 1]).any(), (which, name)
 
 
+def test_attention_step_moves_the_states_version():
+    """a state that a recorded call saved, stepped before its backward pass: refused by autograd, not differentiated with the new values"""
+    B, T, H, D = 2, 5, 2, 16
+    q, k, v, do, state, _, decay = attention_inputs(B, T, H, H, D, D, F32)
+    leaf = q.clone().requires_grad_()
+    o, _ = ops.linear_attention(leaf, k, v, decay, state=state)
+    before = state._version
+    with torch.no_grad():
+        ops.linear_attention_step(q[:, 0], k[:, 0], v[:, 0], decay, state)
+    assert state._version > before
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        o.backward(do)
+    # a view's step counts for its base; inference tensors keep no version
+    both = randn(2, B, H, D, D)
+    before = both._version
+    ops.linear_attention_step(q[:, 0], k[:, 0], v[:, 0], decay, both[1])
+    assert both._version > before
+    with torch.inference_mode():
+        ops.linear_attention_step(q[:, 0], k[:, 0], v[:, 0], decay, torch.zeros(B, H, D, D, device=DEV))
+
+
 # ------------------------------------------------------------------------------------- streams, graphs, refusals, together
 def all_operators(x, w, rng, q, k, v, decay, state, out):
     """every operator once into the dict `out` (explicit forms, as a captured step calls them)"""
