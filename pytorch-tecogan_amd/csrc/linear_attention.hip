@@ -1464,6 +1464,24 @@ struct StepArgs {
   int v4;                           // v's addresses are aligned to 4 elements
 };
 
+// exp(a) as two floats, for one product that rounds once: a rate of -1e-6 in a single float would be off by 1.3 %, the same way for every token of a
+// stream.  Fast decays and growth have nothing to lose beside their own size: one float.
+struct StepDecay {
+  float hi, lo;
+  __device__ __forceinline__ StepDecay(float a) {
+    const float m = expm1f(a);
+    hi = 1.f + m;
+    lo = (1.f - hi) + m;   // (exact: |m| < 1)
+    if (!(__builtin_fabsf(a) < 0.5f)) {
+      hi = expf(a);
+      lo = 0.f;
+    }
+  }
+  __device__ __forceinline__ float apply(float s, float x) const {   // exp(a) s + x; an infinite s stays (0 * infinity would be NaN)
+    return fmaf(hi, s, fmaf(lo, __builtin_amdgcn_fmed3f(s, -3.4028234e38f, 3.4028234e38f), x));
+  }
+};
+
 // One token.  What counts is the state: read once, written once.  LN lanes of a wave hold W floats each of a state row, so 64 / LN rows are
 // in one load; NB such loads are in flight.  WS waves share a state's rows (few states: the machine would wait for a handful of waves) and
 // add their parts of o through LDS.
@@ -1481,7 +1499,7 @@ template <typename T, int W, int NB, int WS> __global__ __launch_bounds__(256) v
     const int h = (int)(u - row * p.H);
     const int64_t bi = row;
     float* const S = p.state + (int64_t)u * p.M * p.N;
-    const float decay = expf(p.log_decay[h]);
+    const StepDecay decay(p.log_decay[h]);
     const int64_t oq = bi * p.qb + h * p.qh, ok = bi * p.kb + h / p.share * p.kh, ov = bi * p.vb + h / p.share * p.vh;
     for (int n = ln * W; n < ((p.N + W * LN - 1) / (W * LN)) * W * LN; n += W * LN) {
       float v[W], acc[W];
@@ -1515,7 +1533,7 @@ template <typename T, int W, int NB, int WS> __global__ __launch_bounds__(256) v
           const int m = m0 + i * rows + lm;
 #pragma unroll
           for (int e = 0; e < W; ++e) {
-            s[i][e] = fmaf(decay, s[i][e], k[i] * v[e]);
+            s[i][e] = decay.apply(s[i][e], k[i] * v[e]);
             acc[e] = fmaf(q[i], s[i][e], acc[e]);
           }
           if (n < p.N && m < p.M) {
@@ -1580,11 +1598,11 @@ template <typename T> __global__ __launch_bounds__(256) void la_step_small_kerne
     const unsigned next = u + stride;
     Unit y = x;
     if (next < p.units) y = fetch(next);
-    const float decay = expf(x.decay);
+    const StepDecay decay(x.decay);
     f32x4 acc;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      x.s[e] = fmaf(decay, x.s[e], x.k * x.v[e]);
+      x.s[e] = decay.apply(x.s[e], x.k * x.v[e]);
       acc[e] = x.q * x.s[e];
     }
     if (live) *reinterpret_cast<f32x4*>(p.state + (int64_t)u * states + mine) = x.s;

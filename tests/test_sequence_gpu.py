@@ -786,6 +786,35 @@ def test_attention_step_moves_the_states_version():
         ops.linear_attention_step(q[:, 0], k[:, 0], v[:, 0], decay, torch.zeros(B, H, D, D, device=DEV))
 
 
+@pytest.mark.parametrize("B,DK,DV", [(40, 16, 16), (3, 64, 64), (300, 40, 24), (5, 33, 15), (600, 64, 128)])
+def test_attention_step_keeps_slow_decays(B, DK, DV):
+    """One step of a state with k = 0: exp(log_decay) S rounded once.  A factor rounded to fp32 before the product would be off by up to 2^-25, a rate of
+    -1e-6 by 3 %.  fp32's expm1 (decays slower than -0.5) and exp are off by at most 2 units in the last place, of exp(a) - 1 and exp(a)."""
+    decays = (-1e-6, -1e-5, -1e-4, -3e-3, -0.11, -0.4, -0.6, -2.5, 0.0, 1e-5, 0.3)
+    decay = torch.tensor(decays, device=DEV)
+    H = len(decays)
+    state = randn(B, H, DK, DV, seed=1)
+    old = state.double()
+    q, k, v = randn(B, H, DK, seed=2), torch.zeros(B, H, DK, device=DEV), randn(B, H, DV, seed=3)
+    ops.linear_attention_step(q, k, v, decay, state)
+    a = decay.double()[:, None, None]
+    off = 4 * U * torch.where(a.abs() < 0.5, torch.expm1(a).abs(), torch.exp(a)) * old.abs()
+    want = old * torch.exp(a)
+    bound = HALF[F32] * (1 + 2.0 ** -7) * want.abs() + off + TINY[F32]
+    assert bool(((state.double() - want).abs() <= bound).all()), float((((state.double() - want).abs() - bound) / want.abs()).max()) / U
+
+
+def test_attention_step_keeps_infinite_states():
+    """a state that has left fp32's range stays there, whatever the decay"""
+    decay = torch.tensor([0.0, -1e-5, -0.3, -3.0], device=DEV)
+    for DK, DV in ((16, 16), (64, 64), (5, 7)):
+        q, k, v, state = randn(2, 4, DK, seed=1), randn(2, 4, DK, seed=2), randn(2, 4, DV, seed=3), randn(2, 4, DK, DV, seed=4)
+        state[:, :, 1, 2], state[:, :, 3, 0] = math.inf, -math.inf
+        ops.linear_attention_step(q, k, v, decay, state)
+        assert bool((state[:, :, 1, 2] == math.inf).all()) and bool((state[:, :, 3, 0] == -math.inf).all())
+        assert int(torch.isfinite(state).logical_not().sum()) == 16
+
+
 # ------------------------------------------------------------------------------------- streams, graphs, refusals, together
 def all_operators(x, w, rng, q, k, v, decay, state, out):
     """every operator once into the dict `out` (explicit forms, as a captured step calls them)"""
