@@ -249,6 +249,26 @@ struct Decay {
   }
 };
 
+// A state's factor g^n = e^a as two floats, whose product with the state rounds once.  Slow decays: in a single float a rate of -1e-6 would be off by 1.3 %,
+// the same way at every use.  Fast ones (and growth), where 1 + (g^n - 1) would lose the digits of a small power: `fast`, e^a in one float.
+struct Factor {
+  float hi, lo;
+  __device__ __forceinline__ Factor(float a, float fast) {
+    const float m = expm1f(a);
+    hi = 1.f + m;
+    lo = (1.f - hi) + m;   // (exact: |m| < 1)
+    if (!(__builtin_fabsf(a) < 0.5f)) {
+      hi = fast;
+      lo = 0.f;
+    }
+  }
+  __device__ __forceinline__ Factor(const Decay& d, int n) : Factor(d.la * (float)n, d.pow(n)) {}
+  __device__ __forceinline__ float operator()(float s) const { return fmaf(s, hi, s * lo); }
+  __device__ __forceinline__ float plus(float s, float x) const {   // g^n s + x; an infinite s stays (0 * infinity would be NaN)
+    return fmaf(hi, s, fmaf(lo, __builtin_amdgcn_fmed3f(s, -3.4028234e38f, 3.4028234e38f), x));
+  }
+};
+
 __device__ __forceinline__ void wave_fence() {   // the wave's own LDS writes and reads keep their order
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   __builtin_amdgcn_wave_barrier();
@@ -355,12 +375,11 @@ template <typename T, int MT, int NS = 1> struct Wave {
 template <int CT> struct Weights {
   static constexpr int C = 16 * CT;
   f32x4 inside[CT], whole[CT], tail[CT];   // scale g^{i-j} by tile distance (i = c, j = 4g + e); zs g^{n-1-j+sh} of whole chunks, and of the one of `tokens` that ends a sequence
-  float from[CT], whole_keep, tail_keep, g1;   // za g^{i+1-sh}; g^n - 1; g
+  float from[CT], g1;   // za g^{i+1-sh}; g
+  Factor whole_keep, tail_keep;   // g^n
   int tokens;
-  __device__ __forceinline__ Weights(const Decay& decay, int c, int g, float scale, float za, float zs, int sh) {
+  __device__ __forceinline__ Weights(const Decay& decay, int c, int g, float scale, float za, float zs, int sh) : whole_keep(decay, C), tail_keep(0.f, 1.f) {
     g1 = decay.pow(1);
-    whole_keep = expm1f(decay.la * (float)C);
-    tail_keep = 0.f;
     tokens = 0;
 #pragma unroll
     for (int t = 0; t < CT; ++t) {   // (the fourth of four neighbouring powers, the others by one more factor each)
@@ -379,7 +398,7 @@ template <int CT> struct Weights {
   __device__ __forceinline__ void length(const Decay& decay, int cnt, int g, float zs, int sh) {   // a sequence's last chunk has cnt tokens
     if (cnt >= C || cnt == tokens) return;
     tokens = cnt;
-    tail_keep = expm1f(decay.la * (float)cnt);
+    tail_keep = Factor(decay, cnt);
     const float w0 = zs * decay.pow(sh);
 #pragma unroll
     for (int t = 0; t < CT; ++t) {
@@ -393,10 +412,10 @@ template <int CT> struct Weights {
     }
   }
   __device__ __forceinline__ f32x4 into(int cnt, int t) const { return cnt < C ? tail[t] : whole[t]; }
-  __device__ __forceinline__ f32x4 kept(f32x4 s, int cnt) const {   // g^n S as S + (g^n - 1) S: a slow decay's last bits stay
-    const float k = cnt < C ? tail_keep : whole_keep;
+  __device__ __forceinline__ f32x4 kept(f32x4 s, int cnt) const {   // g^n S
+    const Factor k = cnt < C ? tail_keep : whole_keep;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) s[e] = fmaf(s[e], k, s[e]);
+    for (int e = 0; e < 4; ++e) s[e] = k(s[e]);
     return s;
   }
   __device__ __forceinline__ f32x4 masked(f32x4 x, int it, int jt, int c, int g) const {
@@ -904,7 +923,9 @@ template <typename T, int MT, int CT, int NS, bool STATE> __global__ __launch_bo
 // (la_kernel's loops over segments and chunks cost more scalar instructions and branches here than the chunk itself: 39 us for the gradients
 // of 16384 sequences of 10 tokens x 16 channels, 23 us here.)  Forward 13.0 us, 38 MB at 2.9 TB/s (four sequences a wave: the launch and the decay's
 // powers are a third of it); 65536 sequences, 4 heads of 16 channels 149 us, 4.1 TB/s.
-template <typename T, int MT> __global__ __launch_bounds__(256, 2) void la_short_kernel(LaArgs p) {
+// Heads of up to 32 channels are held to the registers of four waves per SIMD, which they fit (4096 sequences of 10 tokens x 32 fp16 channels 34.3 us, 37.4
+// with 131 registers and three waves).
+template <typename T, int MT> __global__ __launch_bounds__(256, MT <= 2 ? 4 : 2) void la_short_kernel(LaArgs p) {
   typedef Mat<T> X;
   typedef Stage<T, MT, 1> G;
   typedef typename X::Raw Raw;
@@ -980,7 +1001,7 @@ template <typename T, int MT> __global__ __launch_bounds__(256, 2) void la_short
     }
   };
   f32x4 inside, into;
-  float keep = 0.f;
+  Factor keep(0.f, 1.f);
   const float g1 = decay.pow(1), from = r.za * decay.pow(c + 1 - r.sh);
   {
     const int d = c - 4 * g;
@@ -989,7 +1010,7 @@ template <typename T, int MT> __global__ __launch_bounds__(256, 2) void la_short
     for (int e = 2; e >= 0; --e) inside[e] = d - e > 0 ? inside[e + 1] * g1 : p.scale;
   }
   auto weights = [&](int n) {
-    keep = expm1f(decay.la * (float)n);
+    keep = Factor(decay, n);
     const int d = n - 1 - 4 * g;
     const float w0 = r.zs * decay.pow(r.sh);
     float w = r.zs * decay.pow(max(d - 3, 0) + r.sh);
@@ -1094,7 +1115,7 @@ template <typename T, int MT> __global__ __launch_bounds__(256, 2) void la_short
           f32x4 v = zero;
           if (s0)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = fmaf(S[t][e], keep, S[t][e]);
+            for (int e = 0; e < 4; ++e) v[e] = keep(S[t][e]);
           S[t] = X::add(X::op(columns(area_b, G::kRow, t)), ws, v);
         }
       }
@@ -1198,10 +1219,11 @@ template <typename T, int MT> __global__ __launch_bounds__(256, MT == 1 ? 4 : 2)
   if (DK != 16 * MT || DV != 16 * MT)   // (channels behind DK and DV)
     for (int i = lane * 16; i < 4 * kRows16; i += 1024) *reinterpret_cast<u32x4*>(area + i) = u32x4{0, 0, 0, 0};
 
-  // scale g^{i-j}: [j][i] for dq, [i][j] for dk and dv;  scale g^{i+1} by lane and by element;  g^{n-1-j} by lane, and g^n - 1
+  // scale g^{i-j}: [j][i] for dq, [i][j] for dk and dv;  scale g^{i+1} by lane and by element;  g^{n-1-j} by lane, and g^n
   f32x4 below, above, into;
   const float g1 = decay.pow(1), from = p.scale * decay.pow(c + 1);
-  float back = 0.f, keep = 0.f;
+  float back = 0.f;
+  Factor keep(0.f, 1.f);
   int known = -1;
   {
     const int d = c - 4 * g;
@@ -1284,7 +1306,7 @@ template <typename T, int MT> __global__ __launch_bounds__(256, MT == 1 ? 4 : 2)
     if (n != known) {
       known = n;
       back = decay.pow(max(n - 1 - c, 0));
-      keep = expm1f(decay.la * (float)n);
+      keep = Factor(decay, n);
     }
     f32x4 S[MT];
     if (n > 0) {
@@ -1346,7 +1368,7 @@ template <typename T, int MT> __global__ __launch_bounds__(256, MT == 1 ? 4 : 2)
 #pragma unroll
         for (int t = 0; t < MT; ++t) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) S[t][e] = fmaf(S[t][e], keep, S[t][e]);
+          for (int e = 0; e < 4; ++e) S[t][e] = keep(S[t][e]);
           S[t] = X::add(X::op(cols(0, t)), ws, S[t]);
         }
       }
@@ -1464,24 +1486,6 @@ struct StepArgs {
   int v4;                           // v's addresses are aligned to 4 elements
 };
 
-// exp(a) as two floats, for one product that rounds once: a rate of -1e-6 in a single float would be off by 1.3 %, the same way for every token of a
-// stream.  Fast decays and growth have nothing to lose beside their own size: one float.
-struct StepDecay {
-  float hi, lo;
-  __device__ __forceinline__ StepDecay(float a) {
-    const float m = expm1f(a);
-    hi = 1.f + m;
-    lo = (1.f - hi) + m;   // (exact: |m| < 1)
-    if (!(__builtin_fabsf(a) < 0.5f)) {
-      hi = expf(a);
-      lo = 0.f;
-    }
-  }
-  __device__ __forceinline__ float apply(float s, float x) const {   // exp(a) s + x; an infinite s stays (0 * infinity would be NaN)
-    return fmaf(hi, s, fmaf(lo, __builtin_amdgcn_fmed3f(s, -3.4028234e38f, 3.4028234e38f), x));
-  }
-};
-
 // One token.  What counts is the state: read once, written once.  LN lanes of a wave hold W floats each of a state row, so 64 / LN rows are
 // in one load; NB such loads are in flight.  WS waves share a state's rows (few states: the machine would wait for a handful of waves) and
 // add their parts of o through LDS.
@@ -1499,7 +1503,8 @@ template <typename T, int W, int NB, int WS> __global__ __launch_bounds__(256) v
     const int h = (int)(u - row * p.H);
     const int64_t bi = row;
     float* const S = p.state + (int64_t)u * p.M * p.N;
-    const StepDecay decay(p.log_decay[h]);
+    const float log_decay = p.log_decay[h];
+    const Factor decay(log_decay, expf(log_decay));
     const int64_t oq = bi * p.qb + h * p.qh, ok = bi * p.kb + h / p.share * p.kh, ov = bi * p.vb + h / p.share * p.vh;
     for (int n = ln * W; n < ((p.N + W * LN - 1) / (W * LN)) * W * LN; n += W * LN) {
       float v[W], acc[W];
@@ -1533,7 +1538,7 @@ template <typename T, int W, int NB, int WS> __global__ __launch_bounds__(256) v
           const int m = m0 + i * rows + lm;
 #pragma unroll
           for (int e = 0; e < W; ++e) {
-            s[i][e] = decay.apply(s[i][e], k[i] * v[e]);
+            s[i][e] = decay.plus(s[i][e], k[i] * v[e]);
             acc[e] = fmaf(q[i], s[i][e], acc[e]);
           }
           if (n < p.N && m < p.M) {
@@ -1598,11 +1603,11 @@ template <typename T> __global__ __launch_bounds__(256) void la_step_small_kerne
     const unsigned next = u + stride;
     Unit y = x;
     if (next < p.units) y = fetch(next);
-    const StepDecay decay(x.decay);
+    const Factor decay(x.decay, expf(x.decay));
     f32x4 acc;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      x.s[e] = decay.apply(x.s[e], x.k * x.v[e]);
+      x.s[e] = decay.plus(x.s[e], x.k * x.v[e]);
       acc[e] = x.q * x.s[e];
     }
     if (live) *reinterpret_cast<f32x4*>(p.state + (int64_t)u * states + mine) = x.s;

@@ -815,6 +815,23 @@ def test_attention_step_keeps_infinite_states():
         assert int(torch.isfinite(state).logical_not().sum()) == 16
 
 
+@pytest.mark.parametrize("dt", [F32, BF16, F16])
+@pytest.mark.parametrize("T,D", [(10, 16), (16, 20), (33, 16), (64, 64), (64, 17), (40, 128), (1100, 32), (1100, 19)])
+def test_attention_fading_states_keep_their_digits(T, D, dt):
+    """Tokens with k = 0 (q, do = 0 for the gradient) leave exp(log_decay T) S however small it is: one power and one product for each 16 (10) tokens or
+    more, each off by at most 4 units in the last place (the power: 3, fp32's exponent included)."""
+    decays = (-0.2, -0.5, -0.9, -0.05)
+    decay = torch.tensor(decays if T < 100 else [d / 16 for d in decays], device=DEV)
+    q, k, v, do, state, dstate, _ = attention_inputs(2, T, 4, 4, D, D, dt)
+    last = ops.linear_attention(q, torch.zeros_like(k), v, decay, state=state)[1]
+    first = ops.linear_attention_backward(torch.zeros_like(do), q, k, v, decay, state=state, dstate=dstate)[3]
+    g = torch.exp(decay.double() * T)[:, None, None]
+    units = 5 * (T // 16 + 1)
+    for got, s in ((last, state), (first, dstate)):
+        want = s.double() * g
+        assert bool(((got.double() - want).abs() <= units * U * want.abs() + TINY[F32]).all()), float(((got.double() - want) / want).abs().max()) / U
+
+
 # ------------------------------------------------------------------------------------- streams, graphs, refusals, together
 def all_operators(x, w, rng, q, k, v, decay, state, out):
     """every operator once into the dict `out` (explicit forms, as a captured step calls them)"""
