@@ -253,6 +253,13 @@ struct Decay {
 // the same way at every use.  Fast ones (and growth), where 1 + (g^n - 1) would lose the digits of a small power: `fast`, e^a in one float.
 struct Factor {
   float hi, lo;
+  Factor() = default;
+  __device__ __forceinline__ static Factor of(float hi, float lo) {
+    Factor f;
+    f.hi = hi;
+    f.lo = lo;
+    return f;
+  }
   __device__ __forceinline__ Factor(float a, float fast) {
     const float m = expm1f(a);
     hi = 1.f + m;
@@ -413,7 +420,7 @@ template <int CT> struct Weights {
   }
   __device__ __forceinline__ f32x4 into(int cnt, int t) const { return cnt < C ? tail[t] : whole[t]; }
   __device__ __forceinline__ f32x4 kept(f32x4 s, int cnt) const {   // g^n S
-    const Factor k = cnt < C ? tail_keep : whole_keep;
+    const Factor k = Factor::of(cnt < C ? tail_keep.hi : whole_keep.hi, cnt < C ? tail_keep.lo : whole_keep.lo);
 #pragma unroll
     for (int e = 0; e < 4; ++e) s[e] = k(s[e]);
     return s;
@@ -1424,7 +1431,7 @@ template <typename T, int MT> __global__ __launch_bounds__(256, MT == 1 ? 4 : 2)
 // takes 64 elements of one state; its waves take consecutive segments each and meet through LDS
 constexpr int kMaxSegments = 256;
 __global__ __launch_bounds__(1024) void la_scan_kernel(LaArgs p) {
-  __shared__ float total[16][64], fades[16];
+  __shared__ float total[16][64], fades[16][2];
   const Role& r = p.r[blockIdx.z];
   const int states = r.M * r.N, x = threadIdx.x & 63, z = threadIdx.x >> 6, at = blockIdx.x * 64 + x, h = blockIdx.y % p.H, bi = blockIdx.y / p.H;
   const int64_t pair = blockIdx.y;
@@ -1433,31 +1440,39 @@ __global__ __launch_bounds__(1024) void la_scan_kernel(LaArgs p) {
   const bool live = at < states;
   float* const seg = r.seg + pair * p.segments * states + at;
   const int joins = p.segments - 1, G = blockDim.x >> 6, K = (joins + G - 1) / G, s0 = min(z * K, joins), s1 = min(s0 + K, joins);   // this group's segments
-  // the decay over segment s: whole, the one that holds the sequence's end, or behind it
+  // the decay over segment s: whole, the one that holds the sequence's end, or behind it (two floats each: a rounded factor would be off the same way
+  // at every joint, 256 of them by 2^-17 together)
   const int last = n / p.seg;
-  const float over = decay.pow(p.seg), part = decay.pow(n - last * p.seg);
+  const Factor over(decay, p.seg), part(decay, n - last * p.seg);
   float own[kMaxSegments / 16], run = 0.f;
 #pragma unroll
   for (int k = 0; k < kMaxSegments / 16; ++k)
     if (k < K) own[k] = s0 + k < s1 && live ? seg[(int64_t)(s0 + k + 1) * states] : 0.f;
   const float first = r.s0 && live ? r.s0[pair * states + at] : 0.f;
-  auto fade = [&](int s) { return s >= s1 ? 1.f : s < last ? over : s == last ? part : 1.f; };
+  auto fade = [&](int s) {   // (by value, each float by itself: a choice between objects would go through memory)
+    const bool whole = s < s1 && s < last, end = s < s1 && s == last;
+    return Factor::of(whole ? over.hi : end ? part.hi : 1.f, whole ? over.lo : end ? part.lo : 0.f);
+  };
 #pragma unroll
   for (int k = 0; k < kMaxSegments / 16; ++k)
-    if (k < K) run = fmaf(fade(s0 + k), run, own[k]);
+    if (k < K) run = fade(s0 + k).plus(run, own[k]);
   total[z][x] = run;
-  if (x == 0) fades[z] = decay.pow(min(max(n - s0 * p.seg, 0), (s1 - s0) * p.seg));   // (all but the last segment are whole)
+  if (x == 0) {   // (all but the last segment are whole)
+    const Factor all(decay, min(max(n - s0 * p.seg, 0), (s1 - s0) * p.seg));
+    fades[z][0] = all.hi;
+    fades[z][1] = all.lo;
+  }
   __syncthreads();
   run = first;
 #pragma unroll
   for (int y = 0; y < 15; ++y)
-    if (y < z) run = fmaf(fades[y], run, total[y][x]);
+    if (y < z) run = Factor::of(fades[y][0], fades[y][1]).plus(run, total[y][x]);
   if (!live) return;
   if (z == 0) seg[0] = first;
 #pragma unroll
   for (int k = 0; k < kMaxSegments / 16; ++k)
     if (k < K && s0 + k < s1) {
-      run = fmaf(fade(s0 + k), run, own[k]);
+      run = fade(s0 + k).plus(run, own[k]);
       seg[(int64_t)(s0 + k + 1) * states] = run;
     }
 }

@@ -832,6 +832,23 @@ def test_attention_fading_states_keep_their_digits(T, D, dt):
         assert bool(((got.double() - want).abs() <= units * U * want.abs() + TINY[F32]).all()), float(((got.double() - want) / want).abs().max()) / U
 
 
+@pytest.mark.parametrize("rate", [-1.1e-6, -2.3e-6, -1.7e-5])
+def test_attention_slow_decays_across_segments(rate):
+    """One sequence of 16384 tokens with k = 0: what is left of the state.  Its elements are rounded at every joint (256 at most) by errors that do not depend on each
+    other, so their mean over 4096 elements is off by less than 6 sqrt(256 / 4096 / 3) 2^-24; a joint's factor that is itself rounded is off the same
+    way for all of them, up to 256 times 2^-25."""
+    T, D = 16384, 64
+    decay = torch.full((1,), rate, device=DEV)
+    state = 1 + torch.rand(1, 1, D, D, generator=torch.Generator().manual_seed(1)).to(DEV)
+    q, k, v = (randn(1, T, 1, D, dt=BF16, seed=i) for i in range(3))
+    zero = torch.zeros_like(k)
+    want = state.double() * torch.exp(decay.double() * T)
+    for got in (ops.linear_attention(q, zero, v, decay, state=state)[1], ops.linear_attention_backward(zero, q, k, v, decay, state=state, dstate=state)[3]):
+        e = (got.double() - want) / want
+        assert abs(float(e.mean())) < 6 * math.sqrt(256 / (3 * D * D)) * U, float(e.mean()) / U
+        assert float(e.abs().max()) < 257 * U
+
+
 # ------------------------------------------------------------------------------------- streams, graphs, refusals, together
 def all_operators(x, w, rng, q, k, v, decay, state, out):
     """every operator once into the dict `out` (explicit forms, as a captured step calls them)"""
