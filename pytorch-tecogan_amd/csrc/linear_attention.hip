@@ -1855,7 +1855,7 @@ extern "C" int tg_linear_attention(int dtype, const tg_la_desc* d, const void* q
   a.scale = d->scale;
   const bool wide = Q.wide && K.wide && V.wide && d->DK % 4 == 0 && d->DV % 4 == 0 && (reinterpret_cast<uintptr_t>(o) & (4 * elem_bytes(dtype) - 1)) == 0;
   const int piece = 16 / elem_bytes(dtype);
-  const bool pieces = wide && Q.pieces && K.pieces && V.pieces && d->DK % piece == 0 && d->DV % piece == 0;
+  const bool pieces = wide && Q.pieces && K.pieces && V.pieces && tg_aligned16(o) && d->DK % piece == 0 && d->DV % piece == 0;
   a.r[0] = Role{Q.o, K.o, V.o, o, state_in, state_out, scratch, d->DK, d->DV, d->DV, 1, d->scale, 1.f, 0, 0, 1, 0, wide, pieces};
   if (a.segments > 1 && (rc = join_segments(dtype, a, 1, st)) != TG_OK) return rc;
   return launch_dt(dtype, a, 1, false, st);

@@ -6,6 +6,7 @@ smallest step, 2^-25).  Sums in fp32 are off by at most (number of additions one
 magnitudes; the operators add at most ADDS in a row before they join partial sums in a tree.  linear_attention additionally splits scores and
 states into two bf16 halves beside 16-bit inputs: 2^-16 of the magnitudes for each split on the way of a term (at most 4: weight, state, fp16's
 own two halves)."""
+import ctypes as C
 import math
 import os
 import subprocess
@@ -847,6 +848,29 @@ def test_attention_slow_decays_across_segments(rate):
         e = (got.double() - want) / want
         assert abs(float(e.mean())) < 6 * math.sqrt(256 / (3 * D * D)) * U, float(e.mean()) / U
         assert float(e.abs().max()) < 257 * U
+
+
+@pytest.mark.parametrize("dt", [BF16, F16, F32])
+def test_attention_output_off_16_bytes(dt):
+    """the C entry takes any output that is aligned to its elements: o one element, 8 or 12 bytes past a multiple of 16, beside aligned operands"""
+    lib, size, code = L.load(), torch.finfo(dt).bits // 8, {F32: L.TG_F32, BF16: L.TG_BF16, F16: L.TG_F16}[dt]
+    for B, T, H, DK, DV in ((3, 10, 2, 16, 16), (2, 40, 2, 32, 64), (1, 900, 1, 64, 64), (700, 20, 2, 64, 64)):
+        q, k, v, _, state, _, decay = attention_inputs(B, T, H, H, DK, DV, dt)
+        want, mag = attention_oracle(q, k, v, decay, DK ** -0.5, state, None)
+        st = lambda d: (T * H * d, H * d, d)   # noqa: E731
+        desc = L.LaDesc(B, T, H, H, DK, DV, st(DK), st(DK), st(DV), DK ** -0.5)
+        need = lib.tg_linear_attention_scratch_floats(code, C.byref(desc))
+        for off in (size, 8, 12):
+            room = torch.full((B * T * H * DV + 32 // size,), 7.0, dtype=dt, device=DEV)
+            last, scratch = torch.empty_like(state), torch.empty(max(need, 1), device=DEV)
+            assert room.data_ptr() % 16 == 0
+            rc = lib.tg_linear_attention(code, C.byref(desc), q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                                         decay.data_ptr(), None, state.data_ptr(), room.data_ptr() + off, last.data_ptr(), scratch.data_ptr(),
+                                         torch.cuda.current_stream().cuda_stream)
+            assert rc == 0
+            o = room[off // size:off // size + B * T * H * DV].view(B, T, H, DV)
+            close(o, want["o"], dt, mag["o"], attention_units(dt, T, max(DK, DV)), "o")
+            assert bool((room[:off // size] == 7).all()) and bool((room[off // size + B * T * H * DV:] == 7).all())
 
 
 # ------------------------------------------------------------------------------------- streams, graphs, refusals, together
