@@ -4,7 +4,7 @@ the reference's code/ops.py:45-88 and have no counterpart there.
 
 Each operator takes device tensors (fp32, bf16 or fp16), enqueues its HIP kernels on the current stream of the tensors' device and
 allocates its outputs and workspaces like any torch operation; nothing synchronises.  Where an input requires a gradient the result
-carries one (first order).  The explicit forms - `stats=True` and the `*_backward` functions - are what a captured step uses: autograd
+carries one (first order, reverse mode; dual tensors of forward mode are refused).  The explicit forms - `stats=True` and the `*_backward` functions - are what a captured step uses: autograd
 itself is not captured (a backward pass recorded while an eager graph of the same leaves lives ends the process), so inside a capture a
 call that would build an autograd graph raises; use torch.no_grad() there, or the explicit forms on detached tensors."""
 import struct
@@ -75,6 +75,15 @@ def _f32(x, t, what, shape):
     if not isinstance(t, torch.Tensor) or t.device != x.device or t.dtype != torch.float32 or t.shape != shape:
         _fail(f"{what} must be a float32 tensor of shape {tuple(shape)} on {x.device}")
     return t if t.is_contiguous() else t.contiguous()
+
+
+_forward_ad = torch.autograd.forward_ad
+
+
+def _no_tangents(*tensors):
+    """refuses dual tensors: they do not require a gradient, so their tangents would be dropped without a word"""
+    if _forward_ad._current_level >= 0 and any(isinstance(t, torch.Tensor) and _forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        _fail("no forward-mode derivatives: the operators have gradients (reverse mode) only")
 
 
 def _wants_grad(*tensors):
@@ -162,6 +171,7 @@ def rms_norm(x, weight=None, residual=None, eps=1e-6, stats=False):
     """y = s / sqrt(mean(s^2) + eps) * weight over the last dimension, s = x (+ residual).  weight: float32 (channels,) or None (ones);
     residual: like x.  Returns y, or (y, s) with a residual (s, the residual stream, in x's type; y comes from the unrounded sum), and at the
     end the rows' 1 / sqrt(...) (float32) with `stats` - what rms_norm_backward takes."""
+    _no_tangents(x, weight, residual)
     if _grad(x, weight, residual):
         out = _RMSNorm.apply(x, weight, residual, eps)
         out = out if stats else out[:-1]
@@ -175,6 +185,7 @@ def rms_norm_backward(dy, x, rstd, weight=None, residual=None, ds=None, dweight=
     """(dx, dweight) of rms_norm from dy, its inputs and its `stats`; ds: the gradient that reaches s on other ways (the residual stream's).
     dx is the gradient of x and of the residual alike; dweight is float32, None if not wanted.  Rows are added in a fixed order: the same
     call gives the same bits."""
+    _no_tangents(dy, x, rstd, weight, residual, ds)
     dt, channels, weight = _norm_args(x, weight, residual, 0.0)
     _like(x, dy, "dy")
     rows = x.numel() // channels
@@ -198,6 +209,7 @@ def rms_norm_backward(dy, x, rstd, weight=None, residual=None, ds=None, dweight=
 def rms_norm_e4m3(x, weight=None, residual=None, eps=1e-6):
     """rms_norm with an 8-bit output: (q, scale), or (q, scale, s) with a residual; q float8_e4m3fn like x, scale float32 per row =
     max(max|y|, 2^-100) / 448, y ~ q * scale.  A serving form: it has no gradient."""
+    _no_tangents(x, weight, residual)
     if _wants_grad(x, weight, residual):
         _fail("rms_norm_e4m3 has no gradient: call it under torch.no_grad()")
     dt, channels, weight = _norm_args(x, weight, residual, eps)
@@ -252,6 +264,7 @@ class _Dropout(torch.autograd.Function):
 def dropout(x, p, rng, layer=0, residual=None):
     """(residual +) keep * x / (1 - p).  Element i of x (in row-major order, whatever x's strides) is dropped with probability p (to 2^-32) by
     the counter-based generator at (rng seed, rng step, layer, i); the mask is not stored, and is the same for every element type."""
+    _no_tangents(x, residual)
     if _grad(x, residual):
         return _Dropout.apply(x, p, rng, layer, residual)
     return _drop(x, p, rng, layer, residual)
@@ -259,6 +272,7 @@ def dropout(x, p, rng, layer=0, residual=None):
 
 def dropout_backward(dy, p, rng, layer=0):
     """The gradient of x from y's: the same mask again, from the same (seed, step) and layer.  (The residual's gradient is dy.)"""
+    _no_tangents(dy)
     return _drop(dy, p, rng, layer, None)
 
 
@@ -353,6 +367,7 @@ def linear_attention(q, k, v, log_decay, scale=None, state=None, lengths=None):
     float32 (B, H, Dk, Dv), zeros if None; lengths: int32 (B,), tokens at and behind it are not read, their rows of o are zero and the last S is
     the one at the length.  o (B, T, H, Dv) in q's type, S in float32.  Gradients reach q, k, v and state.  An infinity or NaN in one token
     reaches that token and later ones only."""
+    _no_tangents(q, k, v, log_decay, state)
     if _grad(q, k, v, state):
         _desc(q, k, v, log_decay, scale, False)   # (its refusals, before anything is recorded)
         return _LinearAttention.apply(q, k, v, log_decay, scale, state, lengths)
@@ -362,6 +377,7 @@ def linear_attention(q, k, v, log_decay, scale=None, state=None, lengths=None):
 def linear_attention_backward(do, q, k, v, log_decay, scale=None, state=None, lengths=None, dstate=None):
     """(dq, dk, dv, gradient of the first state) of linear_attention from the gradients of o and, if given, of the last state; the gradient of
     the first state is None where `state` is.  The gradients of shared key / value heads are summed in 32 bits."""
+    _no_tangents(do, q, k, v, log_decay, state, dstate)
     dt, d, (B, T, H, DK, DV), q, k, v, log_decay = _desc(q, k, v, log_decay, scale, False, recorded=False)
     dev, shape = q.device, (B, H, DK, DV)
     do = _channels_last(_like(q, do, "do", (B, T, H, DV)))
@@ -381,6 +397,7 @@ def linear_attention_step(q, k, v, log_decay, state, scale=None):
     """The next token of every sequence: q (B, H, Dk), k (B, Hk, Dk), v (B, Hk, Dv) -> o (B, H, Dv); `state`, float32 (B, H, Dk, Dv) and
     contiguous, is updated in place (and counts as modified for autograd).  The single-token form of linear_attention (as generator.recurrent_step is
     of generator.recurrent); it has no gradient."""
+    _no_tangents(q, k, v, log_decay, state)
     if _wants_grad(q, k, v, state):
         _fail("linear_attention_step has no gradient: call it under torch.no_grad(), or linear_attention with one token")
     dt, d, (B, _, H, DK, DV), q, k, v, log_decay = _desc(q, k, v, log_decay, scale, True)

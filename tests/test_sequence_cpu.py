@@ -117,6 +117,23 @@ def test_host_tensors_are_refused():
             call()
 
 
+def test_forward_mode_is_refused():
+    """a dual tensor does not require a gradient: without a check its tangent would be dropped"""
+    fw = torch.autograd.forward_ad
+    x, q = torch.zeros(4, 64), torch.zeros(2, 3, 2, 16)
+    rng, decay, state = torch.zeros(2, dtype=torch.int64), torch.zeros(2), torch.zeros(2, 2, 16, 16)
+    with fw.dual_level():
+        d = lambda t: fw.make_dual(t, torch.ones_like(t))   # noqa: E731
+        for call in (lambda: ops.rms_norm(d(x)), lambda: ops.rms_norm(x, residual=d(x)), lambda: ops.rms_norm_e4m3(d(x)), lambda: ops.rms_norm_backward(d(x), x, x[:, 0]),
+                     lambda: ops.dropout(d(x), 0.1, rng), lambda: ops.dropout(x, 0.1, rng, residual=d(x)), lambda: ops.dropout_backward(d(x), 0.1, rng),
+                     lambda: ops.linear_attention(q, d(q), q, decay), lambda: ops.linear_attention(q, q, q, decay, state=d(state)),
+                     lambda: ops.linear_attention_backward(q, q, q, q, decay, state=state, dstate=d(state)), lambda: ops.linear_attention_step(q[:, 0], q[:, 0], q[:, 0], decay, d(state))):
+            with pytest.raises(L.TecoganHipError, match="forward-mode"):
+                call()
+        with pytest.raises(L.TecoganHipError, match="device tensor"):
+            ops.rms_norm(x)   # (a plain tensor inside a level is looked at as ever)
+
+
 def test_names_are_public():
     """`from ops import *` (code/ops.py) re-exports every public name of the package's ops module"""
     from pytorch_tecogan_amd import sequence

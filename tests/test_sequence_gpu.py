@@ -976,6 +976,24 @@ def test_autograd_is_refused_inside_a_capture():
     assert y.shape == x.shape
 
 
+def test_forward_mode_is_refused():
+    """no operator hands a tangent on: a dual tensor is refused instead of losing its own"""
+    x, w, r = randn(4, 64), randn(64), randn(4, 64)
+    q, state, decay, rng = randn(2, 3, 2, 16), randn(2, 2, 16, 16), torch.zeros(2, device=DEV), ops.dropout_rng(1, DEV)
+    fw = torch.autograd.forward_ad
+    with fw.dual_level():
+        d = lambda t: fw.make_dual(t, torch.ones_like(t))   # noqa: E731
+        for call in (lambda: ops.rms_norm(d(x), w), lambda: ops.rms_norm(x, d(w)), lambda: ops.rms_norm(x, w, residual=d(r)), lambda: ops.rms_norm_e4m3(d(x), w),
+                     lambda: ops.rms_norm_backward(d(x), x, randn(4), w), lambda: ops.rms_norm_backward(x, x, randn(4), w, ds=d(x)), lambda: ops.dropout(d(x), 0.1, rng),
+                     lambda: ops.dropout(x, 0.1, rng, residual=d(r)), lambda: ops.dropout_backward(d(x), 0.1, rng), lambda: ops.linear_attention(d(q), q, q, decay),
+                     lambda: ops.linear_attention(q, q, d(q), decay), lambda: ops.linear_attention(q, q, q, d(decay)), lambda: ops.linear_attention(q, q, q, decay, state=d(state)),
+                     lambda: ops.linear_attention_backward(d(q), q, q, q, decay), lambda: ops.linear_attention_backward(q, q, q, q, decay, state=state, dstate=d(state)),
+                     lambda: ops.linear_attention_step(d(q[:, 0]), q[:, 0], q[:, 0], decay, state[:2])):
+            with pytest.raises(L.TecoganHipError, match="forward-mode"):
+                call()
+        assert torch.equal(ops.rms_norm(x, w), ops.rms_norm(x.clone(), w))   # (plain tensors inside a level are served)
+
+
 FIRST_CALL = """
 import torch
 import pytorch_tecogan_amd
