@@ -90,11 +90,19 @@ def _wants_grad(*tensors):
     return torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in tensors)
 
 
-def _grad(*tensors):
-    """whether autograd has to record this call"""
-    if not _wants_grad(*tensors):
+def _capturing(dev):
+    """whether the current stream of `dev` records a graph (torch asks the current device's)"""
+    if dev.index == _device():
+        return torch.cuda.is_current_stream_capturing()
+    with torch.cuda.device(dev):
+        return torch.cuda.is_current_stream_capturing()
+
+
+def _grad(x, *others):
+    """whether autograd has to record this call on x's device"""
+    if not _wants_grad(x, *others) or not isinstance(x, torch.Tensor) or not x.is_cuda:   # (an x that is none is refused by the call itself)
         return False
-    if torch.cuda.is_current_stream_capturing():
+    if _capturing(x.device):
         _fail("autograd is not captured into graphs: use torch.no_grad(), or the explicit backward functions on detached tensors")
     return True
 

@@ -134,6 +134,42 @@ def test_forward_mode_is_refused():
             ops.rms_norm(x)   # (a plain tensor inside a level is looked at as ever)
 
 
+class OnDevice(torch.Tensor):
+    """a host tensor that says it is on a device"""
+    index = 0
+    is_cuda = property(lambda self: True)
+    device = property(lambda self: torch.device("cuda", self.index))
+
+
+@pytest.mark.parametrize("current,of_tensor,capturing,refused", [(0, 0, 0, True), (0, 1, 1, True), (0, 1, 0, False), (1, 0, 1, False), (1, 0, 0, True), (0, 0, 1, False)])
+def test_a_capture_is_looked_for_on_the_tensors_device(monkeypatch, current, of_tensor, capturing, refused):
+    """the stream that a call enqueues on is its tensors' device's, whichever device is the current one"""
+    from pytorch_tecogan_amd import sequence
+    now = [current]
+
+    class Device:
+        def __init__(self, dev):
+            self.index = dev.index
+
+        def __enter__(self):
+            self.before, now[0] = now[0], self.index
+
+        def __exit__(self, *a):
+            now[0] = self.before
+
+    monkeypatch.setattr(sequence, "_device", lambda: now[0])
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: now[0] == capturing)
+    x = torch.zeros(4, 64).as_subclass(OnDevice).requires_grad_()
+    x.index = of_tensor
+    if refused:
+        with pytest.raises(L.TecoganHipError, match="not captured"):
+            sequence._grad(x)
+    else:
+        assert sequence._grad(x)
+    assert now == [current]
+
+
 def test_names_are_public():
     """`from ops import *` (code/ops.py) re-exports every public name of the package's ops module"""
     from pytorch_tecogan_amd import sequence
