@@ -170,6 +170,13 @@ def test_a_capture_is_looked_for_on_the_tensors_device(monkeypatch, current, of_
     assert now == [current]
 
 
+def test_the_packed_descriptor_is_the_structure():
+    """sequence.py packs tg_la_desc as bytes; _lib.LaDesc says its layout field by field"""
+    from pytorch_tecogan_amd import sequence
+    d = L.LaDesc(3, 5, 8, 2, 24, 40, (1, 2, 3), (4, 5, 6), (7, 8, 1 << 40), 0.3)
+    assert sequence._DESC.pack(3, 5, 8, 2, 24, 40, 1, 2, 3, 4, 5, 6, 7, 8, 1 << 40, 0.3) == bytes(d)
+
+
 def test_names_are_public():
     """`from ops import *` (code/ops.py) re-exports every public name of the package's ops module"""
     from pytorch_tecogan_amd import sequence

@@ -873,6 +873,57 @@ def test_attention_output_off_16_bytes(dt):
             assert bool((room[:off // size] == 7).all()) and bool((room[off // size + B * T * H * DV:] == 7).all())
 
 
+@pytest.mark.parametrize("dt", [F32, BF16, F16])
+@pytest.mark.parametrize("T,D,units", [(1, 16, 16), (2, 16, 24), (1, 17, 16), (2, 17, 24), (40, 16, 40), (40, 64, 40), (40, 33, 40), (40, 128, 40)])
+def test_attention_states_are_fp32(T, D, units, dt):
+    """One term (two for T = 2) in each element of the last state and of the first one's gradient, with weights that no 16 bits hold: off by the power
+    (4 units of 2^-24), up to three more factors of it (5 each), the products and the parts' sums (8), the decay of the state (5) - not by the 64 units of
+    an operand in two bf16 parts."""
+    q, k, v, do, state, dstate, _ = attention_inputs(6, T, 4, 4, D, D, dt)
+    decay = -torch.tensor([0.3, 0.011, 0.17, 0.05], device=DEV)
+    if T > 2:
+        for t in (k, q):
+            one = t[:, T // 2].clone()
+            t.zero_()
+            t[:, T // 2] = one
+    for s, ds in ((state, dstate), (None, None)):
+        last = ops.linear_attention(q, k, v, decay, scale=0.25, state=s)[1]
+        first = ops.linear_attention_backward(do, q, k, v, decay, scale=0.25, state=torch.zeros_like(state) if s is None else s, dstate=ds)[3]
+        want, mag = attention_oracle(q, k, v, decay, 0.25, s, None, do, ds)
+        close(last, want["state"], F32, mag["state"], units, "state")
+        close(first, want["dstate"], F32, mag["dstate"], units, "dstate")
+
+
+def test_generator_published_vectors():
+    """Random123's known answers for ten rounds: the oracle at all zeros, all ones and the digits of pi; the kernel at all zeros, word by word - kept at
+    p = word / 2^32 and dropped at (word + 1) / 2^32"""
+    zeros = [0x6627e8d5, 0xe169c58d, 0xbc57ac4c, 0x9b00dbd8]
+    assert philox_block(0, 0) == zeros
+    assert philox_block((1 << 64) - 1, (1 << 64) - 1, 0xffffffff, 0xffffffff) == [0x408f276d, 0x41c83b0e, 0xa20bc7c6, 0x6d5451fd]
+    assert philox_block(0x85a308d3243f6a88, 0x299f31d0a4093822, 0x03707344, 0x13198a2e) == [0xd16cfe09, 0x94fdcceb, 0x5001e420, 0x24126ea1]
+    x, rng = torch.ones(4, device=DEV), ops.dropout_rng(0, DEV)
+    for i, word in enumerate(zeros):
+        assert float(ops.dropout(x, word / 2.0 ** 32, rng)[i]) != 0 and float(ops.dropout(x, (word + 1) / 2.0 ** 32, rng)[i]) == 0
+
+
+def test_the_same_tensor_twice():
+    """one tensor in several places of a call: its gradient is the sum over them"""
+    x, w, dy, ds = randn(5, 64, seed=1), randn(64, seed=2), randn(5, 64, seed=3), randn(5, 64, seed=4)
+    leaf = x.clone().requires_grad_()
+    y, s = ops.rms_norm(leaf, w, residual=leaf)
+    got, = torch.autograd.grad([y, s], [leaf], [dy, ds])
+    dx, _ = ops.rms_norm_backward(dy, x, ops.rms_norm(x, w, residual=x, stats=True)[2], w, residual=x, ds=ds)
+    assert torch.equal(got, 2 * dx)
+    rng = ops.dropout_rng(3, DEV)
+    got, = torch.autograd.grad(ops.dropout(leaf, 0.4, rng, residual=leaf), [leaf], dy)
+    assert torch.equal(got, ops.dropout_backward(dy, 0.4, rng) + dy)
+    q, _, _, do, _, _, decay = attention_inputs(2, 21, 3, 3, 16, 16, F32)
+    leaf = q.clone().requires_grad_()
+    got, = torch.autograd.grad(ops.linear_attention(leaf, leaf, leaf, decay)[0], [leaf], do)
+    dq, dk, dv, _ = ops.linear_attention_backward(do, q, q, q, decay)
+    close(got, dq.double() + dk.double() + dv.double(), F32, dq.double().abs() + dk.double().abs() + dv.double().abs(), 2, "dq + dk + dv")
+
+
 # ------------------------------------------------------------------------------------- streams, graphs, refusals, together
 def all_operators(x, w, rng, q, k, v, decay, state, out):
     """every operator once into the dict `out` (explicit forms, as a captured step calls them)"""
