@@ -596,7 +596,8 @@ int tg_dropout(int dtype, const void* x, const void* res, void* y, int64_t n, do
  * behind lengths[b] (clamped to 0 .. T) are not read, their rows of the outputs are zero and the last state is the one at the length.
  * state_in null: zeros.  tg_linear_attention_bwd: dstate_out null: zeros; dstate_in may be null.  scratch: *_scratch_floats floats (0: may
  * be null), this call's alone until it has run.  log_decay is a constant (no gradient).
- * tg_linear_attention_step: one token (strides of sequence and head; T and the token stride are not looked at), `state` updated in place. */
+ * tg_linear_attention_step: one token (strides of sequence and head), `state` updated in place.  T and the token strides have no meaning there, but
+ * have to be in range (T in 0 .. 2^30, strides 0 .. 2^31 - 1; 0 does). */
 typedef struct {
   int32_t B, T, H, HK, DK, DV;
   int64_t q_stride[3], k_stride[3], v_stride[3];   /* sequence, token, head */

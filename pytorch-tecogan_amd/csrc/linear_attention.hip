@@ -621,8 +621,8 @@ template <typename T, int MT, int CT, bool STATE> __global__ __launch_bounds__(2
 
 // How a chunk's rows reach a wave.  Where operands are aligned to 16 bytes and their channels fill 16-byte pieces, a wave reads whole rows, 16 bytes per
 // lane and neighbouring lanes side by side, into its own part of the LDS and takes the tiles from there.  (Tiles straight from memory -
-// 16 rows at a time, 8 bytes per lane - cost one L1 access per LANE: 54 per load instruction, and the L1s became the bound: 370 us
-// instead of 311 for 65536 sequences of 120 tokens, the more waves the worse.)  The next chunk's rows are on their way, in registers,
+// 16 rows at a time, 8 bytes per lane - cost one L1 access per LANE: 54 per load instruction, and the L1s became the bound: for 65536 sequences of
+// 120 tokens 370 us where the first staged form took 311, the more waves the worse.)  The next chunk's rows are on their way, in registers,
 // while this one is worked on.
 template <typename T, int MT, int CT, int NS = 1> struct Stage {
   static constexpr int kBytes = ElemTraits<T>::kBytes;
@@ -637,8 +637,10 @@ template <typename T, int MT, int CT, int NS = 1> struct Stage {
 
 // The staged form.  Addresses are a uniform pointer to the chunk's lowest token, which moves on by a constant, and every lane's own offset:
 // the loop holds no multiplication and no scalar load (with both, 187 scalar instructions and 7 loads stood beside 325 vector ones a chunk).
-// Measured: 65536 sequences of 120 tokens x 16 fp16 channels 224 - 233 us, 1.0 GB at 4.4 TB/s, bound by memory; two of 16384 tokens, 4 bf16 heads of
-// 64 channels: 23 us, the gradients 63 us, bound by issuing some 500 vector instructions a chunk at two waves per SIMD, with no registers for a third.
+// Measured: 65536 sequences of 120 tokens x 16 fp16 channels 247 - 260 us (269 under the profiler), 1.0 GB at 3.9 - 4.1 TB/s, bound by memory; two of
+// 16384 tokens, 4 bf16 heads of 64 channels: 25 us, the gradients 67 us, bound by issuing a chunk's vector instructions (splits, masks, the state's
+// factor) beside its 36 matrix ones at two waves per SIMD, with no registers for a third.  The four slices of such a head stage the same rows and compute
+// the same scores, each wave for itself.
 template <typename T, int MT, int CT, int NS, bool STATE> __global__ __launch_bounds__(256, 2) void la_kernel(LaArgs p) {
   typedef Mat<T> X;
   typedef Stage<T, MT, CT, NS> G;
@@ -647,7 +649,8 @@ template <typename T, int MT, int CT, int NS, bool STATE> __global__ __launch_bo
   constexpr int kBytes = ElemTraits<T>::kBytes;
   constexpr int C = 16 * CT;
   // Rows of less than 128 bytes: the cache lines hold other heads' rows as well, so the heads' waves load at the same time (65536 sequences of 120
-  // tokens x 16 channels: 236 us, 286 with each wave in its own time; wider rows only lose, 16384 tokens x 64 channels training 128 us, 136 so)
+  // tokens x 16 channels: 260 us, 310 with each wave in its own time; wider rows only lose, 2 x 16384 tokens x 64 channels 44 us and gradients 94, 47 and
+  // 102 so)
   constexpr bool kTogether = 16 * MT * kBytes < 128;
   constexpr f32x4 zero = {0.f, 0.f, 0.f, 0.f};
   extern __shared__ __align__(16) char lds[];           // [waves][kArea], then [2][waves][NS][CT][64] sums of 4 floats if a role folds
@@ -928,8 +931,8 @@ template <typename T, int MT, int CT, int NS, bool STATE> __global__ __launch_bo
 // Sequences of at most 16 tokens (a training clip's frames): the same arithmetic for ONE chunk, straight through.  A wave walks its sequences with
 // addresses that move on by a constant, the next one's rows on their way; what depends on the length is made again only where it changes.
 // (la_kernel's loops over segments and chunks cost more scalar instructions and branches here than the chunk itself: 39 us for the gradients
-// of 16384 sequences of 10 tokens x 16 channels, 23 us here.)  Forward 13.0 us, 38 MB at 2.9 TB/s (four sequences a wave: the launch and the decay's
-// powers are a third of it); 65536 sequences, 4 heads of 16 channels 149 us, 4.1 TB/s.
+// of 16384 sequences of 10 tokens x 16 channels, 23 us here, when both were built.)  Forward 13.5 us, 38 MB at 2.8 TB/s (four sequences a wave: the
+// launch and the decay's powers are a third of it); 65536 sequences, 4 heads of 16 channels, states in and out: 171 - 185 us, 872 MB at 4.7 - 5.1 TB/s.
 // Heads of up to 32 channels are held to the registers of four waves per SIMD, which they fit (4096 sequences of 10 tokens x 32 fp16 channels 34.3 us, 37.4
 // with 131 registers and three waves).
 template <typename T, int MT> __global__ __launch_bounds__(256, MT <= 2 ? 4 : 2) void la_short_kernel(LaArgs p) {
@@ -969,8 +972,8 @@ template <typename T, int MT> __global__ __launch_bounds__(256, MT <= 2 ? 4 : 2)
   const int piece = lane % G::kLanes * 16, piece_c = lane % kBytes * 16, row_a = lane / G::kLanes, row_c = lane / kBytes;
   const bool live_a = piece < M * kBytes && row_a < 16, live_c = slice * 16 * kBytes + piece_c < N * kBytes && row_c < 16;
   const int piece_r = live_a ? piece : 0, piece_rc = live_c ? piece_c : 0;   // (lanes without a piece bring another's again: see la_kernel)
-  constexpr bool kTogether = 16 * MT * kBytes < 128;   // (see la_kernel; 65536 sequences of 10 tokens, 4 heads of 16 channels: 149 us, 175 without.
-                                                       // The gradients in one pass have fewer waves and lose by it: 164 us, 160 without)
+  constexpr bool kTogether = 16 * MT * kBytes < 128;   // (see la_kernel; 65536 sequences of 10 tokens, 4 heads of 16 channels: 171 - 185 us, 216 without.
+                                                       // The gradients in one pass have fewer waves and lose by it: 417 us, 407 - 414 without)
   // lengths, and what goes by them: the lanes' places in a sequence, the weights in the state, the rows of out
   auto length = [&](int bi) { return p.lengths ? min(max(p.lengths[bi], 0), Tn) : Tn; };
   unsigned oa[G::kLoads], ob[G::kLoads], oc;
@@ -1173,9 +1176,9 @@ template <typename T, int MT> __global__ __launch_bounds__(256, MT <= 2 ? 4 : 2)
 }
 
 // The three gradients of such sequences in one pass: a wave brings q, k, v and do once instead of nine rows' worth for three roles, and takes one
-// slice of dq, dk and dv from them, tokens in their own order (23 us as three roles of la_short_kernel, 15.6 so, for 16384 sequences of 10 tokens x
-// 16 channels).  p.r[] are the roles of the general form.  Heads of up to 16 channels are held to the registers of four waves per SIMD, which they fit
-// (16384 sequences, 4 heads, bf16: forward and this 138 us, 173 with the 171 registers and two waves that the compiler takes by itself).
+// slice of dq, dk and dv from them, tokens in their own order (15.9 us for 16384 sequences of 10 tokens x 16 channels; as three roles of
+// la_short_kernel, when this was built, 23 where it took 15.6).  p.r[] are the roles of the general form.  Heads of up to 16 channels are held to the
+// registers of four waves per SIMD, which they fit (65536 sequences, bf16: 98 us, 133 with the 171 registers and two waves that the compiler takes by itself).
 template <typename T, int MT> __global__ __launch_bounds__(256, MT == 1 ? 4 : 2) void la_short_grad_kernel(LaArgs p) {
   typedef Mat<T> X;
   typedef Stage<T, MT, 1> G;
@@ -1503,7 +1506,8 @@ struct StepArgs {
 
 // One token.  What counts is the state: read once, written once.  LN lanes of a wave hold W floats each of a state row, so 64 / LN rows are
 // in one load; NB such loads are in flight.  WS waves share a state's rows (few states: the machine would wait for a handful of waves) and
-// add their parts of o through LDS.
+// add their parts of o through LDS.  8192 states of 64 x 64: 67 us, 268 MB at 4.0 TB/s; 2048 of 128 x 128: 97 us, 2.8 TB/s; rows that do not fill 16
+// bytes go one float a lane, 8192 of 64 x 63: 155 us, 1.7 TB/s (a wave brings no state while it works on another, see la_step_small_kernel).
 template <typename T, int W, int NB, int WS> __global__ __launch_bounds__(256) void la_step_kernel(StepArgs p) {
   __shared__ float part[WS == 1 ? 1 : 4][WS == 1 ? 1 : 128];
   static_assert(WS == 1 || WS == 4, "a workgroup's waves leave together");
@@ -1587,7 +1591,7 @@ template <typename T, int W, int NB, int WS> __global__ __launch_bounds__(256) v
 }
 
 // States of one load (16 x 16 floats and smaller, M <= 64 / LN): a wave walks them with the next one on its way.  (One state at a time and
-// wave, however many waves, moved 3.7 TB/s: 38 us for 65536 of 16 x 16; 25 us so, 5.6 TB/s.)
+// wave, however many waves, moved 3.7 TB/s: 38 us for 65536 of 16 x 16; 27 us so, 5.3 TB/s.)
 template <typename T> __global__ __launch_bounds__(256) void la_step_small_kernel(StepArgs p) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int LN = 1;
@@ -1649,10 +1653,11 @@ constexpr int kFold = 4;   // shared heads that are summed inside a workgroup; m
 inline int tiles(int m) { return m <= 16 ? 1 : m <= 32 ? 2 : m <= 64 ? 4 : 8; }
 
 // Segments: as many as two waves per SIMD need, each of at least kMinSegment tokens.  They cost an additional pass over b and c and two launches, about
-// what the whole sequence takes in 400 tokens of 16 bits or in 200 of fp32, and twice that where the machine is half full already: forward of two sequences,
-// 4 heads of 64, whole and in segments, bf16 300 tokens 17 us and 20, 700 tokens 30 and 19; fp32 200 tokens 25 and 19; of 20 sequences, bf16 700 tokens
-// 31 and 37, 1000 tokens 44 and 41; fp32 300 tokens 34 and 38, 520 tokens 53 and 46.  Two segments never bring anything (64 sequences of 2000 tokens,
-// fp32: 189 us whole and 215)
+// what the whole sequence takes in 400 tokens of 16 bits or in 200 of fp32, and twice that where the machine is half full already.  Forward (gradients) of
+// two sequences, 4 heads of 64, states in and out, whole and in segments: bf16 300 tokens 20 us and 17 (20 and 21), 700 tokens 36 and 20 (36 and 26); fp32
+// 200 tokens 26 and 18 (26 and 20); of 20 sequences: bf16 700 tokens 37 and 42 (41 and 50), 1000 tokens 51 and 45 (54 and 61); fp32 300 tokens 35 and 40 (39 and
+// 51), 520 tokens 56 and 48 (58 and 69: the gradients' three roles leave room for two segments).  Two segments never bring anything (64 sequences of 2000
+// tokens, fp32: 191 us whole and 214)
 constexpr int64_t kWaves = 2048;
 constexpr int kMinSegment = 32;
 constexpr int kCUs = 256;
@@ -1713,8 +1718,8 @@ template <typename T, int MT> int go_short(const LaArgs& a, dim3 grid, int threa
   return go(la_short_kernel<T, MT>, resident, Stage<T, MT, 1>::kArea, 1, a.group > 1, a, grid, threads, st);
 }
 // Slices of 32 columns share a chunk's scores, its rows and the columns of b between two of 16: worth it where half the waves still fill the
-// machine (128 sequences of 2000 tokens, 4 bf16 heads of 64: 151 us, 194 in slices of 16; gradients 408 us, 642), not where sequences are cut
-// into segments for want of waves (20 such sequences: 70 us, 53 in slices of 16; gradients 89 us, 81).  For heads wider than 16 channels beside
+// machine (128 sequences of 2000 tokens, 4 bf16 heads of 64: 145 - 152 us, 177 in slices of 16; gradients 418 us, 671), not where sequences are cut
+// into segments for want of waves (20 such sequences: 79 us, 59 in slices of 16; gradients 101 us, 95).  For heads wider than 16 channels beside
 // operands of 17 .. 64 in 16 bits; fp32 and 128 channels do not fit the registers so
 constexpr int64_t kWideWaves = 512;
 inline bool can_be_wide(int dtype, int M, int N) { return dtype != TG_F32 && N > 16 && (tiles(M) == 2 || tiles(M) == 4); }

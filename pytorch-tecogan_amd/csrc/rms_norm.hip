@@ -13,8 +13,8 @@
 // the sum instead of 1e-7, for one operand less to read).  dw: every workgroup adds the rows it walks in registers and writes one partial row,
 // a second launch adds those in index order - no atomics, the same bits every time.
 //
-// Bound by memory once the rows are many: 655360 bf16 rows of 64 with a residual to e4m3 56 us, 296 MB at 5.3 TB/s; 40960 rows 6.6 us forward (3.3 us
-// is an empty machine's start and end), gradient 6.9 + 2.6.
+// Bound by memory once the rows are many: 655360 bf16 rows of 64 with a residual to e4m3 58 us, 296 MB at 5.1 TB/s; 40960 rows 6.6 us forward (3.2 us
+// is an empty machine's start and end), gradient 6.7 + 2.6.
 #include "common.h"
 
 namespace {

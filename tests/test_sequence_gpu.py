@@ -3,9 +3,9 @@
 
 Tolerances, from the arithmetic: a stored result is off by half a step of its type (HALF, relative to the value; fp16 also by half its
 smallest step, 2^-25).  Sums in fp32 are off by at most (number of additions one after the other) x 2^-24 of the sum of the terms'
-magnitudes; the operators add at most ADDS in a row before they join partial sums in a tree.  linear_attention additionally splits scores and
-states into two bf16 halves beside 16-bit inputs: 2^-16 of the magnitudes for each split on the way of a term (at most 4: weight, state, fp16's
-own two halves)."""
+magnitudes; the operators add at most ADDS in a row before they join partial sums in a tree.  The bounds of linear_attention's random cases leave
+room for scores and states of two bf16 halves beside 16-bit inputs: 2^-16 of the magnitudes for each split on the way of a term (at most 4: weight,
+state, fp16's own two halves); the cases of whole numbers and of single terms hold them to fp32's 24 bits."""
 import ctypes as C
 import math
 import os
