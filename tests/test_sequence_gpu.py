@@ -924,6 +924,52 @@ def test_the_same_tensor_twice():
     close(got, dq.double() + dk.double() + dv.double(), F32, dq.double().abs() + dk.double().abs() + dv.double().abs(), 2, "dq + dk + dv")
 
 
+@pytest.mark.parametrize("dt", [F32, BF16])
+def test_attention_growing_memories(dt):
+    """log_decay above zero: powers that grow, in one chunk, in several and across segments"""
+    for T, D in ((9, 16), (40, 32), (70, 33), (900, 64)):
+        q, k, v, do, state, dstate, _ = attention_inputs(1, T, 3, 3, D, D, dt, seed=T)
+        decay = torch.tensor([0.3, 0.02, 1e-4], device=DEV) * min(1.0, 40 / T)
+        o, last = ops.linear_attention(q, k, v, decay, state=state)
+        got = ops.linear_attention_backward(do, q, k, v, decay, state=state, dstate=dstate)
+        want, mag = attention_oracle(q, k, v, decay, D ** -0.5, state, None, do, dstate)
+        for name, g, t in zip(("o", "state", "dq", "dk", "dv", "dstate"), (o, last, *got), (dt, F32, dt, dt, dt, F32)):
+            close(g, want[name], t, mag[name], attention_units(dt, T, D), name)
+
+
+@pytest.mark.parametrize("D", [64, 63])
+def test_attention_past_32_bit_offsets(D):
+    """4194344 tokens of 8 heads: 4.3 GB an operand.  The memory is gone after 400 tokens (e^-80), so the first and the last 200 are those of windows of 600"""
+    T, H = (1 << 22) + 40, 8
+    g = torch.Generator(device=DEV).manual_seed(1)
+    q, k, v, do = (torch.randn(1, T, h, D, dtype=BF16, device=DEV, generator=g) for h in (H, 1, 1, H))
+    decay = torch.linspace(-0.2, -0.6, H, device=DEV)
+    o, last = ops.linear_attention(q, k, v, decay)
+    dq, dk, dv, _ = ops.linear_attention_backward(do, q, k, v, decay)
+    for lo, rows in ((0, slice(0, 200)), (T - 600, slice(400, 600))):
+        cut = lambda t: t[:, lo:lo + 600]   # noqa: E731
+        want, mag = attention_oracle(cut(q), cut(k), cut(v), decay, D ** -0.5, None, None, cut(do))
+        for name, t in (("o", o), ("dq", dq), ("dk", dk), ("dv", dv)):
+            close(cut(t)[:, rows], want[name][:, rows], BF16, mag[name][:, rows], attention_units(BF16, 600, D) * H, name)
+        if lo:
+            close(last, want["state"], F32, mag["state"], attention_units(BF16, 600, D), "state")
+
+
+def test_rms_norm_past_32_bit_offsets():
+    """33554435 rows of 64 and 65537 of 32772 (4.3 GB each): the last rows have the bits that they have alone"""
+    for rows, channels in (((1 << 25) + 3, 64), ((1 << 16) + 1, (1 << 15) + 4)):
+        x = torch.randn(rows, channels, dtype=BF16, device=DEV, generator=torch.Generator(device=DEV).manual_seed(2))
+        y, rstd = ops.rms_norm(x, stats=True)
+        dx, _ = ops.rms_norm_backward(x, x, rstd, dweight=False)
+        q, scale = ops.rms_norm_e4m3(x)
+        end = x[-5:].clone()
+        y1, r1 = ops.rms_norm(end, stats=True)
+        q1, s1 = ops.rms_norm_e4m3(end)
+        assert torch.equal(y[-5:], y1) and torch.equal(rstd[-5:], r1) and torch.equal(q[-5:].float(), q1.float()) and torch.equal(scale[-5:], s1)
+        assert torch.equal(dx[-5:], ops.rms_norm_backward(end, end, r1, dweight=False)[0])
+        del x, y, dx, q
+
+
 # ------------------------------------------------------------------------------------- streams, graphs, refusals, together
 def all_operators(x, w, rng, q, k, v, decay, state, out):
     """every operator once into the dict `out` (explicit forms, as a captured step calls them)"""
