@@ -4,9 +4,10 @@ the reference's code/ops.py:45-88 and have no counterpart there.
 
 Each operator takes device tensors (fp32, bf16 or fp16), enqueues its HIP kernels on the current stream of the tensors' device and
 allocates its outputs and workspaces like any torch operation; nothing synchronises.  Where an input requires a gradient the result
-carries one (first order, reverse mode; dual tensors of forward mode are refused).  The explicit forms - `stats=True` and the `*_backward` functions - are what a captured step uses: autograd
-itself is not captured (a backward pass recorded while an eager graph of the same leaves lives ends the process), so inside a capture a
-call that would build an autograd graph raises; use torch.no_grad() there, or the explicit forms on detached tensors."""
+carries one (first order, reverse mode; dual tensors of forward mode are refused).  The explicit forms - `stats=True` and the `*_backward`
+functions - are what a captured step uses: autograd itself is not captured (a backward pass recorded while an eager graph of the same leaves
+lives ends the process), so inside a capture a call that would build an autograd graph raises; use torch.no_grad() there, or the explicit
+forms on detached tensors."""
 import struct
 
 import torch
